@@ -70,7 +70,8 @@ const char* whirl_last_error(void);
 int whirl_version(void);
 
 /* Kernel launches this process has made through the library so far, per family: [0] greedy picks, [1] multi-pass
- * selection, [2] single-pass sampler, [3] small helper kernels.  Fills min(n, 4) entries.  (The reference logs launches
+ * selection, [2] single-pass sampler, [3] small helper kernels, [4] log-probabilities and losses, [5] block tables.  Fills
+ * min(n, 6) entries.  (The reference logs launches
  * with WHIRL_LAUNCH_LOG, src/hip/launch_log.h.) */
 void whirl_launch_counts(uint64_t* out, int n);
 
@@ -322,6 +323,153 @@ size_t whirl_spec_workspace_bytes(int seqs, int L);
 int whirl_spec_accept_residual(const void* target, const void* draft, int dtype, int seqs, int L, int n, const int* draft_tok,
                                const float* inv_t, const double* u_acc, const double* u_res, int* n_acc, int* next_tok, void* ws,
                                size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------------------------------
+ * Training on sampled tokens: log-probabilities, losses and their gradients down to the logits.  No counterpart in the
+ * reference, which only serves.
+ *
+ * Logits are rows [rows][n] whose row r starts at x + r * ld elements (ld >= n; a padded vocabulary leaves a gap), f32 or bf16,
+ * aligned to their own size; rows aligned to 16 bytes are the fast case.  With z = x * inv_t (inv_t > 0: the scalar, or
+ * inv_t_rows[row] where that is given):
+ *     max = max_j x_j,  sum = sum_j exp((x_j - max) * inv_t)          (stats [rows][2], the convention of whirl_sample_rows)
+ *     p_j = exp((x_j - max) * inv_t) / sum,  logp = log p[token],  H = - sum_j p_j log p_j   (an entry of p = 0 adds nothing)
+ * Entries may be -inf or the type's lowest value (forbidden tokens: p = 0, gradient 0).  A row that holds a NaN or +inf, or
+ * -inf alone, has no distribution: its outputs and its gradient are NaN.
+ * A row COUNTS when its token lies in [0, n), its weight (where the call has weights) is > 0 and, where sequences matter, it
+ * lies inside one.  Rows that do not count are not read: their outputs and statistics are 0, and so is their row of dx.
+ * dx has the type of x, rows ld_dx apart; it may be x itself (with the same ld), and must not overlap x in another way.
+ * Sums run in a fixed order: the same call gives the same bits.
+ * ---------------------------------------------------------------------------------------------------------------- */
+
+/* logp [rows], stats [rows][2] and entropy [rows] of the given tokens; any of the three outputs may be null. */
+int whirl_token_logprobs(const void* x, int dtype, int rows, int n, int64_t ld, const int32_t* token, float inv_t,
+                         const float* inv_t_rows, float* logp, float* stats, float* entropy, void* stream);
+
+/* The gradient of a loss L of those outputs: dx_j = inv_t * (g * ([j == token] - p_j) - h * p_j * (log p_j + H)), with
+ * g = g_logp[row] = dL/dlogp and h = g_entropy[row] = dL/dH (null: 0; needs entropy, the forward call's).  stats: the forward
+ * call's, or what whirl_sample_rows / whirl_topk_rows wrote for the same rows at the same inv_t (without penalties).  A row
+ * with g = h = 0 is not read and gets zeros. */
+int whirl_token_logprobs_grad(const void* x, int dtype, int rows, int n, int64_t ld, const int32_t* token, float inv_t,
+                              const float* inv_t_rows, const float* stats, const float* entropy, const float* g_logp,
+                              const float* g_entropy, void* dx, int64_t ld_dx, void* stream);
+
+/* Bytes of workspace of the two losses below (0 <= rows, seqs). */
+size_t whirl_loss_workspace_bytes(int rows, int seqs);
+
+/* how a loss weighs its rows: s_row = w, w / (sum of w), or w / (sum of w over the row's sequence) / (sequences whose sum is
+ * > 0).  The sums run over the rows that count; a sum of 0 leaves s = 0. */
+enum { WHIRL_MEAN_SUM = 0, WHIRL_MEAN_TOKENS = 1, WHIRL_MEAN_SEQS = 2 };
+
+/* The clipped policy loss with a KL term, from the logits, and its gradient in the same pass.  Per row that counts:
+ *     d = clamp(logp - old_logp, -20, 20), r = exp(d);  pg = -min(r * adv, clamp(r, 1 - clip_low, 1 + clip_high) * adv);
+ *     where dual_clip > 0 and adv < 0: pg = min(pg, -dual_clip * adv)
+ *     k = clamp(ref_logp - logp, -20, 20), kl = exp(k) - k - 1
+ *     row_loss = pg + kl_coef * kl - ent_coef * H;   loss = sum of s * row_loss
+ * The gradient is 0 through a clip or clamp that binds.  old_logp null: the policy that sampled is the present one (r = 1,
+ * gradient -adv).  ref_logp null: no KL term. */
+typedef struct whirl_policy_params {
+    const int32_t* token;      /* [rows] */
+    const float* adv;          /* [rows] advantages */
+    const float* old_logp;     /* [rows] (null) */
+    const float* ref_logp;     /* [rows] (null) */
+    const float* weight;       /* [rows] (null = 1) */
+    const int32_t* seq_start;  /* [seqs + 1] first row of every sequence, not decreasing, and the end of the last: WHIRL_MEAN_SEQS */
+    int32_t seqs;
+    int32_t mean;              /* WHIRL_MEAN_* */
+    const float* inv_t_rows;   /* [rows] (null = inv_t) */
+    float inv_t, clip_low, clip_high, dual_clip, kl_coef, ent_coef;
+} whirl_policy_params;
+typedef struct whirl_policy_out { /* only loss is required */
+    float* loss;      /* [1] */
+    float* logp;      /* [rows] */
+    float* stats;     /* [rows][2] */
+    float* entropy;   /* [rows] */
+    float* kl;        /* [rows] */
+    float* row_loss;  /* [rows] */
+    float* g_logp;    /* [rows] d loss / d logp (the entropy's part is -ent_coef * s, not in here) */
+    float* row_scale; /* [rows] s */
+    void* dx;         /* d loss / d x (null: no gradient wanted) */
+    int64_t ld_dx;
+} whirl_policy_out;
+int whirl_policy_loss(const void* x, int dtype, int rows, int n, int64_t ld, const whirl_policy_params* params,
+                      const whirl_policy_out* out, void* ws, size_t ws_bytes, void* stream);
+
+/* A preference loss over pairs of sequences: sequence 2 i is the chosen one of pair i, 2 i + 1 the rejected one, and sequence s
+ * holds the rows seq_start[s] .. seq_start[s + 1).  With P_s = sum of w * (logp - ref_logp) over the rows of s that count
+ * (divided by the sum of their w with average != 0; 0 for a sequence without such rows):
+ *     h = beta * (P_chosen - P_rejected) - margin
+ *     WHIRL_PREF_SIGMOID  -(1 - smoothing) * log sigmoid(h) - smoothing * log sigmoid(-h)
+ *     WHIRL_PREF_HINGE    max(0, 1 - h)
+ *     WHIRL_PREF_SQUARED  ((h - 1/2) / beta)^2
+ * loss = the mean over the pairs (0 without pairs); reward [pairs][2] = beta * P.  ref_logp null: 0. */
+enum { WHIRL_PREF_SIGMOID = 0, WHIRL_PREF_HINGE = 1, WHIRL_PREF_SQUARED = 2 };
+typedef struct whirl_preference_params {
+    const int32_t* token;      /* [rows] */
+    const int32_t* seq_start;  /* [2 * pairs + 1], not decreasing */
+    const float* ref_logp;     /* [rows] (null) */
+    const float* weight;       /* [rows] (null = 1) */
+    const float* inv_t_rows;   /* [rows] (null = inv_t) */
+    int32_t pairs;
+    int32_t kind;              /* WHIRL_PREF_* */
+    int32_t average;
+    float inv_t, beta, smoothing, margin;
+} whirl_preference_params;
+typedef struct whirl_preference_out { /* only loss is required */
+    float* loss;      /* [1] */
+    float* pair_loss; /* [pairs] */
+    float* reward;    /* [pairs][2] */
+    float* logp;      /* [rows] */
+    float* stats;     /* [rows][2] */
+    float* g_logp;    /* [rows] */
+    void* dx;         /* (null: no gradient wanted) */
+    int64_t ld_dx;
+} whirl_preference_out;
+int whirl_preference_loss(const void* x, int dtype, int rows, int n, int64_t ld, const whirl_preference_params* params,
+                          const whirl_preference_out* out, void* ws, size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------------------------------
+ * The rows of the next step: cache block tables and slot maps from the sequences' lengths, on the device.  It closes the loop
+ * of whirl_accept_rows, whose acc decides how many tokens a sequence keeps and whose row0 this call makes, without a
+ * read-back.  No counterpart in the reference (one sequence batch, contiguous caches).
+ *
+ * A cache holds num_blocks blocks of block_size token slots; token p of sequence s lies in block table[s][p / block_size], slot
+ * table[s][p / block_size] * block_size + p % block_size.  owned[s] entries of table[s] are in use; the free blocks are the
+ * stack free_ids[0 .. free_count).  A block belongs to one sequence at a time (no sharing of prefixes).
+ *
+ * whirl_block_tables_step: sequence s holds length[s] tokens and gets n_new[s] more in this step (a finished one: length 0,
+ * n_new 0).  It then needs target = ceil((length + n_new) / block_size) blocks:
+ *   status[s] = WHIRL_SEQ_INVALID  length or n_new negative, their sum above INT32_MAX, or target above max_blocks;
+ *               WHIRL_SEQ_REFUSED  n_new > 0 and the n_new of the valid sequences up to it pass max_rows; or it needs blocks
+ *                                  and the needs of the sequences up to it pass the blocks at hand (nobody overtakes);
+ *               WHIRL_SEQ_OK       else.
+ * The blocks at hand are the free ones and those that this step gives back: a sequence inside max_rows that owns more than its target
+ * gives back table[s][target .. owned), pushed on the stack in the sequences' order.  New blocks come from the stack's top, in
+ * the sequences' order.  An OK sequence owns its target afterwards; any other keeps its blocks and length and gets no rows.
+ * Entries of table behind owned and of free_ids behind free_count are left as they were.
+ * Rows: row0[s] = the first row of sequence s, row0[seqs] = their number; row r of sequence s at position p = length[s] + r -
+ * row0[s] gets slot[r], position[r] = p and seq[r] = s.  The rows from row0[seqs] to max_rows (a padded batch) get slot -1,
+ * position 0, seq -1.
+ * ---------------------------------------------------------------------------------------------------------------- */
+enum { WHIRL_SEQ_OK = 0, WHIRL_SEQ_REFUSED = 1, WHIRL_SEQ_INVALID = 2 };
+#define WHIRL_MAX_SEQS 65536
+typedef struct whirl_block_tables {
+    int32_t* table;      /* [seqs][max_blocks] */
+    int32_t* owned;      /* [seqs] */
+    int32_t* free_ids;   /* [num_blocks] */
+    int32_t* free_count; /* [1] */
+    int32_t seqs, max_blocks, num_blocks, block_size; /* seqs <= WHIRL_MAX_SEQS */
+} whirl_block_tables;
+typedef struct whirl_step_rows {
+    int64_t* slot;     /* [max_rows] */
+    int32_t* position; /* [max_rows] (may be null) */
+    int32_t* seq;      /* [max_rows] (may be null) */
+    int32_t* row0;     /* [seqs + 1] */
+    int32_t* status;   /* [seqs] */
+    int32_t max_rows;
+} whirl_step_rows;
+size_t whirl_block_workspace_bytes(int seqs);
+int whirl_block_tables_step(const int32_t* length, const int32_t* n_new, const whirl_block_tables* tables, const whirl_step_rows* rows,
+                            void* ws, size_t ws_bytes, void* stream);
 
 /* ---- draw generators ------------------------------------------------------------------------------------------------
  * The reference draws one uniform per sampled row on the host, Sampler::uniform(seed, pos) (src/sampling/sampler.h:46-52,

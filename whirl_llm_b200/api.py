@@ -58,12 +58,45 @@ class SampleOut(C.Structure):
                 ("counters", C.c_void_p)]
 
 
+class PolicyParams(C.Structure):
+    _fields_ = [("token", C.c_void_p), ("adv", C.c_void_p), ("old_logp", C.c_void_p), ("ref_logp", C.c_void_p), ("weight", C.c_void_p),
+                ("seq_start", C.c_void_p), ("seqs", C.c_int32), ("mean", C.c_int32), ("inv_t_rows", C.c_void_p), ("inv_t", C.c_float),
+                ("clip_low", C.c_float), ("clip_high", C.c_float), ("dual_clip", C.c_float), ("kl_coef", C.c_float),
+                ("ent_coef", C.c_float)]
+
+
+class PolicyOut(C.Structure):
+    _fields_ = [("loss", C.c_void_p), ("logp", C.c_void_p), ("stats", C.c_void_p), ("entropy", C.c_void_p), ("kl", C.c_void_p),
+                ("row_loss", C.c_void_p), ("g_logp", C.c_void_p), ("row_scale", C.c_void_p), ("dx", C.c_void_p), ("ld_dx", C.c_int64)]
+
+
+class PreferenceParams(C.Structure):
+    _fields_ = [("token", C.c_void_p), ("seq_start", C.c_void_p), ("ref_logp", C.c_void_p), ("weight", C.c_void_p),
+                ("inv_t_rows", C.c_void_p), ("pairs", C.c_int32), ("kind", C.c_int32), ("average", C.c_int32), ("inv_t", C.c_float),
+                ("beta", C.c_float), ("smoothing", C.c_float), ("margin", C.c_float)]
+
+
+class PreferenceOut(C.Structure):
+    _fields_ = [("loss", C.c_void_p), ("pair_loss", C.c_void_p), ("reward", C.c_void_p), ("logp", C.c_void_p), ("stats", C.c_void_p),
+                ("g_logp", C.c_void_p), ("dx", C.c_void_p), ("ld_dx", C.c_int64)]
+
+
+class BlockTables(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("owned", C.c_void_p), ("free_ids", C.c_void_p), ("free_count", C.c_void_p), ("seqs", C.c_int32),
+                ("max_blocks", C.c_int32), ("num_blocks", C.c_int32), ("block_size", C.c_int32)]
+
+
+class StepRowsOut(C.Structure):
+    _fields_ = [("slot", C.c_void_p), ("position", C.c_void_p), ("seq", C.c_void_p), ("row0", C.c_void_p), ("status", C.c_void_p),
+                ("max_rows", C.c_int32)]
+
+
 def _load() -> C.CDLL:
     if not os.path.exists(LIB_PATH):
         raise ImportError(f"{LIB_PATH} is missing: build it with `python -m whirl_llm_b200.build` "
                           "(there is no fallback implementation)")
     lib = C.CDLL(LIB_PATH)
-    vp, i, f, sz = C.c_void_p, C.c_int, C.c_float, C.c_size_t
+    vp, i, f, sz, i64 = C.c_void_p, C.c_int, C.c_float, C.c_size_t, C.c_int64
     sigs = {
         "whirl_status_string": (C.c_char_p, [i]),
         "whirl_last_error": (C.c_char_p, []),
@@ -98,6 +131,13 @@ def _load() -> C.CDLL:
         "whirl_uniform_philox4x32": (C.c_double, [C.c_uint64, C.c_uint64, C.c_uint32, C.c_uint32]),
         "whirl_fill_draws": (i, [vp, vp, i, i, C.c_uint32, vp, vp, vp]),
         "whirl_test_waits": (None, [C.c_uint32, i]),
+        "whirl_token_logprobs": (i, [vp, i, i, i, i64, vp, f, vp, vp, vp, vp, vp]),
+        "whirl_token_logprobs_grad": (i, [vp, i, i, i, i64, vp, f, vp, vp, vp, vp, vp, vp, i64, vp]),
+        "whirl_loss_workspace_bytes": (sz, [i, i]),
+        "whirl_policy_loss": (i, [vp, i, i, i, i64, C.POINTER(PolicyParams), C.POINTER(PolicyOut), vp, sz, vp]),
+        "whirl_preference_loss": (i, [vp, i, i, i, i64, C.POINTER(PreferenceParams), C.POINTER(PreferenceOut), vp, sz, vp]),
+        "whirl_block_workspace_bytes": (sz, [i]),
+        "whirl_block_tables_step": (i, [vp, vp, C.POINTER(BlockTables), C.POINTER(StepRowsOut), vp, sz, vp]),
     }
     for name, (res, args) in sigs.items():
         fn = getattr(lib, name)
@@ -111,7 +151,9 @@ DECLARED = ["whirl_status_string", "whirl_last_error", "whirl_version", "whirl_w
             "whirl_spec_accept_residual",
             "whirl_topk_rows", "whirl_topk_rows_shard", "whirl_merge_sample_rows", "whirl_sample_rows", "whirl_sample_rows_host", "whirl_host_release", "whirl_host_last_error",
             "whirl_launch_counts", "whirl_check", "whirl_shard_block_words", "whirl_merge_sample_rows_packed", "whirl_test_waits", "whirl_accept_rows",
-            "whirl_uniform_splitmix", "whirl_race_base", "whirl_philox4x32_10", "whirl_uniform_philox4x32", "whirl_fill_draws"]
+            "whirl_uniform_splitmix", "whirl_race_base", "whirl_philox4x32_10", "whirl_uniform_philox4x32", "whirl_fill_draws",
+            "whirl_token_logprobs", "whirl_token_logprobs_grad", "whirl_loss_workspace_bytes", "whirl_policy_loss", "whirl_preference_loss",
+            "whirl_block_workspace_bytes", "whirl_block_tables_step"]
 
 
 def _check(status: int):
@@ -394,9 +436,9 @@ def fill_draws(seed: torch.Tensor, pos_idx: torch.Tensor, generator: int = GEN_S
 
 def launch_counts() -> dict:
     """Kernel launches made through the library by this process so far, per family."""
-    a = (C.c_uint64 * 4)()
-    lib.whirl_launch_counts(a, 4)
-    return dict(rowscan=a[0], select_generic=a[1], single_pass=a[2], aux=a[3])
+    a = (C.c_uint64 * 6)()
+    lib.whirl_launch_counts(a, 6)
+    return dict(rowscan=a[0], select_generic=a[1], single_pass=a[2], aux=a[3], loss=a[4], blocks=a[5])
 
 
 def sample_rows_host(x_host, params: dict, rows: int, n: int, dtype: int, out: dict, kept_cap: int = 0, device: int = 0):
@@ -512,3 +554,199 @@ def spec_accept_residual(target, draft, draft_tok, inv_t, u_acc, u_res):
                                           u_res.data_ptr(), n_acc.data_ptr(), nxt.data_ptr(), ws.data_ptr(), ws.numel(),
                                           torch.cuda.current_stream(dev).cuda_stream))
     return n_acc, nxt
+
+
+# ---- training on sampled tokens -------------------------------------------------------------------------------------------
+
+MEAN_SUM, MEAN_TOKENS, MEAN_SEQS = 0, 1, 2
+PREF_SIGMOID, PREF_HINGE, PREF_SQUARED = 0, 1, 2
+
+
+def _loss_rows(x: torch.Tensor):
+    """Logits [rows, n] whose rows may lie further apart than n (a padded vocabulary): (dtype, rows, n, ld)."""
+    if not x.is_cuda:
+        raise ValueError("logits must be on a CUDA device (this library has no CPU path)")
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"logits must be [rows, n], got {tuple(x.shape)}")
+    rows, n = x.shape
+    s0, s1 = x.stride()
+    if (n > 1 and s1 != 1) or (rows > 1 and s0 < n):
+        raise ValueError(f"logits must be rows of consecutive elements that do not overlap, got strides {(s0, s1)}")
+    return _dtype(x), rows, n, (s0 if rows > 1 else n)
+
+
+def _vec(t: Optional[torch.Tensor], name: str, dtype, shape, x: torch.Tensor):
+    """The address of a contiguous tensor of the given type and shape on x's device (None stays None)."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.device != x.device or t.shape != shape or not t.is_contiguous():
+        raise TypeError(f"{name}: want a contiguous {dtype} tensor of shape {tuple(shape)} on {x.device}, got {t.dtype} {tuple(t.shape)} "
+                        f"on {t.device}")
+    return t.data_ptr()
+
+
+def _grad_out(x: torch.Tensor, dx: Optional[torch.Tensor], ld: int) -> torch.Tensor:
+    """dx, checked; a new one has x's row pitch."""
+    if dx is None:
+        rows, n = x.shape
+        return torch.empty((rows, ld), dtype=x.dtype, device=x.device)[:, :n] if ld != n else torch.empty((rows, n), dtype=x.dtype, device=x.device)
+    if dx.dtype != x.dtype or dx.device != x.device or dx.shape != x.shape:
+        raise TypeError(f"dx: want {x.dtype} {tuple(x.shape)} on {x.device}, got {dx.dtype} {tuple(dx.shape)} on {dx.device}")
+    return dx
+
+
+def _call(x: torch.Tensor, fn, *args):
+    """fn(*args, stream) with x's device current."""
+    if x.device.index == torch.cuda.current_device():
+        _check(fn(*args, torch.cuda.current_stream(x.device).cuda_stream))
+    else:
+        with torch.cuda.device(x.device):
+            _check(fn(*args, torch.cuda.current_stream(x.device).cuda_stream))
+
+
+@dataclass
+class LogprobResult:
+    logp: torch.Tensor                # [rows] float32
+    stats: torch.Tensor               # [rows, 2] float32: max, sum exp((x - max) * inv_t)
+    entropy: Optional[torch.Tensor]   # [rows] float32
+
+
+def token_logprobs(x, token, inv_t: float = 1.0, inv_t_rows=None, want_entropy: bool = False) -> LogprobResult:
+    """Log-probability of token[r] under row r of the logits, the row's softmax statistics, and its entropy
+    (whirl_token_logprobs).  x [rows, n] float32 / bfloat16, rows may be padded; token [rows] int32.  A row whose token lies
+    outside [0, n) is not read and gets zeros."""
+    dt, rows, n, ld = _loss_rows(x)
+    f32, rs = torch.float32, (rows,)
+    tok, it = _vec(token, "token", torch.int32, rs, x), _vec(inv_t_rows, "inv_t_rows", f32, rs, x)
+    logp = torch.empty(rows, dtype=f32, device=x.device)
+    stats = torch.empty((rows, 2), dtype=f32, device=x.device)
+    entropy = torch.empty(rows, dtype=f32, device=x.device) if want_entropy else None
+    _call(x, lib.whirl_token_logprobs, x.data_ptr(), dt, rows, n, ld, tok, inv_t, it, logp.data_ptr(), stats.data_ptr(), _p(entropy))
+    return LogprobResult(logp, stats, entropy)
+
+
+def token_logprobs_grad(x, token, stats, g_logp, inv_t: float = 1.0, inv_t_rows=None, entropy=None, g_entropy=None, dx=None) -> torch.Tensor:
+    """The gradient by the logits of a loss whose gradients by logp and (optionally) entropy are g_logp and g_entropy [rows]
+    float32 (whirl_token_logprobs_grad).  stats, entropy: what token_logprobs returned.  dx may be x itself."""
+    dt, rows, n, ld = _loss_rows(x)
+    f32, rs = torch.float32, (rows,)
+    args = (_vec(token, "token", torch.int32, rs, x), inv_t, _vec(inv_t_rows, "inv_t_rows", f32, rs, x), _vec(stats, "stats", f32, (rows, 2), x),
+            _vec(entropy, "entropy", f32, rs, x), _vec(g_logp, "g_logp", f32, rs, x), _vec(g_entropy, "g_entropy", f32, rs, x))
+    dx = _grad_out(x, dx, ld)
+    _call(x, lib.whirl_token_logprobs_grad, x.data_ptr(), dt, rows, n, ld, *args, dx.data_ptr(), _loss_rows(dx)[3])
+    return dx
+
+
+@dataclass
+class PolicyResult:
+    loss: torch.Tensor                # [] float32
+    logp: torch.Tensor                # [rows] float32, and so on
+    stats: torch.Tensor               # [rows, 2]
+    entropy: Optional[torch.Tensor]   # (with ent_coef or want_entropy)
+    kl: Optional[torch.Tensor]        # (with ref_logp)
+    row_loss: torch.Tensor
+    g_logp: torch.Tensor              # d loss / d logp
+    row_scale: torch.Tensor           # a row's share of the loss; the entropy's gradient is -ent_coef * row_scale
+    dx: Optional[torch.Tensor]        # d loss / d x
+
+
+def policy_loss(x, token, adv, old_logp=None, ref_logp=None, weight=None, seq_start=None, inv_t: float = 1.0, inv_t_rows=None,
+                clip_low: float = 0.2, clip_high: float = 0.2, dual_clip: float = 0.0, kl_coef: float = 0.0, ent_coef: float = 0.0,
+                mean: int = MEAN_TOKENS, want_grad: bool = True, want_entropy: bool = False, dx=None) -> PolicyResult:
+    """The clipped policy loss with a KL term on logits x [rows, n] and the tokens sampled from them, with its gradient by the
+    logits (whirl_policy_loss).  adv, old_logp, ref_logp, weight: [rows] float32 (weight 0: a prompt or padding row, not read);
+    seq_start: [seqs + 1] int32, needed by MEAN_SEQS.  dx may be x itself."""
+    dt, rows, n, ld = _loss_rows(x)
+    f32, i32, rs, dev = torch.float32, torch.int32, (rows,), x.device
+    if mean == MEAN_SEQS and (seq_start is None or seq_start.dim() != 1 or seq_start.numel() < 1):
+        raise ValueError("policy_loss: MEAN_SEQS needs seq_start [seqs + 1]")
+    seqs = 0 if seq_start is None else seq_start.numel() - 1
+    p = PolicyParams(_vec(token, "token", i32, rs, x), _vec(adv, "adv", f32, rs, x), _vec(old_logp, "old_logp", f32, rs, x),
+                     _vec(ref_logp, "ref_logp", f32, rs, x), _vec(weight, "weight", f32, rs, x),
+                     None if seq_start is None else _vec(seq_start, "seq_start", i32, (seqs + 1,), x), seqs, mean,
+                     _vec(inv_t_rows, "inv_t_rows", f32, rs, x), inv_t, clip_low, clip_high, dual_clip, kl_coef, ent_coef)
+    ent, kl = want_entropy or ent_coef != 0.0, ref_logp is not None
+    v = torch.empty((6, rows), dtype=f32, device=dev).unbind(0)
+    loss, stats = torch.empty((), dtype=f32, device=dev), torch.empty((rows, 2), dtype=f32, device=dev)
+    if want_grad:
+        dx = _grad_out(x, dx, ld)
+    r = PolicyResult(loss, v[0], stats, v[4] if ent else None, v[5] if kl else None, v[1], v[2], v[3], dx if want_grad else None)
+    o = PolicyOut(loss.data_ptr(), v[0].data_ptr(), stats.data_ptr(), _p(r.entropy), _p(r.kl), v[1].data_ptr(), v[2].data_ptr(), v[3].data_ptr(),
+                  _p(r.dx), _loss_rows(dx)[3] if want_grad else 0)
+    ws = torch.empty(lib.whirl_loss_workspace_bytes(rows, seqs), dtype=torch.uint8, device=dev)
+    _call(x, lib.whirl_policy_loss, x.data_ptr(), dt, rows, n, ld, C.byref(p), C.byref(o), ws.data_ptr(), ws.numel())
+    return r
+
+
+@dataclass
+class PreferenceResult:
+    loss: torch.Tensor          # [] float32
+    pair_loss: torch.Tensor     # [pairs]
+    reward: torch.Tensor        # [pairs, 2]: chosen, rejected
+    logp: torch.Tensor          # [rows]
+    stats: torch.Tensor         # [rows, 2]
+    g_logp: torch.Tensor        # [rows]
+    dx: Optional[torch.Tensor]  # d loss / d x
+
+
+def preference_loss(x, token, seq_start, ref_logp=None, weight=None, inv_t: float = 1.0, inv_t_rows=None, beta: float = 0.1,
+                    kind: int = PREF_SIGMOID, smoothing: float = 0.0, margin: float = 0.0, average: bool = False, want_grad: bool = True,
+                    dx=None) -> PreferenceResult:
+    """The preference loss of pairs of sequences packed row after row in x [rows, n] (chosen, rejected, chosen, rejected ...;
+    sequence s holds the rows seq_start[s] to seq_start[s + 1]), with its gradient by the logits (whirl_preference_loss).
+    ref_logp, weight: [rows] float32.  dx may be x itself."""
+    dt, rows, n, ld = _loss_rows(x)
+    f32, i32, rs, dev = torch.float32, torch.int32, (rows,), x.device
+    if seq_start.dim() != 1 or seq_start.numel() % 2 != 1:
+        raise ValueError(f"preference_loss: seq_start is [2 * pairs + 1], got {tuple(seq_start.shape)}")
+    pairs = seq_start.numel() // 2
+    p = PreferenceParams(_vec(token, "token", i32, rs, x), _vec(seq_start, "seq_start", i32, (2 * pairs + 1,), x),
+                         _vec(ref_logp, "ref_logp", f32, rs, x), _vec(weight, "weight", f32, rs, x), _vec(inv_t_rows, "inv_t_rows", f32, rs, x),
+                         pairs, kind, int(average), inv_t, beta, smoothing, margin)
+    logp, g_logp = torch.empty((2, rows), dtype=f32, device=dev).unbind(0)
+    pair_loss, reward = torch.empty(pairs, dtype=f32, device=dev), torch.empty((pairs, 2), dtype=f32, device=dev)
+    loss, stats = torch.empty((), dtype=f32, device=dev), torch.empty((rows, 2), dtype=f32, device=dev)
+    dx = _grad_out(x, dx, ld) if want_grad else None
+    o = PreferenceOut(loss.data_ptr(), pair_loss.data_ptr(), reward.data_ptr(), logp.data_ptr(), stats.data_ptr(), g_logp.data_ptr(), _p(dx),
+                      _loss_rows(dx)[3] if want_grad else 0)
+    ws = torch.empty(lib.whirl_loss_workspace_bytes(rows, pairs), dtype=torch.uint8, device=dev)
+    _call(x, lib.whirl_preference_loss, x.data_ptr(), dt, rows, n, ld, C.byref(p), C.byref(o), ws.data_ptr(), ws.numel())
+    return PreferenceResult(loss, pair_loss, reward, logp, stats, g_logp, dx)
+
+
+# ---- the rows of the next step --------------------------------------------------------------------------------------------
+
+SEQ_OK, SEQ_REFUSED, SEQ_INVALID = 0, 1, 2
+MAX_SEQS = 65536
+
+
+@dataclass
+class StepRows:
+    slot: torch.Tensor      # [max_rows] int64, -1 behind the last row
+    position: torch.Tensor  # [max_rows] int32
+    seq: torch.Tensor       # [max_rows] int32, -1 behind the last row
+    row0: torch.Tensor      # [seqs + 1] int32
+    status: torch.Tensor    # [seqs] int32: SEQ_*
+
+
+def block_tables_step(length, n_new, table, owned, free_ids, free_count, block_size: int, max_rows: int,
+                      rows: Optional[StepRows] = None) -> StepRows:
+    """Blocks, slots and positions of the next step's rows from the sequences' lengths (whirl_block_tables_step).  length, n_new,
+    owned [seqs], table [seqs, max_blocks], free_ids [num_blocks], free_count [1]: int32; the last four are updated."""
+    if table.dim() != 2 or not table.is_cuda:
+        raise ValueError("block_tables_step: table must be [seqs, max_blocks] on a CUDA device")
+    i32, dev = torch.int32, table.device
+    seqs, width = table.shape
+    if rows is None:
+        rows = StepRows(torch.empty(max_rows, dtype=torch.int64, device=dev), *torch.empty((2, max_rows), dtype=i32, device=dev).unbind(0),
+                        torch.empty(seqs + 1, dtype=i32, device=dev), torch.empty(seqs, dtype=i32, device=dev))
+    t = BlockTables(_vec(table, "table", i32, (seqs, width), table), _vec(owned, "owned", i32, (seqs,), table),
+                    _vec(free_ids, "free_ids", i32, (free_ids.numel(),), table), _vec(free_count, "free_count", i32, (1,), table), seqs, width,
+                    free_ids.numel(), block_size)
+    o = StepRowsOut(_vec(rows.slot, "slot", torch.int64, (max_rows,), table), _vec(rows.position, "position", i32, (max_rows,), table),
+                    _vec(rows.seq, "seq", i32, (max_rows,), table), _vec(rows.row0, "row0", i32, (seqs + 1,), table),
+                    _vec(rows.status, "status", i32, (seqs,), table), max_rows)
+    ws = torch.empty(lib.whirl_block_workspace_bytes(seqs), dtype=torch.uint8, device=dev)
+    _call(table, lib.whirl_block_tables_step, _vec(length, "length", i32, (seqs,), table), _vec(n_new, "n_new", i32, (seqs,), table),
+          C.byref(t), C.byref(o), ws.data_ptr(), ws.numel())
+    return rows

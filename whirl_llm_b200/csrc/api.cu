@@ -22,7 +22,7 @@ thread_local uint32_t g_wait_limit = 0;
 thread_local uint32_t g_lose_copy = 0;
 
 // host-side launch counters per kernel family (whirl_launch_counts)
-std::atomic<uint64_t> g_launch[4];
+std::atomic<uint64_t> g_launch[wb::LAUNCH_FAMILIES];
 enum { LC_ROWSCAN = 0, LC_GENERIC = 1, LC_SINGLE = 2, LC_AUX = 3 };
 void bump(int which, uint64_t n = 1) { g_launch[which].fetch_add(n, std::memory_order_relaxed); }
 
@@ -466,8 +466,159 @@ int whirl_merge_sample_rows_packed(const void* blocks, int shards, int rows, int
                       shards, words, words, rows, K_s, n_total, prm, out, stream);
 }
 
+namespace {
+
+// logits rows of the loss entry points
+int bad_rows(const char* who, const void* x, int dtype, int rows, int n, int64_t ld, const int32_t* token, float inv_t, const float* inv_t_rows) {
+    const std::string w(who);
+    if (rows < 0 || n <= 0 || bad_dtype(dtype) || ld < n) return fail(WHIRL_ERR_INVALID, (w + ": bad rows / n / dtype / ld").c_str());
+    if (rows > 0 && (!x || !token)) return fail(WHIRL_ERR_INVALID, (w + ": x / token is null").c_str());
+    if (reinterpret_cast<uintptr_t>(x) & (dtype == WHIRL_F32 ? 3 : 1)) return fail(WHIRL_ERR_INVALID, (w + ": x is not aligned to its type").c_str());
+    if (!inv_t_rows && !(inv_t > 0.f && inv_t <= 3.4e38f)) return fail(WHIRL_ERR_INVALID, (w + ": inv_t has to be positive and finite").c_str());
+    return WHIRL_OK;
+}
+int bad_dx(const char* who, const void* x, int dtype, int rows, int n, int64_t ld, const void* dx, int64_t ld_dx) {
+    const std::string w(who);
+    const int64_t e = dtype == WHIRL_F32 ? 4 : 2;
+    if (ld_dx < n || (reinterpret_cast<uintptr_t>(dx) & (e - 1))) return fail(WHIRL_ERR_INVALID, (w + ": bad ld_dx, or dx is not aligned to its type").c_str());
+    if (rows == 0 || (dx == x && ld_dx == ld)) return WHIRL_OK;
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(dx);
+    if (a < b + uintptr_t(e * (int64_t(rows - 1) * ld_dx + n)) && b < a + uintptr_t(e * (int64_t(rows - 1) * ld + n)))
+        return fail(WHIRL_ERR_INVALID, (w + ": dx overlaps x without being it").c_str());
+    return WHIRL_OK;
+}
+
+struct LossWs {
+    size_t stats, entropy, g_logp, g_entropy, row_loss, row_scale, row_term, seq_term, total;
+};
+LossWs loss_ws(int rows, int seqs) {
+    const size_t r = rows < 1 ? 1 : size_t(rows), s = seqs < 1 ? 1 : size_t(seqs);
+    LossWs w;
+    size_t o = 0;
+    w.row_term = o, o = align_up(o + r * 8, 256);
+    w.seq_term = o, o = align_up(o + s * 8, 256);
+    w.stats = o, o = align_up(o + r * 8, 256);
+    w.entropy = o, o = align_up(o + r * 4, 256);
+    w.g_logp = o, o = align_up(o + r * 4, 256);
+    w.g_entropy = o, o = align_up(o + r * 4, 256);
+    w.row_loss = o, o = align_up(o + r * 4, 256);
+    w.row_scale = o, o = align_up(o + r * 4, 256);
+    w.total = o;
+    return w;
+}
+float* or_ws(float* user, void* ws, size_t off) { return user ? user : reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + off); }
+
+}  // namespace
+
+int whirl_token_logprobs(const void* x, int dtype, int rows, int n, int64_t ld, const int32_t* token, float inv_t, const float* inv_t_rows,
+                         float* logp, float* stats, float* entropy, void* stream) {
+    if (const int st = bad_rows("token_logprobs", x, dtype, rows, n, ld, token, inv_t, inv_t_rows)) return st;
+    if (rows == 0 || (!logp && !stats && !entropy)) return WHIRL_OK;
+    wb::LossArgs a{};
+    a.x = x, a.ld = ld, a.rows = rows, a.n = n, a.token = token, a.inv_t = inv_t, a.inv_t_rows = inv_t_rows;
+    a.logp = logp, a.stats = stats, a.entropy = entropy;
+    const cudaError_t e = wb::logprobs_launch(a, dtype, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? WHIRL_OK : fail_cuda(e, "token_logprobs launch");
+}
+
+int whirl_token_logprobs_grad(const void* x, int dtype, int rows, int n, int64_t ld, const int32_t* token, float inv_t, const float* inv_t_rows,
+                              const float* stats, const float* entropy, const float* g_logp, const float* g_entropy, void* dx, int64_t ld_dx,
+                              void* stream) {
+    if (const int st = bad_rows("token_logprobs_grad", x, dtype, rows, n, ld, token, inv_t, inv_t_rows)) return st;
+    if (rows == 0) return WHIRL_OK;
+    if (!stats || !g_logp || !dx || (g_entropy && !entropy)) return fail(WHIRL_ERR_INVALID, "token_logprobs_grad: stats / g_logp / dx is null, or g_entropy without entropy");
+    if (const int st = bad_dx("token_logprobs_grad", x, dtype, rows, n, ld, dx, ld_dx)) return st;
+    wb::LossArgs a{};
+    a.x = x, a.ld = ld, a.rows = rows, a.n = n, a.token = token, a.inv_t = inv_t, a.inv_t_rows = inv_t_rows;
+    a.stats = const_cast<float*>(stats), a.entropy = const_cast<float*>(entropy);
+    a.g_logp = const_cast<float*>(g_logp), a.g_entropy = const_cast<float*>(g_entropy);
+    a.dx = dx, a.ld_dx = ld_dx;
+    const cudaError_t e = wb::logprobs_grad_launch(a, dtype, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? WHIRL_OK : fail_cuda(e, "token_logprobs_grad launch");
+}
+
+size_t whirl_loss_workspace_bytes(int rows, int seqs) { return loss_ws(rows, seqs).total + 256; }
+
+int whirl_policy_loss(const void* x, int dtype, int rows, int n, int64_t ld, const whirl_policy_params* p, const whirl_policy_out* o, void* ws,
+                      size_t ws_bytes, void* stream) {
+    if (!p || !o || !o->loss) return fail(WHIRL_ERR_INVALID, "policy_loss: params / out / loss is null");
+    if (const int st = bad_rows("policy_loss", x, dtype, rows, n, ld, p->token, p->inv_t, p->inv_t_rows)) return st;
+    if (rows > 0 && !p->adv) return fail(WHIRL_ERR_INVALID, "policy_loss: adv is null");
+    if (p->mean != WHIRL_MEAN_SUM && p->mean != WHIRL_MEAN_TOKENS && p->mean != WHIRL_MEAN_SEQS) return fail(WHIRL_ERR_INVALID, "policy_loss: bad mean");
+    if (p->mean == WHIRL_MEAN_SEQS && (p->seqs < 0 || !p->seq_start)) return fail(WHIRL_ERR_INVALID, "policy_loss: WHIRL_MEAN_SEQS needs seq_start / seqs");
+    if (!(p->clip_low >= 0.f) || !(p->clip_high >= 0.f) || !(p->dual_clip >= 0.f) || !(p->kl_coef == p->kl_coef) || !(p->ent_coef == p->ent_coef))
+        return fail(WHIRL_ERR_INVALID, "policy_loss: a clip is negative, or a coefficient is NaN");
+    if (o->dx)
+        if (const int st = bad_dx("policy_loss", x, dtype, rows, n, ld, o->dx, o->ld_dx)) return st;
+    const LossWs w = loss_ws(rows, p->mean == WHIRL_MEAN_SEQS ? p->seqs : 0);
+    void* base = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(ws) + 255) & ~uintptr_t(255));
+    if (!ws || ws_bytes < w.total + 256) return fail(WHIRL_ERR_WORKSPACE, "policy_loss: workspace missing or too small (whirl_loss_workspace_bytes)");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (rows == 0) {
+        const cudaError_t e = cudaMemsetAsync(o->loss, 0, sizeof(float), st);
+        return e == cudaSuccess ? WHIRL_OK : fail_cuda(e, "cudaMemsetAsync");
+    }
+    const bool ent = p->ent_coef != 0.f;
+    wb::LossArgs a{};
+    a.x = x, a.ld = ld, a.rows = rows, a.n = n, a.token = p->token, a.inv_t = p->inv_t, a.inv_t_rows = p->inv_t_rows, a.weight = p->weight;
+    if (p->mean == WHIRL_MEAN_SEQS) a.seq_start = p->seq_start, a.seqs = p->seqs;
+    a.logp = o->logp, a.stats = or_ws(o->stats, base, w.stats), a.entropy = ent ? or_ws(o->entropy, base, w.entropy) : o->entropy;
+    a.g_logp = or_ws(o->g_logp, base, w.g_logp), a.g_entropy = ent ? or_ws(nullptr, base, w.g_entropy) : nullptr;
+    a.dx = o->dx, a.ld_dx = o->ld_dx;
+    a.adv = p->adv, a.old_logp = p->old_logp, a.ref_logp = p->ref_logp;
+    a.clip_low = p->clip_low, a.clip_high = p->clip_high, a.dual_clip = p->dual_clip, a.kl_coef = p->kl_coef, a.ent_coef = p->ent_coef;
+    a.kl = o->kl, a.row_loss = or_ws(o->row_loss, base, w.row_loss), a.row_scale = or_ws(o->row_scale, base, w.row_scale);
+    a.row_term = reinterpret_cast<double*>(static_cast<uint8_t*>(base) + w.row_term);
+    a.seq_term = reinterpret_cast<double*>(static_cast<uint8_t*>(base) + w.seq_term);
+    const cudaError_t e = wb::policy_launch(a, dtype, p->mean, o->loss, st);
+    return e == cudaSuccess ? WHIRL_OK : fail_cuda(e, "policy_loss launch");
+}
+
+int whirl_preference_loss(const void* x, int dtype, int rows, int n, int64_t ld, const whirl_preference_params* p, const whirl_preference_out* o,
+                          void* ws, size_t ws_bytes, void* stream) {
+    if (!p || !o || !o->loss) return fail(WHIRL_ERR_INVALID, "preference_loss: params / out / loss is null");
+    if (const int st = bad_rows("preference_loss", x, dtype, rows, n, ld, p->token, p->inv_t, p->inv_t_rows)) return st;
+    if (p->pairs < 0 || p->pairs > (1 << 29) || !p->seq_start) return fail(WHIRL_ERR_INVALID, "preference_loss: bad pairs, or seq_start is null");
+    if (p->kind != WHIRL_PREF_SIGMOID && p->kind != WHIRL_PREF_HINGE && p->kind != WHIRL_PREF_SQUARED) return fail(WHIRL_ERR_INVALID, "preference_loss: bad kind");
+    if (!(p->beta > 0.f && p->beta <= 3.4e38f) || !(p->smoothing >= 0.f && p->smoothing <= 1.f) || !(p->margin == p->margin))
+        return fail(WHIRL_ERR_INVALID, "preference_loss: beta has to be positive, smoothing in [0, 1], margin a number");
+    if (o->dx)
+        if (const int st = bad_dx("preference_loss", x, dtype, rows, n, ld, o->dx, o->ld_dx)) return st;
+    const LossWs w = loss_ws(rows, p->pairs);
+    void* base = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(ws) + 255) & ~uintptr_t(255));
+    if (!ws || ws_bytes < w.total + 256) return fail(WHIRL_ERR_WORKSPACE, "preference_loss: workspace missing or too small (whirl_loss_workspace_bytes)");
+    wb::LossArgs a{};
+    a.x = x, a.ld = ld, a.rows = rows, a.n = n, a.token = p->token, a.inv_t = p->inv_t, a.inv_t_rows = p->inv_t_rows, a.weight = p->weight;
+    a.seq_start = p->seq_start, a.seqs = 2 * p->pairs;
+    a.logp = o->logp, a.stats = or_ws(o->stats, base, w.stats), a.g_logp = or_ws(o->g_logp, base, w.g_logp);
+    a.dx = o->dx, a.ld_dx = o->ld_dx, a.ref_logp = p->ref_logp;
+    a.row_scale = or_ws(nullptr, base, w.row_scale);
+    a.row_term = reinterpret_cast<double*>(static_cast<uint8_t*>(base) + w.row_term);
+    a.seq_term = reinterpret_cast<double*>(static_cast<uint8_t*>(base) + w.seq_term);
+    wb::PairArgs q{p->pairs, p->kind, p->average, p->beta, p->smoothing, p->margin, o->pair_loss, o->reward};
+    const cudaError_t e = wb::preference_launch(a, q, dtype, o->loss, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? WHIRL_OK : fail_cuda(e, "preference_loss launch");
+}
+
+size_t whirl_block_workspace_bytes(int seqs) { return wb::block_tables_ws_bytes(seqs < 1 ? 1 : seqs) + 256; }
+
+int whirl_block_tables_step(const int32_t* length, const int32_t* n_new, const whirl_block_tables* t, const whirl_step_rows* r, void* ws,
+                            size_t ws_bytes, void* stream) {
+    if (!t || !r || t->seqs < 0 || t->max_blocks < 0 || t->num_blocks < 0 || t->block_size < 1 || r->max_rows < 0)
+        return fail(WHIRL_ERR_INVALID, "block_tables_step: tables / rows is null, or a size is bad");
+    if (t->seqs > WHIRL_MAX_SEQS) return fail(WHIRL_ERR_UNSUPPORTED, "block_tables_step: seqs above WHIRL_MAX_SEQS");
+    if (!t->free_count || !r->row0 || (t->num_blocks > 0 && !t->free_ids) || (r->max_rows > 0 && !r->slot))
+        return fail(WHIRL_ERR_INVALID, "block_tables_step: free_count / free_ids / row0 / slot is null");
+    if (t->seqs > 0 && (!length || !n_new || !t->owned || !r->status || (t->max_blocks > 0 && !t->table)))
+        return fail(WHIRL_ERR_INVALID, "block_tables_step: length / n_new / owned / status / table is null");
+    if (!ws || ws_bytes < whirl_block_workspace_bytes(t->seqs)) return fail(WHIRL_ERR_WORKSPACE, "block_tables_step: workspace missing or too small (whirl_block_workspace_bytes)");
+    void* base = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(ws) + 255) & ~uintptr_t(255));
+    const cudaError_t e = wb::block_tables_launch(length, n_new, *t, *r, base, sm_count(), static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? WHIRL_OK : fail_cuda(e, "block_tables_step launch");
+}
+
 void whirl_launch_counts(uint64_t* out, int n) {
-    for (int i = 0; i < n && i < 4; ++i) out[i] = g_launch[i].load(std::memory_order_relaxed);
+    for (int i = 0; i < n && i < wb::LAUNCH_FAMILIES; ++i) out[i] = g_launch[i].load(std::memory_order_relaxed);
 }
 
 }  // extern "C"

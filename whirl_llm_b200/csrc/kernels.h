@@ -13,6 +13,7 @@ namespace wb {
 // set by api.cu: the calling thread's error message and the launch counters
 void set_last_error(const char* msg);
 void count_launch(int family);
+enum { LAUNCH_LOSS = 4, LAUNCH_BLOCKS = 5, LAUNCH_FAMILIES = 6 };  // (0 .. 3 are counted by api.cu)
 
 // ---- greedy picks (rowscan.cu)
 enum { RS_ARGMAX = 0, RS_ARGMAX_PROB = 1, RS_DRAFT_PICK = 2 };
@@ -159,6 +160,53 @@ cudaError_t accept_rows_launch(const whirl_accept_in& in, const whirl_relax_para
 cudaError_t accept_residual_launch(const void* target, const void* draft, int dtype, int seqs, int L, int n, const int32_t* draft_tok,
                                    const float* inv_t, const double* u_acc, const double* u_res, void* stats_ws, int32_t* n_acc,
                                    int32_t* next_tok, cudaStream_t st);
+
+// ---- log-probabilities and losses (losses.cu)
+enum { EPI_NONE = 0, EPI_POLICY = 1, EPI_PREF = 2 };
+struct LossArgs {
+    const void* x;  // [rows], ld elements apart
+    int64_t ld;
+    int rows, n;
+    const int32_t* token;
+    float inv_t;
+    const float* inv_t_rows;
+    const float* weight;       // null = 1
+    const int32_t* seq_start;  // null: rows need not lie in a sequence
+    int seqs;
+    // forward outputs (null: not wanted); the gradient reads stats, entropy, g_logp and g_entropy
+    float* logp;
+    float* stats;
+    float* entropy;
+    float* g_logp;
+    float* g_entropy;
+    void* dx;
+    int64_t ld_dx;
+    // policy loss
+    const float* adv;
+    const float* old_logp;
+    const float* ref_logp;  // (the preference loss too)
+    float clip_low, clip_high, dual_clip, kl_coef, ent_coef;
+    float* kl;
+    float* row_loss;
+    float* row_scale;  // [rows] s of the policy loss; the rows' weights of the preference loss
+    double* row_term;  // [rows] scaled row losses / weighted log ratios
+    double* seq_term;  // [seqs] weight sums / pair losses
+};
+struct PairArgs {
+    int pairs, kind, average;
+    float beta, smoothing, margin;
+    float* pair_loss;
+    float* reward;
+};
+cudaError_t logprobs_launch(const LossArgs& a, int dtype, cudaStream_t st);
+cudaError_t logprobs_grad_launch(const LossArgs& a, int dtype, cudaStream_t st);
+cudaError_t policy_launch(const LossArgs& a, int dtype, int mean, float* loss, cudaStream_t st);
+cudaError_t preference_launch(const LossArgs& a, const PairArgs& p, int dtype, float* loss, cudaStream_t st);
+
+// ---- cache block tables (block_tables.cu)
+size_t block_tables_ws_bytes(int seqs);
+cudaError_t block_tables_launch(const int32_t* length, const int32_t* n_new, const whirl_block_tables& t, const whirl_step_rows& r, void* ws,
+                                int sm_count, cudaStream_t st);
 
 // ---- vocab-sharded candidates (merge.cu)
 cudaError_t merge_sample_launch(const int32_t* ids, const float* vals, const float* stats, int shards, size_t cand_stride,
