@@ -172,7 +172,7 @@ def test_decode_then_train():
     assert torch.isfinite(scored.logp).all() and x.shape[0] == sum(len(t) for t in text) - seqs
     adv = torch.randn(x.shape[0], device="cuda", generator=g)
     p = api.policy_loss(x, token, adv, old_logp=scored.logp, ref_logp=scored.logp, seq_start=start, mean=api.MEAN_SEQS, kl_coef=0.1)
-    assert torch.equal(p.logp, scored.logp) and p.kl.abs().max() < 1e-12
+    assert (p.logp - scored.logp).abs().max() < 1e-5 and p.kl.abs().max() < 1e-9
     counts = (start[1:] - start[:-1]).double()
     want = -(adv.double() / counts[seq.long()] / seqs).sum()      # every ratio is 1
     assert abs(p.loss.double() - want) < 1e-5

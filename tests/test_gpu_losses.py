@@ -221,7 +221,8 @@ def test_policy(rows, n, pad, off, mean, dtype):
     for a, b in zip(vars(r).values(), vars(again).values()):
         assert a is None or torch.equal(a, b)  # the same bits
     f = call(want_grad=False)
-    assert f.dx is None and torch.equal(f.loss, r.loss) and torch.equal(f.g_logp, r.g_logp)
+    assert f.dx is None  # (another kernel: its sums run in another order)
+    check_policy(f, x64, token, it, stats, adv, old, rf, weight, mean, starts, dtype, n, **kw)
     # no entropy, no KL, no weights, on-policy
     kw2 = dict(clip_low=0.2, clip_high=0.2)
     r = api.policy_loss(x, token.cuda(), adv.cuda(), seq_start=st, inv_t=1.25, mean=mean, **kw2)
@@ -377,15 +378,21 @@ def test_rows_past_2_to_31_elements():
         token[r] = 1000 * i + 5
     res = api.token_logprobs(x, token)
     small = api.token_logprobs(x[pick].contiguous(), token[pick].contiguous())
-    assert torch.equal(res.logp[pick], small.logp) and torch.equal(res.stats[pick], small.stats)
+    # (a batch of four rows is split over more thread blocks: sums in another order)
+    close(res.logp[pick], small.logp.cpu(), 2 * ref.logp_tol(n, small.logp.cpu().double()))
+    close(res.stats[pick], small.stats.cpu(), 2 * ref.sum_error(n) * small.stats.cpu().double())
     gl = torch.ones(rows, device="cuda")
     d = api.token_logprobs_grad(x[pick].contiguous(), token[pick].contiguous(), small.stats, gl[:4])
+    res.stats[pick] = small.stats
     dx = api.token_logprobs_grad(x, token, res.stats, gl)
     assert torch.equal(dx[pick], d) and (dx[100] == 0).all() and (dx[8998] == 0).all()
     adv = torch.ones(rows, device="cuda")
     p = api.policy_loss(x, token, adv, mean=0, dx=dx)
     q = api.policy_loss(x[pick].contiguous(), token[pick].contiguous(), adv[:4], mean=0)
-    assert torch.equal(p.loss, q.loss) and torch.equal(dx[pick], q.dx) and (dx[8998] == 0).all()
+    close(p.loss, q.loss.cpu(), 1e-6 * q.loss.abs().item())
+    # both are off by at most a bf16 half step and some 1e-6 from the same value
+    close(dx[pick], q.dx.cpu(), 2 * (2.0 ** -8 + 1e-5) * q.dx.cpu().double().abs() + 1e-6)
+    assert (dx[8998] == 0).all()
 
 
 def test_streams_threads_and_graphs():

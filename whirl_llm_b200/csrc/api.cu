@@ -489,7 +489,7 @@ int bad_dx(const char* who, const void* x, int dtype, int rows, int n, int64_t l
 }
 
 struct LossWs {
-    size_t stats, entropy, g_logp, g_entropy, row_loss, row_scale, row_term, seq_term, total;
+    size_t stats, entropy, g_logp, g_entropy, row_scale, row_term, seq_term, ticket, total;
 };
 LossWs loss_ws(int rows, int seqs) {
     const size_t r = rows < 1 ? 1 : size_t(rows), s = seqs < 1 ? 1 : size_t(seqs);
@@ -501,8 +501,8 @@ LossWs loss_ws(int rows, int seqs) {
     w.entropy = o, o = align_up(o + r * 4, 256);
     w.g_logp = o, o = align_up(o + r * 4, 256);
     w.g_entropy = o, o = align_up(o + r * 4, 256);
-    w.row_loss = o, o = align_up(o + r * 4, 256);
     w.row_scale = o, o = align_up(o + r * 4, 256);
+    w.ticket = o, o += 256;
     w.total = o;
     return w;
 }
@@ -567,10 +567,11 @@ int whirl_policy_loss(const void* x, int dtype, int rows, int n, int64_t ld, con
     a.dx = o->dx, a.ld_dx = o->ld_dx;
     a.adv = p->adv, a.old_logp = p->old_logp, a.ref_logp = p->ref_logp;
     a.clip_low = p->clip_low, a.clip_high = p->clip_high, a.dual_clip = p->dual_clip, a.kl_coef = p->kl_coef, a.ent_coef = p->ent_coef;
-    a.kl = o->kl, a.row_loss = or_ws(o->row_loss, base, w.row_loss), a.row_scale = or_ws(o->row_scale, base, w.row_scale);
+    a.kl = o->kl, a.row_loss = o->row_loss, a.row_scale = or_ws(o->row_scale, base, w.row_scale);
     a.row_term = reinterpret_cast<double*>(static_cast<uint8_t*>(base) + w.row_term);
     a.seq_term = reinterpret_cast<double*>(static_cast<uint8_t*>(base) + w.seq_term);
-    const cudaError_t e = wb::policy_launch(a, dtype, p->mean, o->loss, st);
+    a.ticket = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(base) + w.ticket), a.loss = o->loss;
+    const cudaError_t e = wb::policy_launch(a, dtype, p->mean, st);
     return e == cudaSuccess ? WHIRL_OK : fail_cuda(e, "policy_loss launch");
 }
 

@@ -8,7 +8,9 @@
 #include "../../include/whirl_b200.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cfloat>
+#include <cstdlib>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -18,69 +20,167 @@ namespace wb {
 namespace {
 
 // ---------------------------------------------------------------------------------------------------------------
+// pairs of floats: two results per instruction (add / mul / fma .f32x2)
+// ---------------------------------------------------------------------------------------------------------------
+
+struct F2 {
+    unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 split(F2 a) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+    return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
 // softmax statistics
 // ---------------------------------------------------------------------------------------------------------------
 
-// Partial statistics of a set of logits: m their maximum (-inf without one), s = sum 2^((x - r) c), q = sum of the same terms
-// times their exponent (x - r) c, with the reference r = max(m, -FLT_MAX) and c = inv_t log2 e.  (The exponent is formed from
-// the difference, not as x c - r c: rows of the type's lowest values stay exact, and so does the term of the maximum.)
+// c = inv_t log2 e in two floats, hi rounded down so that lo >= 0 (a difference of -inf keeps its sign in both products).  With one
+// float the exponents of a whole row are off in the same direction, by up to 6e-8 of their size: a bias of some 3e-7 in
+// every log-probability, which sums over a sequence do not average out.
+struct Scale {
+    float hi, lo;
+};
+__device__ __forceinline__ Scale scale_of(float inv_t) {
+    const double c = double(inv_t) * 1.4426950408889634;
+    Scale r;
+    r.hi = __double2float_rd(c);
+    r.lo = fmaxf(float(c - double(r.hi)), 1e-37f);
+    return r;
+}
+
+// Partial statistics of a set of logits: m their maximum (-inf without one), s - e = sum 2^((x - r) c) (e: what Kahan's sum owes),
+// q = sum of the same terms times their exponent (x - r) c, with the reference r = max(m, -FLT_MAX).  (The exponent is formed
+// from the difference, not as x c - r c: rows of the type's lowest values stay exact, and so does the term of the maximum.)
+// A plain float sum is not enough: in the thread that meets the row's peak every later term is rounded to the peak's last
+// bits, 300 times in a row of 151936, all of it landing in the log-probability (measured: 4e-7).
 struct Soft {
-    float m = -INFINITY, s = 0.f, q = 0.f;
+    float m = -INFINITY, s = 0.f, q = 0.f, e = 0.f;
 };
 __device__ __forceinline__ float ref_of(float m) { return fmaxf(m, -FLT_MAX); }
 
 template <bool ENT>
-__device__ __forceinline__ void raise(Soft& a, float m, float c) {  // moves a's reference to that of m >= a.m
-    const float t = (ref_of(a.m) - ref_of(m)) * c, f = ex2_approx(t);
-    if (ENT) a.q = a.s == 0.f ? 0.f : f * fmaf(fmaxf(t, -1000.f), a.s, a.q);
+__device__ __forceinline__ void raise(Soft& a, float m, Scale c) {  // moves a's reference to that of m >= a.m
+    const float d = ref_of(a.m) - ref_of(m), t = fmaf(d, c.lo, d * c.hi), f = ex2_approx(t);
+    if (a.s == 0.f) a.q = 0.f;
+    else if (ENT) a.q = f * fmaf(fmaxf(t, -1000.f), a.s, a.q);
     a.s = a.s == 0.f ? 0.f : a.s * f;
+    a.e *= f;
     a.m = m;
 }
-template <bool ENT>
-__device__ __forceinline__ void merge(Soft& a, Soft b, float c) {
-    const float m = fmaxf(a.m, b.m);
-    raise<ENT>(a, m, c);
-    raise<ENT>(b, m, c);
-    a.s += b.s;
-    if (ENT) a.q += b.q;
-}
-template <bool ENT>
-__device__ __forceinline__ void add(Soft& a, float x, float r, float c) {
-    const float t = (x - r) * c, w = ex2_approx(t);
-    a.s += w;
-    if (ENT) a.q = fmaf(w, fmaxf(t, -1000.f), a.q);  // (0 * -inf is not what a forbidden token adds)
-}
+// N logits: their terms are summed as a tree, the tree's sum goes into the thread's by Kahan's rule
 template <bool ENT, int N>
-__device__ __forceinline__ void add_many(Soft& a, const float (&x)[N], float c) {
+__device__ __forceinline__ void add_many(Soft& a, const float (&x)[N], Scale c) {
     float m = x[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) m = fmaxf(m, x[i]);
     if (m > a.m) raise<ENT>(a, m, c);
     const float r = ref_of(a.m);
+    float sum, qs = 0.f;
+    if (N == 1) {
+        const float d = x[0] - r, t = fmaf(d, c.lo, d * c.hi);
+        sum = ex2_approx(t);
+        if (ENT) qs = sum * fmaxf(t, -1000.f);
+    } else {
+        const F2 nr = f2(-r, -r), hi = f2(c.hi, c.hi), lo = f2(c.lo, c.lo);
+        F2 w[N / 2 > 0 ? N / 2 : 1], q = f2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < N; ++i) add<ENT>(a, x[i], r, c);
+        for (int i = 0; i < N / 2; ++i) {
+            const F2 d = add2(f2(x[2 * i], x[2 * i + 1]), nr);
+            const float2 t = split(fma2(d, lo, mul2(d, hi)));
+            w[i] = f2(ex2_approx(t.x), ex2_approx(t.y));
+            if (ENT) q = fma2(w[i], f2(fmaxf(t.x, -1000.f), fmaxf(t.y, -1000.f)), q);  // (0 * -inf is not what a forbidden token adds)
+        }
+#pragma unroll
+        for (int k = N / 4; k >= 1; k /= 2)
+#pragma unroll
+            for (int i = 0; i < k; ++i) w[i] = add2(w[i], w[i + k]);
+        const float2 p = split(w[0]), v = split(q);
+        sum = p.x + p.y;
+        if (ENT) qs = v.x + v.y;
+    }
+    const float y = __fsub_rn(sum, a.e), t = __fadd_rn(a.s, y);
+    a.e = __fsub_rn(__fsub_rn(t, a.s), y);
+    a.s = t;
+    if (ENT) a.q += qs;
 }
 
-template <bool ENT>
-__device__ Soft block_merge(Soft a, float c, Soft* sh) {  // the result is valid in every thread of warp 0
+// The statistics of all threads of the CTA, then of all CTAs of the cluster; the result is valid in warp 0 of every CTA.  Every
+// thread's sum is brought to the common maximum once (a tree of pairwise merges would scale it several times over, and
+// ex2.approx errs downwards, 5e-8 on average, each time).
+struct ReduceShared {
+    float m[32];
+    float2 sq[32];
+    float4 part[16];  // one per CTA of the cluster
+};
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ float warp_sum_f(float v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        Soft b;
-        b.m = __shfl_xor_sync(0xffffffffu, a.m, o), b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-        if (ENT) b.q = __shfl_xor_sync(0xffffffffu, a.q, o);
-        merge<ENT>(a, b, c);
-    }
-    const int w = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    if (lane_id() == 0) sh[w] = a;
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+template <bool ENT>
+__device__ __forceinline__ Soft reduce(Soft a, Scale c, ReduceShared& sh, int ctas) {
+    const int w = threadIdx.x >> 5, nw = blockDim.x >> 5, lane = lane_id();
+    a.s -= a.e, a.e = 0.f;
+    float m = warp_max(a.m);
+    if (lane == 0) sh.m[w] = m;
+    __syncthreads();
+    m = warp_max(lane < nw ? sh.m[lane] : -INFINITY);
+    raise<ENT>(a, m, c);
+    a.s = warp_sum_f(a.s);
+    if (ENT) a.q = warp_sum_f(a.q);
+    if (lane == 0) sh.sq[w] = make_float2(a.s, a.q);
     __syncthreads();
     if (w == 0) {
-        a = lane_id() < nw ? sh[lane_id()] : Soft{};
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            Soft b;
-            b.m = __shfl_xor_sync(0xffffffffu, a.m, o), b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-            if (ENT) b.q = __shfl_xor_sync(0xffffffffu, a.q, o);
-            merge<ENT>(a, b, c);
+        const float2 v = lane < nw ? sh.sq[lane] : make_float2(0.f, 0.f);
+        a.s = warp_sum_f(v.x);
+        a.q = ENT ? warp_sum_f(v.y) : 0.f;
+    }
+    if (ctas > 1) {
+        if (w == 0 && lane < ctas) {  // lane i tells CTA i
+            uint32_t to;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(&sh.part[cluster_rank()])), "r"(lane));
+            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(m), "f"(a.s), "f"(a.q), "f"(0.f) : "memory");
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (w == 0) {
+            const float4 p = lane < ctas ? sh.part[lane] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+            a.m = p.x, a.s = p.y, a.q = p.z;
+            m = warp_max(a.m);
+            raise<ENT>(a, m, c);
+            a.s = warp_sum_f(a.s);
+            if (ENT) a.q = warp_sum_f(a.q);
         }
     }
     return a;
@@ -146,6 +246,21 @@ __device__ __forceinline__ GradRow grad_row(float m, double sum, double inv_t, i
     q.d = float(inv_t * g);
     return q;
 }
+template <bool ENT, int N>
+__device__ __forceinline__ void grad_many(const GradRow& q, float (&x)[N], int at) {  // at: the token's place, outside [0, N) elsewhere
+    const F2 nr = f2(-q.r, -q.r), c = f2(q.c, q.c), a = f2(q.a, q.a), b = f2(q.b, q.b);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        const float2 t = split(mul2(add2(f2(x[i], x[i + 1]), nr), c));
+        const F2 w = f2(ex2_approx(t.x), ex2_approx(t.y));
+        const float2 v = split(ENT ? mul2(w, fma2(b, f2(fmaxf(t.x, -1000.f), fmaxf(t.y, -1000.f)), a)) : mul2(w, a));
+        x[i] = v.x, x[i + 1] = v.y;
+    }
+    if (unsigned(at) < unsigned(N)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] += i == at ? q.d : 0.f;
+    }
+}
 template <bool ENT>
 __device__ __forceinline__ float grad_of(const GradRow& q, float x) {
     const float t = (x - q.r) * q.c, w = ex2_approx(t);
@@ -156,7 +271,8 @@ __device__ __forceinline__ float grad_of(const GradRow& q, float x) {
 // forward: one CTA per row
 // ---------------------------------------------------------------------------------------------------------------
 
-constexpr int kFwdThreads = 512;
+constexpr int kFwdThreads = 512, kFusedThreads = 256;
+constexpr int kSliceMost = 200 * 1024;  // bytes of a row's slice that a CTA can hold
 
 // the row as a user's call describes it, and whether it counts
 struct RowOf {
@@ -210,9 +326,13 @@ __device__ PolicyRow policy_row(const LossArgs& a, int row, double logp, double 
     return p;
 }
 
-// Writes what a call wants of one row.  One thread.
+// What a row comes to; with `write`, what the call wants of it is written.  One thread.
+struct RowDone {
+    double sum, entropy, g, h;
+};
 template <int EPI, bool ENT>
-__device__ void finish_row(const LossArgs& a, int row, bool live, int token, float inv_t, float x_token, const Soft& s) {
+__device__ RowDone finish_row(const LossArgs& a, int row, bool write, bool live, int token, float inv_t, float x_token, const Soft& s) {
+    RowDone done{};
     double logp = 0.0, entropy = 0.0, sum = 0.0;
     float m = 0.f;
     if (live) {
@@ -223,53 +343,191 @@ __device__ void finish_row(const LossArgs& a, int row, bool live, int token, flo
         logp = (double(x_token) - double(m)) * double(inv_t) - ls;
         if (ENT) entropy = ls - 0.6931471805599453 * double(s.q) / sum;
     }
-    if (a.logp) a.logp[row] = float(logp);
-    if (a.stats) a.stats[2 * int64_t(row)] = m, a.stats[2 * int64_t(row) + 1] = float(sum);
-    if (ENT && a.entropy) a.entropy[row] = float(entropy);
+    done.sum = sum, done.entropy = entropy;
+    if (EPI != EPI_POLICY && !write) return done;
+    if (write && a.logp) a.logp[row] = float(logp);
+    if (write && a.stats) a.stats[2 * int64_t(row)] = m, a.stats[2 * int64_t(row) + 1] = float(sum);
+    if (write && ENT && a.entropy) a.entropy[row] = float(entropy);
     if (EPI == EPI_POLICY) {
         PolicyRow p{};
         float scale = 0.f;
         if (live) scale = a.row_scale[row], p = policy_row(a, row, logp, entropy);
-        if (a.kl) a.kl[row] = float(p.kl);
-        a.row_loss[row] = float(p.loss);
-        a.g_logp[row] = float(double(scale) * p.dlogp);
-        if (a.g_entropy) a.g_entropy[row] = live ? -a.ent_coef * scale : 0.f;
-        a.row_term[row] = live ? double(scale) * p.loss : 0.0;
+        done.g = float(double(scale) * p.dlogp), done.h = live ? -a.ent_coef * scale : 0.f;
+        if (write) {
+            if (a.kl) a.kl[row] = float(p.kl);
+            if (a.row_loss) a.row_loss[row] = float(p.loss);
+            if (a.g_logp) a.g_logp[row] = float(done.g);
+            if (a.g_entropy) a.g_entropy[row] = float(done.h);
+            a.row_term[row] = live ? double(scale) * p.loss : 0.0;
+        }
     } else if (EPI == EPI_PREF) {
         const float w = !live ? 0.f : (a.weight ? a.weight[row] : 1.f);
         a.row_term[row] = live ? double(w) * (logp - (a.ref_logp ? double(a.ref_logp[row]) : 0.0)) : 0.0;
         a.row_scale[row] = w;
         a.g_logp[row] = 0.f;  // (the rows of a pair get theirs from pairs_kernel)
     }
+    return done;
 }
 
-template <typename T, int EPI, bool ENT>
-__global__ void __launch_bounds__(kFwdThreads) forward_kernel(LossArgs a) {
-    constexpr int E = 16 / sizeof(T);
-    __shared__ Soft sh[32];
-    const int row = blockIdx.x, tid = threadIdx.x;
+__device__ double block_sum(double v, double* sh) {  // the same value in every thread
+    v = warp_sum(v);
+    __syncthreads();
+    if (lane_id() == 0) sh[threadIdx.x >> 5] = v;
+    __syncthreads();
+    double t = lane_id() < int(blockDim.x >> 5) ? sh[lane_id()] : 0.0;
+    return warp_sum(t);
+}
+
+// A kernel that may start before the one ahead of it in the stream has ended waits here for that one's results (no wait where it
+// was launched the ordinary way).
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// The CTA that finishes the last row adds up the rows' terms, in their order.  (Called by one CTA per row, after its thread 0 has
+// written the row's term.)
+__device__ void last_sum(const LossArgs& a) {
+    __shared__ bool last;
+    __shared__ double sh_d[32];
+    if (threadIdx.x == 0) {
+        __threadfence();
+        last = atomicAdd(a.ticket, 1u) + 1u == unsigned(a.rows);
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    double t = 0.0;
+    for (int r = threadIdx.x; r < a.rows; r += blockDim.x) t += __ldcg(a.row_term + r);
+    t = block_sum(t, sh_d);
+    if (threadIdx.x == 0) *a.loss = float(t);
+}
+
+__device__ __forceinline__ void copy_async16(void* smem, const void* g) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem)), "l"(g) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void copies_but(int = 0) {  // waits for this thread's copies but its last N groups
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// One cluster per row, each CTA a contiguous slice of `per` 16-byte vectors; the scalars before the first and behind the last
+// boundary belong to rank 0, one per thread.
+template <typename T, int EPI, bool ENT, bool GRAD>
+__global__ void __launch_bounds__(GRAD ? kFusedThreads : kFwdThreads, GRAD ? 5 : 3) rows_kernel(LossArgs a, int per) {
+    constexpr int E = 16 / sizeof(T), NT = GRAD ? kFusedThreads : kFwdThreads;
+    extern __shared__ __align__(16) uint4 slice[];  // GRAD: this CTA's part of the row
+    __shared__ ReduceShared sh;
+    __shared__ GradRow s_q;
+    __shared__ bool s_zero;
+    const int ctas = int(cluster_size()), rank = int(cluster_rank()), tid = threadIdx.x;
+    const int row = int(blockIdx.x / unsigned(ctas));
     const RowOf w = row_of(a, row);
-    if (!w.live) {
-        if (tid == 0) finish_row<EPI, ENT>(a, row, false, w.token, w.inv_t, 0.f, Soft{});
-        return;
-    }
-    const float c = w.inv_t * kLog2e;
     const T* x = static_cast<const T*>(a.x) + int64_t(row) * a.ld;
-    const int head = head_of(x, a.n), nv = (a.n - head) / E;
-    Soft s;
-    const uint4* v = reinterpret_cast<const uint4*>(x + head);
-#pragma unroll 4
-    for (int i = tid; i < nv; i += kFwdThreads) {
-        float e[E];
-        unpack<T>(v[i], e);
-        add_many<ENT>(s, e, c);
+    const int head = head_of(x, a.n), nv = (a.n - head) / E, edge = a.n - nv * E;
+    const int v0 = min(rank * per, nv), cnt = min(per, nv - v0);
+    const uint4* v = reinterpret_cast<const uint4*>(x + head) + v0;
+    const int my_edge = rank == 0 && tid < edge ? (tid < head ? tid : tid + nv * E) : -1;  // (edge < 2 E <= NT)
+    float x_edge = 0.f;
+    GradRow q{};
+    bool zero = true;
+    if (w.live) {
+        const Scale c = scale_of(w.inv_t);
+        Soft s;
+        float x_token = 0.f;
+        if (GRAD) {
+            const int quarter = (cnt + 4 * NT - 1) / (4 * NT);
+            for (int g = 0, i = tid; g < 4; ++g) {
+                for (int k = 0; k < quarter; ++k, i += NT)
+                    if (i < cnt) copy_async16(slice + i, v + i);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            }
+            if (tid == 0) x_token = load_one(x + w.token);
+            if (my_edge >= 0) {
+                x_edge = load_one(x + my_edge);
+                const float e[1] = {x_edge};
+                add_many<ENT, 1>(s, e, c);
+            }
+            for (int g = 0, i = tid; g < 4; ++g) {  // (each thread reads what it copied itself: no barrier)
+                if (g == 0) copies_but<3>();
+                else if (g == 1) copies_but<2>();
+                else if (g == 2) copies_but<1>();
+                else copies_but<0>();
+                for (int k = 0; k < quarter; ++k, i += NT)
+                    if (i < cnt) {
+                        float e[E];
+                        unpack<T>(slice[i], e);
+                        add_many<ENT, E>(s, e, c);
+                    }
+            }
+        } else {
+            if (tid == 0) x_token = load_one(x + w.token);
+            if (my_edge >= 0) {
+                const float e[1] = {load_one(x + my_edge)};
+                add_many<ENT, 1>(s, e, c);
+            }
+            int i = tid;
+            for (; i + 3 * NT < cnt; i += 4 * NT) {
+                const uint4 b[4] = {v[i], v[i + NT], v[i + 2 * NT], v[i + 3 * NT]};
+#pragma unroll
+                for (int k = 0; k < 4; k += 8 / E) {
+                    float e[8];
+                    if (E == 8) unpack<uint16_t>(b[k], e);
+                    else {
+                        float lo[4], hi[4];
+                        unpack<float>(b[k], lo), unpack<float>(b[(k + 1) & 3], hi);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) e[j] = lo[j], e[j + 4] = hi[j];
+                    }
+                    add_many<ENT, 8>(s, e, c);
+                }
+            }
+            for (; i < cnt; i += NT) {
+                float e[E];
+                unpack<T>(v[i], e);
+                add_many<ENT, E>(s, e, c);
+            }
+        }
+        s = reduce<ENT>(s, c, sh, ctas);
+        if (tid == 0) {
+            grid_dependency_wait();  // row_scale_kernel's results; row_scale and the ticket are read below
+            const RowDone d = finish_row<EPI, ENT>(a, row, rank == 0, true, w.token, w.inv_t, x_token, s);
+            if (GRAD) {
+                s_zero = d.g == 0.0 && d.h == 0.0;
+                s_q = grad_row(s.m, d.sum, w.inv_t, w.token, d.g, d.h, d.entropy);
+            }
+        }
+        if (GRAD) {
+            __syncthreads();
+            zero = s_zero;
+            if (!zero) q = s_q;
+        }
+    } else if (tid == 0) {
+        grid_dependency_wait();
+        if (rank == 0) finish_row<EPI, ENT>(a, row, true, false, w.token, w.inv_t, 0.f, Soft{});
     }
-    for (int i = tid; i < head + (a.n - head - nv * E); i += kFwdThreads) {
-        const float e[1] = {load_one(x + (i < head ? i : i + nv * E))};
-        add_many<ENT>(s, e, c);
+    if (GRAD) {
+        T* dx = static_cast<T*>(a.dx) + int64_t(row) * a.ld_dx;
+        if (my_edge >= 0) store_one(dx + my_edge, zero ? 0.f : grad_of<ENT>(q, x_edge) + (my_edge == q.token ? q.d : 0.f));
+        const bool vec = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
+        T* body = dx + head + int64_t(v0) * E;
+        const int at = zero ? -1 : q.token - head - v0 * E;
+        for (int i = tid; i < cnt; i += NT) {
+            uint4 o = make_uint4(0, 0, 0, 0);
+            if (!zero) {
+                float e[E];
+                unpack<T>(slice[i], e);
+                grad_many<ENT, E>(q, e, at - i * E);
+                o = pack<T>(e);
+            }
+            if (vec) {
+                __stcs(reinterpret_cast<uint4*>(body) + i, o);
+            } else {
+                float e[E];
+                unpack<T>(o, e);
+#pragma unroll
+                for (int k = 0; k < E; ++k) store_one(body + int64_t(i) * E + k, e[k]);
+            }
+        }
     }
-    s = block_merge<ENT>(s, c, sh);
-    if (tid == 0) finish_row<EPI, ENT>(a, row, true, w.token, w.inv_t, load_one(x + w.token), s);
+    if (EPI == EPI_POLICY && rank == 0) last_sum(a);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -314,11 +572,7 @@ __global__ void __launch_bounds__(kGradThreads) grad_kernel(LossArgs a, int chun
             dv[i] = make_uint4(0, 0, 0, 0);
         } else {
             unpack<T>(v[i], e);
-#pragma unroll
-            for (int k = 0; k < E; ++k) e[k] = grad_of<ENT>(q, e[k]);
-            const int o = at - head - i * E;
-#pragma unroll
-            for (int k = 0; k < E; ++k) e[k] = o == k ? e[k] + q.d : e[k];
+            grad_many<ENT, E>(q, e, at - head - i * E);
             dv[i] = pack<T>(e);
         }
     }
@@ -339,15 +593,6 @@ __global__ void __launch_bounds__(kGradThreads) grad_kernel(LossArgs a, int chun
 
 constexpr int kSmallThreads = 1024;
 
-__device__ double block_sum(double v, double* sh) {  // the same value in every thread
-    v = warp_sum(v);
-    __syncthreads();
-    if (lane_id() == 0) sh[threadIdx.x >> 5] = v;
-    __syncthreads();
-    double t = lane_id() < int(blockDim.x >> 5) ? sh[lane_id()] : 0.0;
-    return warp_sum(t);
-}
-
 __device__ __forceinline__ float live_weight(const LossArgs& a, int row) {
     if (unsigned(a.token[row]) >= unsigned(a.n)) return 0.f;
     if (!a.weight) return 1.f;
@@ -364,6 +609,8 @@ __device__ __forceinline__ int2 rows_of(const LossArgs& a, int s) {
 __global__ void __launch_bounds__(kSmallThreads) row_scale_kernel(LossArgs a, int mean) {
     __shared__ double sh[32];
     const int tid = threadIdx.x;
+    asm volatile("griddepcontrol.launch_dependents;");
+    if (tid == 0) *a.ticket = 0;
     if (mean != WHIRL_MEAN_SEQS) {
         double k = 1.0;
         if (mean == WHIRL_MEAN_TOKENS) {
@@ -448,18 +695,49 @@ __global__ void __launch_bounds__(kPairThreads) pairs_kernel(LossArgs a, PairArg
     }
 }
 
+// A launch of rows_kernel: `ctas` CTAs per row in a cluster, `per` vectors each.
+template <typename T, int EPI, bool ENT, bool GRAD>
+cudaError_t rows_launch(const LossArgs& a, int ctas, int per, cudaStream_t st) {
+    constexpr int kMost = kSliceMost;
+    static std::atomic<uint64_t> ready{0};  // bit per device: the function's limits are raised
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    auto* const f = rows_kernel<T, EPI, ENT, GRAD>;
+    if (dev > 63 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {
+        if (GRAD) e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_release);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(a.rows) * unsigned(ctas)), cfg.blockDim = dim3(GRAD ? kFusedThreads : kFwdThreads), cfg.stream = st;
+    cfg.dynamicSmemBytes = GRAD ? size_t(per) * 16 : 0;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = unsigned(ctas), at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at, cfg.numAttrs = EPI == EPI_POLICY ? 2 : 1;  // (the policy loss follows row_scale_kernel)
+    e = cudaLaunchKernelEx(&cfg, f, a, per);
+    count_launch(LAUNCH_LOSS);
+    return e;
+}
+template <int EPI, bool GRAD>
+cudaError_t rows_launch(const LossArgs& a, int dtype, bool ent, int ctas, int per, cudaStream_t st) {
+    if (dtype == WHIRL_F32) return ent ? rows_launch<float, EPI, true, GRAD>(a, ctas, per, st) : rows_launch<float, EPI, false, GRAD>(a, ctas, per, st);
+    return ent ? rows_launch<uint16_t, EPI, true, GRAD>(a, ctas, per, st) : rows_launch<uint16_t, EPI, false, GRAD>(a, ctas, per, st);
+}
+
+int vectors_of(int n, int dtype) { return int((int64_t(n) * (dtype == WHIRL_F32 ? 4 : 2) + 15) / 16); }
+
 template <int EPI>
 cudaError_t forward_launch(const LossArgs& a, int dtype, bool ent, cudaStream_t st) {
-    const dim3 grid(unsigned(a.rows)), block(kFwdThreads);
-    if (dtype == WHIRL_F32) {
-        if (ent) forward_kernel<float, EPI, true><<<grid, block, 0, st>>>(a);
-        else forward_kernel<float, EPI, false><<<grid, block, 0, st>>>(a);
-    } else {
-        if (ent) forward_kernel<uint16_t, EPI, true><<<grid, block, 0, st>>>(a);
-        else forward_kernel<uint16_t, EPI, false><<<grid, block, 0, st>>>(a);
-    }
-    count_launch(LAUNCH_LOSS);
-    return cudaGetLastError();
+    const int nv = vectors_of(a.n, dtype);
+    int ctas = 1;
+    while (ctas < 16 && int64_t(a.rows) * ctas < 592 && nv / (2 * ctas) >= kFwdThreads) ctas *= 2;
+    if (const char* v = getenv("WB_CF")) ctas = atoi(v);
+    return rows_launch<EPI, false>(a, dtype, ent, ctas, (nv + ctas - 1) / ctas, st);
 }
 
 }  // namespace
@@ -481,18 +759,22 @@ cudaError_t logprobs_grad_launch(const LossArgs& a, int dtype, cudaStream_t st) 
     return cudaGetLastError();
 }
 
-cudaError_t policy_launch(const LossArgs& a, int dtype, int mean, float* loss, cudaStream_t st) {
+cudaError_t policy_launch(const LossArgs& a, int dtype, int mean, cudaStream_t st) {
     row_scale_kernel<<<1, kSmallThreads, 0, st>>>(a, mean);
     count_launch(LAUNCH_LOSS);
-    cudaError_t e = forward_launch<EPI_POLICY>(a, dtype, a.ent_coef != 0.f || a.entropy, st);
+    cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    if (a.dx) {
-        e = logprobs_grad_launch(a, dtype, st);
-        if (e != cudaSuccess) return e;
-    }
-    sum_kernel<<<1, kSmallThreads, 0, st>>>(a.row_term, a.rows, 1.0, loss);
-    count_launch(LAUNCH_LOSS);
-    return cudaGetLastError();
+    const bool ent = a.ent_coef != 0.f || a.entropy;
+    const int nv = vectors_of(a.n, dtype);
+    int ctas = 1, most = 44 * 1024;
+    if (const char* v = getenv("WB_SL")) most = atoi(v) * 1024;
+    while (ctas < 16 && int64_t(nv + ctas - 1) / ctas * 16 > most) ctas *= 2;
+    while (ctas < 16 && int64_t(a.rows) * ctas < 592 && nv / (2 * ctas) >= kFusedThreads) ctas *= 2;
+    if (const char* v = getenv("WB_CG")) ctas = atoi(v);
+    const int64_t per = (int64_t(nv) + ctas - 1) / ctas;
+    if (a.dx && per * 16 <= kSliceMost) return rows_launch<EPI_POLICY, true>(a, dtype, ent, ctas, int(per), st);
+    e = forward_launch<EPI_POLICY>(a, dtype, ent, st);
+    return e == cudaSuccess && a.dx ? logprobs_grad_launch(a, dtype, st) : e;
 }
 
 cudaError_t preference_launch(const LossArgs& a, const PairArgs& p, int dtype, float* loss, cudaStream_t st) {
