@@ -56,59 +56,67 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
 // softmax statistics
 // ---------------------------------------------------------------------------------------------------------------
 
-// c = inv_t log2 e in two floats, hi rounded down so that lo >= 0 (a difference of -inf keeps its sign in both products).  With one
-// float the exponents of a whole row are off in the same direction, by up to 6e-8 of their size: a bias of some 3e-7 in
-// every log-probability, which sums over a sequence do not average out.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// c = inv_t log2 e in two floats, hi rounded down so that lo >= 0 (a logit of -inf keeps its sign in both products).  With one float
+// the exponents of a whole row are off in the same direction, by up to 6e-8 of their size: a bias of some 3e-7 in every
+// log-probability, which sums over a sequence do not average out.
+// most: logits are clamped to +-most where a reference is made of them, so that most * c stays finite.
 struct Scale {
-    float hi, lo;
+    float hi, lo, most;
 };
 __device__ __forceinline__ Scale scale_of(float inv_t) {
     const double c = double(inv_t) * 1.4426950408889634;
     Scale r;
     r.hi = __double2float_rd(c);
     r.lo = fmaxf(float(c - double(r.hi)), 1e-37f);
+    r.most = fminf(1e37f / r.hi, FLT_MAX);
     return r;
 }
+// the reference exponent of a maximum
+__device__ __forceinline__ float ref_of(float m, const Scale& c) { return fminf(fmaxf(m, -c.most), c.most) * c.hi; }
 
-// Partial statistics of a set of logits: m their maximum (-inf without one), s - e = sum 2^((x - r) c) (e: what Kahan's sum owes),
-// q = sum of the same terms times their exponent (x - r) c, with the reference r = max(m, -FLT_MAX).  (The exponent is formed
-// from the difference, not as x c - r c: rows of the type's lowest values stay exact, and so does the term of the maximum.)
+// Partial statistics of a set of logits: m their maximum (-inf without one), e = ref_of(m), s - k = sum 2^(x c - e) (k: what
+// Kahan's sum owes), q = sum of the same terms times their exponent.  The exponent is one fused multiply-add from the logit; that e is a
+// rounded product shifts all terms of a row by the same factor, which row_sum() takes out again.
 // A plain float sum is not enough: in the thread that meets the row's peak every later term is rounded to the peak's last
 // bits, 300 times in a row of 151936, all of it landing in the log-probability (measured: 4e-7).
 struct Soft {
-    float m = -INFINITY, s = 0.f, q = 0.f, e = 0.f;
+    float m, e, s, k, q;
 };
-__device__ __forceinline__ float ref_of(float m) { return fmaxf(m, -FLT_MAX); }
+__device__ __forceinline__ Soft soft_empty(const Scale& c) { return Soft{-INFINITY, ref_of(-INFINITY, c), 0.f, 0.f, 0.f}; }
 
 template <bool ENT>
-__device__ __forceinline__ void raise(Soft& a, float m, Scale c) {  // moves a's reference to that of m >= a.m
-    const float d = ref_of(a.m) - ref_of(m), t = fmaf(d, c.lo, d * c.hi), f = ex2_approx(t);
-    if (a.s == 0.f) a.q = 0.f;
-    else if (ENT) a.q = f * fmaf(fmaxf(t, -1000.f), a.s, a.q);
-    a.s = a.s == 0.f ? 0.f : a.s * f;
-    a.e *= f;
-    a.m = m;
+__device__ __forceinline__ void raise(Soft& a, float m, const Scale& c) {  // moves a's reference to that of m >= a.m
+    const float e = ref_of(m, c), t = a.e - e, f = ex2_approx(t);
+    if (ENT) a.q = f * fmaf(fmaxf(t, -1000.f), a.s, a.q);
+    a.s *= f, a.k *= f;
+    a.m = m, a.e = e;
 }
 // N logits: their terms are summed as a tree, the tree's sum goes into the thread's by Kahan's rule
 template <bool ENT, int N>
-__device__ __forceinline__ void add_many(Soft& a, const float (&x)[N], Scale c) {
+__device__ __forceinline__ void add_many(Soft& a, const float (&x)[N], const Scale& c) {
     float m = x[0];
 #pragma unroll
-    for (int i = 1; i < N; ++i) m = fmaxf(m, x[i]);
+    for (int i = 1; i + 1 < N; i += 2) m = max3(m, x[i], x[i + 1]);
+    if (N % 2 == 0) m = fmaxf(m, x[N - 1]);
     if (m > a.m) raise<ENT>(a, m, c);
-    const float r = ref_of(a.m);
     float sum, qs = 0.f;
     if (N == 1) {
-        const float d = x[0] - r, t = fmaf(d, c.lo, d * c.hi);
+        const float t = fmaf(x[0], c.hi, fmaf(x[0], c.lo, -a.e));
         sum = ex2_approx(t);
         if (ENT) qs = sum * fmaxf(t, -1000.f);
     } else {
-        const F2 nr = f2(-r, -r), hi = f2(c.hi, c.hi), lo = f2(c.lo, c.lo);
+        const F2 ne = f2(-a.e, -a.e), hi = f2(c.hi, c.hi), lo = f2(c.lo, c.lo);
         F2 w[N / 2 > 0 ? N / 2 : 1], q = f2(0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) {
-            const F2 d = add2(f2(x[2 * i], x[2 * i + 1]), nr);
-            const float2 t = split(fma2(d, lo, mul2(d, hi)));
+            const F2 v = f2(x[2 * i], x[2 * i + 1]);
+            const float2 t = split(fma2(v, hi, fma2(v, lo, ne)));
             w[i] = f2(ex2_approx(t.x), ex2_approx(t.y));
             if (ENT) q = fma2(w[i], f2(fmaxf(t.x, -1000.f), fmaxf(t.y, -1000.f)), q);  // (0 * -inf is not what a forbidden token adds)
         }
@@ -120,8 +128,8 @@ __device__ __forceinline__ void add_many(Soft& a, const float (&x)[N], Scale c) 
         sum = p.x + p.y;
         if (ENT) qs = v.x + v.y;
     }
-    const float y = __fsub_rn(sum, a.e), t = __fadd_rn(a.s, y);
-    a.e = __fsub_rn(__fsub_rn(t, a.s), y);
+    const float y = __fsub_rn(sum, a.k), t = __fadd_rn(a.s, y);
+    a.k = __fsub_rn(__fsub_rn(t, a.s), y);
     a.s = t;
     if (ENT) a.q += qs;
 }
@@ -132,7 +140,7 @@ __device__ __forceinline__ void add_many(Soft& a, const float (&x)[N], Scale c) 
 struct ReduceShared {
     float m[32];
     float2 sq[32];
-    float4 part[16];  // one per CTA of the cluster
+    float4 part[2][16];  // one per CTA of the cluster; a second set for a second reduction
 };
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -144,19 +152,24 @@ __device__ __forceinline__ uint32_t cluster_size() {
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
     return r;
 }
+__device__ __forceinline__ float warp_max_f(float v) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
 __device__ __forceinline__ float warp_sum_f(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 template <bool ENT>
-__device__ __forceinline__ Soft reduce(Soft a, Scale c, ReduceShared& sh, int ctas) {
+__device__ __forceinline__ Soft reduce(Soft a, const Scale& c, ReduceShared& sh, int ctas, int turn) {
     const int w = threadIdx.x >> 5, nw = blockDim.x >> 5, lane = lane_id();
-    a.s -= a.e, a.e = 0.f;
-    float m = warp_max(a.m);
+    a.s -= a.k, a.k = 0.f;
+    float m = warp_max_f(a.m);
     if (lane == 0) sh.m[w] = m;
     __syncthreads();
-    m = warp_max(lane < nw ? sh.m[lane] : -INFINITY);
+    m = warp_max_f(lane < nw ? sh.m[lane] : -INFINITY);
     raise<ENT>(a, m, c);
     a.s = warp_sum_f(a.s);
     if (ENT) a.q = warp_sum_f(a.q);
@@ -170,14 +183,14 @@ __device__ __forceinline__ Soft reduce(Soft a, Scale c, ReduceShared& sh, int ct
     if (ctas > 1) {
         if (w == 0 && lane < ctas) {  // lane i tells CTA i
             uint32_t to;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(&sh.part[cluster_rank()])), "r"(lane));
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(&sh.part[turn][cluster_rank()])), "r"(lane));
             asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(m), "f"(a.s), "f"(a.q), "f"(0.f) : "memory");
         }
         asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
         if (w == 0) {
-            const float4 p = lane < ctas ? sh.part[lane] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
-            a.m = p.x, a.s = p.y, a.q = p.z;
-            m = warp_max(a.m);
+            const float4 p = lane < ctas ? sh.part[turn][lane] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+            a.m = p.x, a.e = ref_of(p.x, c), a.s = p.y, a.q = p.z;
+            m = warp_max_f(a.m);
             raise<ENT>(a, m, c);
             a.s = warp_sum_f(a.s);
             if (ENT) a.q = warp_sum_f(a.q);
@@ -185,6 +198,20 @@ __device__ __forceinline__ Soft reduce(Soft a, Scale c, ReduceShared& sh, int ct
     }
     return a;
 }
+
+// the same for a far row's thread sums, all relative to the row's maximum m
+template <bool ENT>
+__device__ __forceinline__ Soft reduce_far(Soft a, float m, ReduceShared& sh, int ctas) {
+    Scale one{1.f, 0.f, FLT_MAX};
+    a.m = 0.f, a.e = 0.f;  // (references alike: nothing is scaled)
+    a = reduce<ENT>(a, one, sh, ctas, 1);
+    a.m = m;
+    return a;
+}
+
+// A row whose maximum is so large that its reference was clamped, or so low (rows of the type's lowest value) that its terms
+// vanished: exponents from the differences to the maximum, which is known by then.  Thread sums only.
+__device__ __forceinline__ bool is_far(const Soft& a) { return a.m >= -FLT_MAX && a.m <= FLT_MAX && !(a.s > 0.f && a.s <= FLT_MAX); }
 
 // ---------------------------------------------------------------------------------------------------------------
 // reading and writing logits
@@ -230,48 +257,67 @@ __device__ __forceinline__ int head_of(const T* p, int n) {
 // one row's scalars
 // ---------------------------------------------------------------------------------------------------------------
 
-// The row's gradient: dx_j = w_j * (a + b * t_j), + d on the token, with t_j = (x_j - r) c and w_j = 2^t_j.
-//   -inv_t g p_j - inv_t h p_j (log p_j + H),  p_j = w_j / sum,  log p_j = ln 2 t_j - log sum
-//   => a = -(inv_t / sum) (g + h (H - log sum)),  b = -(inv_t / sum) h ln 2
+constexpr double kLn2 = 0.6931471805599453;
+
+// 2^(e - m c): what the rounded reference e of a row with maximum m puts into its sum.  Doubles: m c has to be exact to the last bits
+// of e.
+__device__ __forceinline__ double shift_of(double m, double e, double c) {
+    const double y = kLn2 * (e - m * c);
+    return fabs(y) < 1e-3 ? 1.0 + y * (1.0 + y * (0.5 + y * (1.0 / 6.0))) : exp(y);
+}
+
+// The row's gradient: dx_j = w_j * (a + b * t_j), + d on the token, with t_j = x_j c - e (far: (x_j - e) c) and w_j = 2^t_j, whose sum
+// over the row is s:
+//   -inv_t g p_j - inv_t h p_j (log p_j + H),  p_j = w_j / s,  log p_j = ln 2 t_j - log s
+//   => a = -(inv_t / s) (g + h (H - log s)),  b = -(inv_t / s) h ln 2
 struct GradRow {
-    float r, c, a, b, d;
+    float e, c, a, b, d;
     int token;
+    bool far;
 };
-__device__ __forceinline__ GradRow grad_row(float m, double sum, double inv_t, int token, double g, double h, double entropy) {
-    const double k = inv_t / sum;
+// sum: over exp((x - m) inv_t), m the row's maximum
+__device__ __forceinline__ GradRow grad_row(float m, double sum, float inv_t, int token, double g, double h, double entropy) {
     GradRow q;
-    q.r = ref_of(m), q.c = float(inv_t) * kLog2e, q.token = token;
-    q.a = float(-k * (g + (h == 0.0 ? 0.0 : h * (entropy - log(sum)))));
-    q.b = float(-k * h * 0.6931471805599453);
-    q.d = float(inv_t * g);
+    q.c = inv_t * kLog2e, q.token = token;
+    const float most = fminf(1e37f / q.c, FLT_MAX);
+    q.far = !(m >= -most && m <= most);
+    q.e = q.far ? m : m * q.c;
+    const double s = q.far ? sum : sum / shift_of(m, q.e, q.c), k = double(inv_t) / s;
+    q.a = float(-k * (g + (h == 0.0 ? 0.0 : h * (entropy - log(s)))));
+    q.b = float(-k * h * kLn2);
+    q.d = float(double(inv_t) * g);
     return q;
 }
+template <bool ENT>
+__device__ __forceinline__ float grad_of(const GradRow& q, float x) {
+    const float t = q.far ? (x - q.e) * q.c : fmaf(x, q.c, -q.e), w = ex2_approx(t);
+    return ENT ? w * fmaf(q.b, fmaxf(t, -1000.f), q.a) : w * q.a;
+}
 template <bool ENT, int N>
-__device__ __forceinline__ void grad_many(const GradRow& q, float (&x)[N], int at) {  // at: the token's place, outside [0, N) elsewhere
-    const F2 nr = f2(-q.r, -q.r), c = f2(q.c, q.c), a = f2(q.a, q.a), b = f2(q.b, q.b);
+__device__ __forceinline__ void grad_many(const GradRow& q, float (&x)[N]) {  // (not for a far row)
+    const F2 ne = f2(-q.e, -q.e), c = f2(q.c, q.c), a = f2(q.a, q.a), b = f2(q.b, q.b);
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
-        const float2 t = split(mul2(add2(f2(x[i], x[i + 1]), nr), c));
+        const float2 t = split(fma2(f2(x[i], x[i + 1]), c, ne));
         const F2 w = f2(ex2_approx(t.x), ex2_approx(t.y));
         const float2 v = split(ENT ? mul2(w, fma2(b, f2(fmaxf(t.x, -1000.f), fmaxf(t.y, -1000.f)), a)) : mul2(w, a));
         x[i] = v.x, x[i + 1] = v.y;
     }
-    if (unsigned(at) < unsigned(N)) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] += i == at ? q.d : 0.f;
-    }
 }
-template <bool ENT>
-__device__ __forceinline__ float grad_of(const GradRow& q, float x) {
-    const float t = (x - q.r) * q.c, w = ex2_approx(t);
-    return ENT ? w * fmaf(q.b, fmaxf(t, -1000.f), q.a) : w * q.a;
+// one vector of a row's gradient
+template <typename T, bool ENT>
+__device__ __forceinline__ uint4 grad_vec(const GradRow& q, uint4 v) {
+    float e[16 / sizeof(T)];
+    unpack<T>(v, e);
+    grad_many<ENT, 16 / sizeof(T)>(q, e);
+    return pack<T>(e);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// forward: one CTA per row
+// rows: statistics, what a call wants of them, and (with GRAD) the gradient
 // ---------------------------------------------------------------------------------------------------------------
 
-constexpr int kFwdThreads = 512, kFusedThreads = 256;
+constexpr int kRowThreads = 256;
 constexpr int kSliceMost = 200 * 1024;  // bytes of a row's slice that a CTA can hold
 
 // the row as a user's call describes it, and whether it counts
@@ -326,22 +372,26 @@ __device__ PolicyRow policy_row(const LossArgs& a, int row, double logp, double 
     return p;
 }
 
-// What a row comes to; with `write`, what the call wants of it is written.  One thread.
+// What a row comes to; with `write`, what the call wants of it is written.  One thread.  s: the row's statistics, of which s.s may be
+// relative to a rounded reference (far: to the maximum itself).
 struct RowDone {
     double sum, entropy, g, h;
 };
 template <int EPI, bool ENT>
-__device__ RowDone finish_row(const LossArgs& a, int row, bool write, bool live, int token, float inv_t, float x_token, const Soft& s) {
+__device__ __noinline__ RowDone finish_row(const LossArgs& a, int row, bool write, bool live, int token, float inv_t, float x_token, float m, float e,
+                                           float s, float q, bool far) {
     RowDone done{};
     double logp = 0.0, entropy = 0.0, sum = 0.0;
-    float m = 0.f;
     if (live) {
-        m = s.m;
+        const double c = double(inv_t) * 1.4426950408889634;
         // a row without a finite maximum has no distribution
-        sum = (m >= -FLT_MAX && m <= FLT_MAX) ? double(s.s) : double(NAN);
+        sum = (m >= -FLT_MAX && m <= FLT_MAX) ? (far ? double(s) : double(s) * shift_of(m, e, c)) : double(NAN);
         const double ls = log(sum);
         logp = (double(x_token) - double(m)) * double(inv_t) - ls;
-        if (ENT) entropy = ls - 0.6931471805599453 * double(s.q) / sum;
+        // the terms' mean exponent is q / s from the reference, and e - m c more from the maximum
+        if (ENT) entropy = ls - kLn2 * (double(q) / double(s) + (far ? 0.0 : double(e) - double(m) * c));
+    } else {
+        m = 0.f;
     }
     done.sum = sum, done.entropy = entropy;
     if (EPI != EPI_POLICY && !write) return done;
@@ -403,20 +453,69 @@ __device__ void last_sum(const LossArgs& a) {
 __device__ __forceinline__ void copy_async16(void* smem, const void* g) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem)), "l"(g) : "memory");
 }
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
-__device__ __forceinline__ void copies_but(int = 0) {  // waits for this thread's copies but its last N groups
+__device__ __forceinline__ void copies_but() {  // waits for this thread's copies but its last N groups
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// 16 logits of one thread, in V vectors `stride` apart
+template <typename T, bool ENT>
+__device__ __forceinline__ void add_block(Soft& s, const uint4* v, int stride, const Scale& c) {
+    constexpr int E = 16 / sizeof(T), V = 16 / E;
+    float x[16];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        float e[E];
+        unpack<T>(v[k * stride], e);
+#pragma unroll
+        for (int j = 0; j < E; ++j) x[k * E + j] = e[j];
+    }
+    add_many<ENT, 16>(s, x, c);
+}
+template <typename T, bool ENT>
+__device__ __forceinline__ void add_vec(Soft& s, uint4 v, const Scale& c) {
+    float e[16 / sizeof(T)];
+    unpack<T>(v, e);
+    add_many<ENT, 16 / sizeof(T)>(s, e, c);
+}
+// a far row's thread sums (see is_far); m: the row's maximum
+template <typename T, bool ENT>
+__device__ __noinline__ Soft far_sums(const uint4* v, int cnt, bool have_edge, float x_edge, float m, float c) {
+    constexpr int E = 16 / sizeof(T);
+    Soft a{m, 0.f, 0.f, 0.f, 0.f};
+    for (int i = threadIdx.x; i < cnt; i += blockDim.x) {
+        float x[E];
+        unpack<T>(v[i], x);
+        for (int j = 0; j < E; ++j) {
+            const float t = (x[j] - m) * c, w = ex2_approx(t);
+            a.s += w;
+            if (ENT) a.q = fmaf(w, fmaxf(t, -1000.f), a.q);
+        }
+    }
+    if (have_edge) {
+        const float t = (x_edge - m) * c, w = ex2_approx(t);
+        a.s += w;
+        if (ENT) a.q = fmaf(w, fmaxf(t, -1000.f), a.q);
+    }
+    return a;
+}
+
+// vectors that a thread of the forward kernel has under way: kFwdRing steps of 16 logits each
+template <typename T>
+constexpr int kFwdRing = sizeof(T) == 4 ? 4 : 8;
+
 // One cluster per row, each CTA a contiguous slice of `per` 16-byte vectors; the scalars before the first and behind the last
-// boundary belong to rank 0, one per thread.
+// boundary belong to rank 0, one per thread.  A thread reads only what it copied into shared memory itself, so that the copies
+// need no barrier.
 template <typename T, int EPI, bool ENT, bool GRAD>
-__global__ void __launch_bounds__(GRAD ? kFusedThreads : kFwdThreads, GRAD ? 5 : 3) rows_kernel(LossArgs a, int per) {
-    constexpr int E = 16 / sizeof(T), NT = GRAD ? kFusedThreads : kFwdThreads;
-    extern __shared__ __align__(16) uint4 slice[];  // GRAD: this CTA's part of the row
+__global__ void __launch_bounds__(kRowThreads, GRAD ? 5 : 3) rows_kernel(const __grid_constant__ LossArgs a, int per) {
+    constexpr int E = 16 / sizeof(T), NT = kRowThreads, V = 16 / E;
+    extern __shared__ __align__(16) uint4 slice[];  // GRAD: this CTA's part of the row; else a ring of what is under way
     __shared__ ReduceShared sh;
     __shared__ GradRow s_q;
     __shared__ bool s_zero;
+    __shared__ float s_m;
     const int ctas = int(cluster_size()), rank = int(cluster_rank()), tid = threadIdx.x;
     const int row = int(blockIdx.x / unsigned(ctas));
     const RowOf w = row_of(a, row);
@@ -426,69 +525,75 @@ __global__ void __launch_bounds__(GRAD ? kFusedThreads : kFwdThreads, GRAD ? 5 :
     const uint4* v = reinterpret_cast<const uint4*>(x + head) + v0;
     const int my_edge = rank == 0 && tid < edge ? (tid < head ? tid : tid + nv * E) : -1;  // (edge < 2 E <= NT)
     float x_edge = 0.f;
-    GradRow q{};
-    bool zero = true;
+    bool zero = true, far = false;
     if (w.live) {
         const Scale c = scale_of(w.inv_t);
-        Soft s;
+        Soft s = soft_empty(c);
         float x_token = 0.f;
         if (GRAD) {
-            const int quarter = (cnt + 4 * NT - 1) / (4 * NT);
-            for (int g = 0, i = tid; g < 4; ++g) {
-                for (int k = 0; k < quarter; ++k, i += NT)
-                    if (i < cnt) copy_async16(slice + i, v + i);
-                asm volatile("cp.async.commit_group;" ::: "memory");
-            }
-            if (tid == 0) x_token = load_one(x + w.token);
-            if (my_edge >= 0) {
-                x_edge = load_one(x + my_edge);
-                const float e[1] = {x_edge};
-                add_many<ENT, 1>(s, e, c);
-            }
-            for (int g = 0, i = tid; g < 4; ++g) {  // (each thread reads what it copied itself: no barrier)
-                if (g == 0) copies_but<3>();
-                else if (g == 1) copies_but<2>();
-                else if (g == 2) copies_but<1>();
-                else copies_but<0>();
-                for (int k = 0; k < quarter; ++k, i += NT)
-                    if (i < cnt) {
-                        float e[E];
-                        unpack<T>(slice[i], e);
-                        add_many<ENT, E>(s, e, c);
-                    }
-            }
+#pragma unroll 4
+            for (int i = tid; i < cnt; i += NT) copy_async16(slice + i, v + i);
+            copies_commit();
         } else {
-            if (tid == 0) x_token = load_one(x + w.token);
-            if (my_edge >= 0) {
-                const float e[1] = {load_one(x + my_edge)};
-                add_many<ENT, 1>(s, e, c);
-            }
-            int i = tid;
-            for (; i + 3 * NT < cnt; i += 4 * NT) {
-                const uint4 b[4] = {v[i], v[i + NT], v[i + 2 * NT], v[i + 3 * NT]};
+#pragma unroll 1
+            for (int k = 0; k < kFwdRing<T> - 1; ++k) {
 #pragma unroll
-                for (int k = 0; k < 4; k += 8 / E) {
-                    float e[8];
-                    if (E == 8) unpack<uint16_t>(b[k], e);
-                    else {
-                        float lo[4], hi[4];
-                        unpack<float>(b[k], lo), unpack<float>(b[(k + 1) & 3], hi);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) e[j] = lo[j], e[j + 4] = hi[j];
-                    }
-                    add_many<ENT, 8>(s, e, c);
+                for (int j = 0; j < V; ++j) {
+                    const int i = (k * V + j) * NT + tid;
+                    if (i < cnt) copy_async16(slice + i, v + i);
                 }
-            }
-            for (; i < cnt; i += NT) {
-                float e[E];
-                unpack<T>(v[i], e);
-                add_many<ENT, E>(s, e, c);
+                copies_commit();
             }
         }
-        s = reduce<ENT>(s, c, sh, ctas);
+        if (tid == 0) x_token = load_one(x + w.token);
+        if (my_edge >= 0) {
+            x_edge = load_one(x + my_edge);
+            const float e[1] = {x_edge};
+            add_many<ENT, 1>(s, e, c);
+        }
+        if (GRAD) {
+            copies_but<0>();
+            int i = tid;
+#pragma unroll 1
+            for (; i + (V - 1) * NT < cnt; i += V * NT) add_block<T, ENT>(s, slice + i, NT, c);
+#pragma unroll 1
+            for (; i < cnt; i += NT) add_vec<T, ENT>(s, slice[i], c);
+        } else {
+            constexpr int D = kFwdRing<T>;
+            int slot = 0;  // of the step at hand; the one before it is where the next copies go
+#pragma unroll 1
+            for (int i = tid; i < cnt; i += V * NT) {
+                const int to = slot == 0 ? D - 1 : slot - 1;
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const int k = i + ((D - 1) * V + j) * NT;
+                    if (k < cnt) copy_async16(slice + (to * V + j) * NT + tid, v + k);
+                }
+                copies_commit();
+                copies_but<D - 1>();
+                const uint4* b = slice + slot * V * NT + tid;
+                if (i + (V - 1) * NT < cnt) {
+                    add_block<T, ENT>(s, b, NT, c);
+                } else {
+                    for (int j = 0; i + j * NT < cnt; ++j) add_vec<T, ENT>(s, b[j * NT], c);
+                }
+                slot = slot + 1 == D ? 0 : slot + 1;
+            }
+            copies_but<0>();
+        }
+        s = reduce<ENT>(s, c, sh, ctas, 0);
+        if (tid < 32) far = is_far(s);
+        if (__syncthreads_or(tid == 0 && far)) {  // (every CTA of the cluster has the same statistics)
+            if (tid == 0) s_m = s.m;
+            __syncthreads();
+            const float m = s_m;
+            s = far_sums<T, ENT>(GRAD ? slice : v, cnt, my_edge >= 0, x_edge, m, c.hi);
+            s = reduce_far<ENT>(s, m, sh, ctas);
+            far = true;
+        }
         if (tid == 0) {
             grid_dependency_wait();  // row_scale_kernel's results; row_scale and the ticket are read below
-            const RowDone d = finish_row<EPI, ENT>(a, row, rank == 0, true, w.token, w.inv_t, x_token, s);
+            const RowDone d = finish_row<EPI, ENT>(a, row, rank == 0, true, w.token, w.inv_t, x_token, s.m, s.e, s.s, s.q, far);
             if (GRAD) {
                 s_zero = d.g == 0.0 && d.h == 0.0;
                 s_q = grad_row(s.m, d.sum, w.inv_t, w.token, d.g, d.h, d.entropy);
@@ -497,35 +602,36 @@ __global__ void __launch_bounds__(GRAD ? kFusedThreads : kFwdThreads, GRAD ? 5 :
         if (GRAD) {
             __syncthreads();
             zero = s_zero;
-            if (!zero) q = s_q;
         }
     } else if (tid == 0) {
         grid_dependency_wait();
-        if (rank == 0) finish_row<EPI, ENT>(a, row, true, false, w.token, w.inv_t, 0.f, Soft{});
+        if (rank == 0) finish_row<EPI, ENT>(a, row, true, false, w.token, w.inv_t, 0.f, 0.f, 0.f, 0.f, 0.f, false);
     }
     if (GRAD) {
+        GradRow q{};
+        if (!zero) q = s_q;
         T* dx = static_cast<T*>(a.dx) + int64_t(row) * a.ld_dx;
         if (my_edge >= 0) store_one(dx + my_edge, zero ? 0.f : grad_of<ENT>(q, x_edge) + (my_edge == q.token ? q.d : 0.f));
         const bool vec = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
         T* body = dx + head + int64_t(v0) * E;
-        const int at = zero ? -1 : q.token - head - v0 * E;
-        for (int i = tid; i < cnt; i += NT) {
-            uint4 o = make_uint4(0, 0, 0, 0);
-            if (!zero) {
+        uint4* out = reinterpret_cast<uint4*>(body);
+        if (zero && vec) {
+#pragma unroll 4
+            for (int i = tid; i < cnt; i += NT) __stcs(out + i, make_uint4(0, 0, 0, 0));
+        } else if (vec && !q.far) {
+#pragma unroll 2
+            for (int i = tid; i < cnt; i += NT) __stcs(out + i, grad_vec<T, ENT>(q, slice[i]));
+        } else {
+            for (int i = tid; i < cnt; i += NT) {
                 float e[E];
-                unpack<T>(slice[i], e);
-                grad_many<ENT, E>(q, e, at - i * E);
-                o = pack<T>(e);
-            }
-            if (vec) {
-                __stcs(reinterpret_cast<uint4*>(body) + i, o);
-            } else {
-                float e[E];
-                unpack<T>(o, e);
-#pragma unroll
-                for (int k = 0; k < E; ++k) store_one(body + int64_t(i) * E + k, e[k]);
+                unpack<T>(zero ? make_uint4(0, 0, 0, 0) : slice[i], e);
+#pragma unroll 1
+                for (int k = 0; k < E; ++k) store_one(body + int64_t(i) * E + k, zero ? 0.f : grad_of<ENT>(q, load_one(reinterpret_cast<const T*>(slice + i) + k)));
             }
         }
+        // the token's own element, by the thread that wrote it
+        const int at = zero ? -1 : q.token - head - v0 * E;
+        if (at >= 0 && at < cnt * E && (at / E) % NT == tid) store_one(body + at, grad_of<ENT>(q, load_one(reinterpret_cast<const T*>(slice) + at)) + q.d);
     }
     if (EPI == EPI_POLICY && rank == 0) last_sum(a);
 }
@@ -537,8 +643,8 @@ __global__ void __launch_bounds__(GRAD ? kFusedThreads : kFwdThreads, GRAD ? 5 :
 constexpr int kGradThreads = 256;
 
 template <typename T, bool ENT>
-__global__ void __launch_bounds__(kGradThreads) grad_kernel(LossArgs a, int chunk) {
-    constexpr int E = 16 / sizeof(T);
+__global__ void __launch_bounds__(kGradThreads) grad_kernel(const __grid_constant__ LossArgs a, int chunk) {
+    constexpr int E = 16 / sizeof(T), NT = kGradThreads;
     __shared__ GradRow s_q;
     __shared__ bool s_zero;
     const int row = blockIdx.x, tid = threadIdx.x;
@@ -560,30 +666,34 @@ __global__ void __launch_bounds__(kGradThreads) grad_kernel(LossArgs a, int chun
     const bool zero = s_zero;
     GradRow q{};
     if (!zero) q = s_q;
-    const int at = zero ? -1 : int(int64_t(q.token) - j0 < 0 || int64_t(q.token) - j0 >= n ? -1 : int64_t(q.token) - j0);
-    const bool vec = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
+    const bool vec = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0 && !q.far;
     const int head = vec ? head_of(x, n) : n, nv = (n - head) / E;
     const uint4* v = reinterpret_cast<const uint4*>(x + head);
     uint4* dv = reinterpret_cast<uint4*>(dx + head);
+    const int64_t t64 = zero ? -1 : int64_t(q.token) - j0;
+    const int at = t64 >= 0 && t64 < n ? int(t64) : -1;
+    // the token's own logit, before anything is written (dx may be x)
+    const int t_vec = at - head;
+    const bool mine = at >= head && t_vec < nv * E && (t_vec / E) % NT == tid;
+    const float x_token = mine ? load_one(x + at) : 0.f;
+    if (zero) {
 #pragma unroll 4
-    for (int i = tid; i < nv; i += kGradThreads) {
-        float e[E];
-        if (zero) {
-            dv[i] = make_uint4(0, 0, 0, 0);
-        } else {
-            unpack<T>(v[i], e);
-            grad_many<ENT, E>(q, e, at - head - i * E);
-            dv[i] = pack<T>(e);
+        for (int i = tid; i < nv; i += NT) __stcs(dv + i, make_uint4(0, 0, 0, 0));
+    } else {
+        int i = tid;
+#pragma unroll 1
+        for (; i + 3 * NT < nv; i += 4 * NT) {
+            const uint4 b[4] = {v[i], v[i + NT], v[i + 2 * NT], v[i + 3 * NT]};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) __stcs(dv + i + k * NT, grad_vec<T, ENT>(q, b[k]));
         }
+#pragma unroll 1
+        for (; i < nv; i += NT) __stcs(dv + i, grad_vec<T, ENT>(q, v[i]));
     }
-    for (int i = tid; i < head + (n - head - nv * E); i += kGradThreads) {
+    if (mine) store_one(dx + at, grad_of<ENT>(q, x_token) + q.d);
+    for (int i = tid; i < head + (n - head - nv * E); i += NT) {
         const int j = i < head ? i : i + nv * E;
-        float e = 0.f;
-        if (!zero) {
-            e = grad_of<ENT>(q, load_one(x + j));
-            if (j == at) e += q.d;
-        }
-        store_one(dx + j, e);
+        store_one(dx + j, zero ? 0.f : grad_of<ENT>(q, load_one(x + j)) + (j == at ? q.d : 0.f));
     }
 }
 
@@ -705,14 +815,14 @@ cudaError_t rows_launch(const LossArgs& a, int ctas, int per, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     auto* const f = rows_kernel<T, EPI, ENT, GRAD>;
     if (dev > 63 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {
-        if (GRAD) e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+        e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
         if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_release);
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(a.rows) * unsigned(ctas)), cfg.blockDim = dim3(GRAD ? kFusedThreads : kFwdThreads), cfg.stream = st;
-    cfg.dynamicSmemBytes = GRAD ? size_t(per) * 16 : 0;
+    cfg.gridDim = dim3(unsigned(a.rows) * unsigned(ctas)), cfg.blockDim = dim3(kRowThreads), cfg.stream = st;
+    cfg.dynamicSmemBytes = GRAD ? size_t(per) * 16 : size_t(kFwdRing<T>) * 16 * sizeof(T) * kRowThreads;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = unsigned(ctas), at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
@@ -735,7 +845,7 @@ template <int EPI>
 cudaError_t forward_launch(const LossArgs& a, int dtype, bool ent, cudaStream_t st) {
     const int nv = vectors_of(a.n, dtype);
     int ctas = 1;
-    while (ctas < 16 && int64_t(a.rows) * ctas < 592 && nv / (2 * ctas) >= kFwdThreads) ctas *= 2;
+    while (ctas < 16 && int64_t(a.rows) * ctas < 888 && nv / (2 * ctas) >= 2 * kRowThreads) ctas *= 2;
     if (const char* v = getenv("WB_CF")) ctas = atoi(v);
     return rows_launch<EPI, false>(a, dtype, ent, ctas, (nv + ctas - 1) / ctas, st);
 }
@@ -769,7 +879,7 @@ cudaError_t policy_launch(const LossArgs& a, int dtype, int mean, cudaStream_t s
     int ctas = 1, most = 44 * 1024;
     if (const char* v = getenv("WB_SL")) most = atoi(v) * 1024;
     while (ctas < 16 && int64_t(nv + ctas - 1) / ctas * 16 > most) ctas *= 2;
-    while (ctas < 16 && int64_t(a.rows) * ctas < 592 && nv / (2 * ctas) >= kFusedThreads) ctas *= 2;
+    while (ctas < 16 && int64_t(a.rows) * ctas < 592 && nv / (2 * ctas) >= kRowThreads) ctas *= 2;
     if (const char* v = getenv("WB_CG")) ctas = atoi(v);
     const int64_t per = (int64_t(nv) + ctas - 1) / ctas;
     if (a.dx && per * 16 <= kSliceMost) return rows_launch<EPI_POLICY, true>(a, dtype, ent, ctas, int(per), st);
