@@ -575,12 +575,12 @@ def _loss_rows(x: torch.Tensor):
     return _dtype(x), rows, n, (s0 if rows > 1 else n)
 
 
-def _vec(t: Optional[torch.Tensor], name: str, dtype, shape, x: torch.Tensor):
-    """The address of a contiguous tensor of the given type and shape on x's device (None stays None)."""
+def _vec(t: Optional[torch.Tensor], name: str, dtype, shape, dev: int):
+    """The address of a contiguous tensor of the given type and shape on CUDA device `dev` (None stays None)."""
     if t is None:
         return None
-    if t.dtype != dtype or t.device != x.device or t.shape != shape or not t.is_contiguous():
-        raise TypeError(f"{name}: want a contiguous {dtype} tensor of shape {tuple(shape)} on {x.device}, got {t.dtype} {tuple(t.shape)} "
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+        raise TypeError(f"{name}: want a contiguous {dtype} tensor of shape {tuple(shape)} on cuda:{dev}, got {t.dtype} {tuple(t.shape)} "
                         f"on {t.device}")
     return t.data_ptr()
 
@@ -595,13 +595,16 @@ def _grad_out(x: torch.Tensor, dx: Optional[torch.Tensor], ld: int) -> torch.Ten
     return dx
 
 
-def _call(x: torch.Tensor, fn, *args):
-    """fn(*args, stream) with x's device current."""
-    if x.device.index == torch.cuda.current_device():
-        _check(fn(*args, torch.cuda.current_stream(x.device).cuda_stream))
+def _call(dev: int, fn, *args):
+    """fn(*args, stream) on the device's current stream, with that device current.  (The raw calls: a Stream object and a device
+    context cost several microseconds, as much as a small kernel.)"""
+    if dev == torch._C._cuda_getDevice():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
-        with torch.cuda.device(x.device):
-            _check(fn(*args, torch.cuda.current_stream(x.device).cuda_stream))
+        with torch.cuda.device(dev):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if status:
+        _check(status)
 
 
 @dataclass
@@ -616,12 +619,12 @@ def token_logprobs(x, token, inv_t: float = 1.0, inv_t_rows=None, want_entropy: 
     (whirl_token_logprobs).  x [rows, n] float32 / bfloat16, rows may be padded; token [rows] int32.  A row whose token lies
     outside [0, n) is not read and gets zeros."""
     dt, rows, n, ld = _loss_rows(x)
-    f32, rs = torch.float32, (rows,)
-    tok, it = _vec(token, "token", torch.int32, rs, x), _vec(inv_t_rows, "inv_t_rows", f32, rs, x)
-    logp = torch.empty(rows, dtype=f32, device=x.device)
-    stats = torch.empty((rows, 2), dtype=f32, device=x.device)
-    entropy = torch.empty(rows, dtype=f32, device=x.device) if want_entropy else None
-    _call(x, lib.whirl_token_logprobs, x.data_ptr(), dt, rows, n, ld, tok, inv_t, it, logp.data_ptr(), stats.data_ptr(), _p(entropy))
+    f32, rs, dev = torch.float32, (rows,), x.get_device()
+    tok, it = _vec(token, "token", torch.int32, rs, dev), _vec(inv_t_rows, "inv_t_rows", f32, rs, dev)
+    logp = torch.empty(rows, dtype=f32, device=dev)
+    stats = torch.empty((rows, 2), dtype=f32, device=dev)
+    entropy = torch.empty(rows, dtype=f32, device=dev) if want_entropy else None
+    _call(dev, lib.whirl_token_logprobs, x.data_ptr(), dt, rows, n, ld, tok, inv_t, it, logp.data_ptr(), stats.data_ptr(), _p(entropy))
     return LogprobResult(logp, stats, entropy)
 
 
@@ -629,11 +632,11 @@ def token_logprobs_grad(x, token, stats, g_logp, inv_t: float = 1.0, inv_t_rows=
     """The gradient by the logits of a loss whose gradients by logp and (optionally) entropy are g_logp and g_entropy [rows]
     float32 (whirl_token_logprobs_grad).  stats, entropy: what token_logprobs returned.  dx may be x itself."""
     dt, rows, n, ld = _loss_rows(x)
-    f32, rs = torch.float32, (rows,)
-    args = (_vec(token, "token", torch.int32, rs, x), inv_t, _vec(inv_t_rows, "inv_t_rows", f32, rs, x), _vec(stats, "stats", f32, (rows, 2), x),
-            _vec(entropy, "entropy", f32, rs, x), _vec(g_logp, "g_logp", f32, rs, x), _vec(g_entropy, "g_entropy", f32, rs, x))
+    f32, rs, dev = torch.float32, (rows,), x.get_device()
+    args = (_vec(token, "token", torch.int32, rs, dev), inv_t, _vec(inv_t_rows, "inv_t_rows", f32, rs, dev), _vec(stats, "stats", f32, (rows, 2), dev),
+            _vec(entropy, "entropy", f32, rs, dev), _vec(g_logp, "g_logp", f32, rs, dev), _vec(g_entropy, "g_entropy", f32, rs, dev))
     dx = _grad_out(x, dx, ld)
-    _call(x, lib.whirl_token_logprobs_grad, x.data_ptr(), dt, rows, n, ld, *args, dx.data_ptr(), _loss_rows(dx)[3])
+    _call(dev, lib.whirl_token_logprobs_grad, x.data_ptr(), dt, rows, n, ld, *args, dx.data_ptr(), _loss_rows(dx)[3])
     return dx
 
 
@@ -657,24 +660,25 @@ def policy_loss(x, token, adv, old_logp=None, ref_logp=None, weight=None, seq_st
     logits (whirl_policy_loss).  adv, old_logp, ref_logp, weight: [rows] float32 (weight 0: a prompt or padding row, not read);
     seq_start: [seqs + 1] int32, needed by MEAN_SEQS.  dx may be x itself."""
     dt, rows, n, ld = _loss_rows(x)
-    f32, i32, rs, dev = torch.float32, torch.int32, (rows,), x.device
+    f32, i32, rs, dev = torch.float32, torch.int32, (rows,), x.get_device()
     if mean == MEAN_SEQS and (seq_start is None or seq_start.dim() != 1 or seq_start.numel() < 1):
         raise ValueError("policy_loss: MEAN_SEQS needs seq_start [seqs + 1]")
     seqs = 0 if seq_start is None else seq_start.numel() - 1
-    p = PolicyParams(_vec(token, "token", i32, rs, x), _vec(adv, "adv", f32, rs, x), _vec(old_logp, "old_logp", f32, rs, x),
-                     _vec(ref_logp, "ref_logp", f32, rs, x), _vec(weight, "weight", f32, rs, x),
-                     None if seq_start is None else _vec(seq_start, "seq_start", i32, (seqs + 1,), x), seqs, mean,
-                     _vec(inv_t_rows, "inv_t_rows", f32, rs, x), inv_t, clip_low, clip_high, dual_clip, kl_coef, ent_coef)
+    p = PolicyParams(_vec(token, "token", i32, rs, dev), _vec(adv, "adv", f32, rs, dev), _vec(old_logp, "old_logp", f32, rs, dev),
+                     _vec(ref_logp, "ref_logp", f32, rs, dev), _vec(weight, "weight", f32, rs, dev),
+                     None if seq_start is None else _vec(seq_start, "seq_start", i32, (seqs + 1,), dev), seqs, mean,
+                     _vec(inv_t_rows, "inv_t_rows", f32, rs, dev), inv_t, clip_low, clip_high, dual_clip, kl_coef, ent_coef)
     ent, kl = want_entropy or ent_coef != 0.0, ref_logp is not None
-    v = torch.empty((6, rows), dtype=f32, device=dev).unbind(0)
+    new = lambda: torch.empty(rows, dtype=f32, device=dev)  # noqa: E731  (one allocation each: views of a common one cost more)
+    v = new(), new(), new(), new(), new() if ent else None, new() if kl else None
     loss, stats = torch.empty((), dtype=f32, device=dev), torch.empty((rows, 2), dtype=f32, device=dev)
     if want_grad:
         dx = _grad_out(x, dx, ld)
-    r = PolicyResult(loss, v[0], stats, v[4] if ent else None, v[5] if kl else None, v[1], v[2], v[3], dx if want_grad else None)
+    r = PolicyResult(loss, v[0], stats, v[4], v[5], v[1], v[2], v[3], dx if want_grad else None)
     o = PolicyOut(loss.data_ptr(), v[0].data_ptr(), stats.data_ptr(), _p(r.entropy), _p(r.kl), v[1].data_ptr(), v[2].data_ptr(), v[3].data_ptr(),
                   _p(r.dx), _loss_rows(dx)[3] if want_grad else 0)
     ws = torch.empty(lib.whirl_loss_workspace_bytes(rows, seqs), dtype=torch.uint8, device=dev)
-    _call(x, lib.whirl_policy_loss, x.data_ptr(), dt, rows, n, ld, C.byref(p), C.byref(o), ws.data_ptr(), ws.numel())
+    _call(dev, lib.whirl_policy_loss, x.data_ptr(), dt, rows, n, ld, C.byref(p), C.byref(o), ws.data_ptr(), ws.numel())
     return r
 
 
@@ -696,21 +700,21 @@ def preference_loss(x, token, seq_start, ref_logp=None, weight=None, inv_t: floa
     sequence s holds the rows seq_start[s] to seq_start[s + 1]), with its gradient by the logits (whirl_preference_loss).
     ref_logp, weight: [rows] float32.  dx may be x itself."""
     dt, rows, n, ld = _loss_rows(x)
-    f32, i32, rs, dev = torch.float32, torch.int32, (rows,), x.device
+    f32, i32, rs, dev = torch.float32, torch.int32, (rows,), x.get_device()
     if seq_start.dim() != 1 or seq_start.numel() % 2 != 1:
         raise ValueError(f"preference_loss: seq_start is [2 * pairs + 1], got {tuple(seq_start.shape)}")
     pairs = seq_start.numel() // 2
-    p = PreferenceParams(_vec(token, "token", i32, rs, x), _vec(seq_start, "seq_start", i32, (2 * pairs + 1,), x),
-                         _vec(ref_logp, "ref_logp", f32, rs, x), _vec(weight, "weight", f32, rs, x), _vec(inv_t_rows, "inv_t_rows", f32, rs, x),
+    p = PreferenceParams(_vec(token, "token", i32, rs, dev), _vec(seq_start, "seq_start", i32, (2 * pairs + 1,), dev),
+                         _vec(ref_logp, "ref_logp", f32, rs, dev), _vec(weight, "weight", f32, rs, dev), _vec(inv_t_rows, "inv_t_rows", f32, rs, dev),
                          pairs, kind, int(average), inv_t, beta, smoothing, margin)
-    logp, g_logp = torch.empty((2, rows), dtype=f32, device=dev).unbind(0)
+    logp, g_logp = torch.empty(rows, dtype=f32, device=dev), torch.empty(rows, dtype=f32, device=dev)
     pair_loss, reward = torch.empty(pairs, dtype=f32, device=dev), torch.empty((pairs, 2), dtype=f32, device=dev)
     loss, stats = torch.empty((), dtype=f32, device=dev), torch.empty((rows, 2), dtype=f32, device=dev)
     dx = _grad_out(x, dx, ld) if want_grad else None
     o = PreferenceOut(loss.data_ptr(), pair_loss.data_ptr(), reward.data_ptr(), logp.data_ptr(), stats.data_ptr(), g_logp.data_ptr(), _p(dx),
                       _loss_rows(dx)[3] if want_grad else 0)
     ws = torch.empty(lib.whirl_loss_workspace_bytes(rows, pairs), dtype=torch.uint8, device=dev)
-    _call(x, lib.whirl_preference_loss, x.data_ptr(), dt, rows, n, ld, C.byref(p), C.byref(o), ws.data_ptr(), ws.numel())
+    _call(dev, lib.whirl_preference_loss, x.data_ptr(), dt, rows, n, ld, C.byref(p), C.byref(o), ws.data_ptr(), ws.numel())
     return PreferenceResult(loss, pair_loss, reward, logp, stats, g_logp, dx)
 
 
@@ -735,18 +739,22 @@ def block_tables_step(length, n_new, table, owned, free_ids, free_count, block_s
     owned [seqs], table [seqs, max_blocks], free_ids [num_blocks], free_count [1]: int32; the last four are updated."""
     if table.dim() != 2 or not table.is_cuda:
         raise ValueError("block_tables_step: table must be [seqs, max_blocks] on a CUDA device")
-    i32, dev = torch.int32, table.device
+    i32, dev = torch.int32, table.get_device()
     seqs, width = table.shape
+    blocks, ss = free_ids.numel(), (seqs,)
     if rows is None:
-        rows = StepRows(torch.empty(max_rows, dtype=torch.int64, device=dev), *torch.empty((2, max_rows), dtype=i32, device=dev).unbind(0),
-                        torch.empty(seqs + 1, dtype=i32, device=dev), torch.empty(seqs, dtype=i32, device=dev))
-    t = BlockTables(_vec(table, "table", i32, (seqs, width), table), _vec(owned, "owned", i32, (seqs,), table),
-                    _vec(free_ids, "free_ids", i32, (free_ids.numel(),), table), _vec(free_count, "free_count", i32, (1,), table), seqs, width,
-                    free_ids.numel(), block_size)
-    o = StepRowsOut(_vec(rows.slot, "slot", torch.int64, (max_rows,), table), _vec(rows.position, "position", i32, (max_rows,), table),
-                    _vec(rows.seq, "seq", i32, (max_rows,), table), _vec(rows.row0, "row0", i32, (seqs + 1,), table),
-                    _vec(rows.status, "status", i32, (seqs,), table), max_rows)
-    ws = torch.empty(lib.whirl_block_workspace_bytes(seqs), dtype=torch.uint8, device=dev)
-    _call(table, lib.whirl_block_tables_step, _vec(length, "length", i32, (seqs,), table), _vec(n_new, "n_new", i32, (seqs,), table),
-          C.byref(t), C.byref(o), ws.data_ptr(), ws.numel())
+        rows = StepRows(torch.empty(max_rows, dtype=torch.int64, device=dev), torch.empty(max_rows, dtype=i32, device=dev),
+                        torch.empty(max_rows, dtype=i32, device=dev), torch.empty(seqs + 1, dtype=i32, device=dev),
+                        torch.empty(seqs, dtype=i32, device=dev))
+        out = rows.slot.data_ptr(), rows.position.data_ptr(), rows.seq.data_ptr(), rows.row0.data_ptr(), rows.status.data_ptr()
+    else:
+        mr = (max_rows,)
+        out = (_vec(rows.slot, "slot", torch.int64, mr, dev), _vec(rows.position, "position", i32, mr, dev), _vec(rows.seq, "seq", i32, mr, dev),
+               _vec(rows.row0, "row0", i32, (seqs + 1,), dev), _vec(rows.status, "status", i32, ss, dev))
+    t = BlockTables(_vec(table, "table", i32, (seqs, width), dev), _vec(owned, "owned", i32, ss, dev), _vec(free_ids, "free_ids", i32, (blocks,), dev),
+                    _vec(free_count, "free_count", i32, (1,), dev), seqs, width, blocks, block_size)
+    o = StepRowsOut(*out, max_rows)
+    nbytes = lib.whirl_block_workspace_bytes(seqs)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _call(dev, lib.whirl_block_tables_step, _vec(length, "length", i32, ss, dev), _vec(n_new, "n_new", i32, ss, dev), t, o, ws.data_ptr(), nbytes)
     return rows

@@ -40,85 +40,138 @@ __host__ __device__ Plan plan_of(void* ws, int seqs) {
 
 constexpr int kPlanThreads = 1024;
 
-__device__ __forceinline__ int64_t warp_scan_incl64(int64_t v) {
+// N running sums over the CTA at once: v becomes the inclusive prefix sums, total the sums.  sh: 32 words each, free again behind the
+// call's last barrier
+template <int N>
+__device__ __forceinline__ void block_scan(int64_t (&v)[N], int64_t (&total)[N], int64_t (*sh)[32]) {
+    const int w = threadIdx.x >> 5, lane = lane_id();
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t t = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane_id() >= o) v += t;
+    for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int64_t t = __shfl_up_sync(0xffffffffu, v[k], o);
+            if (lane >= o) v[k] += t;
+        }
+    if (lane == 31)
+#pragma unroll
+        for (int k = 0; k < N; ++k) sh[k][w] = v[k];
+    __syncthreads();
+    // every warp adds up the warps before it itself: one barrier less than a second scan by one of them
+    int64_t t[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) t[k] = sh[k][lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int64_t u = __shfl_up_sync(0xffffffffu, t[k], o);
+            if (lane >= o) t[k] += u;
+        }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const int64_t before = __shfl_sync(0xffffffffu, t[k], (w - 1) & 31);
+        total[k] = __shfl_sync(0xffffffffu, t[k], 31);
+        if (w) v[k] += before;
     }
-    return v;
+    __syncthreads();
 }
-// inclusive prefix sum over the CTA; total = the sum.  sh: 33 words, free again after the call's last barrier
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sh, int64_t& total) {
-    const int w = threadIdx.x >> 5;
-    v = warp_scan_incl64(v);
-    if (lane_id() == 31) sh[w] = v;
-    __syncthreads();
-    if (w == 0) {
-        const int64_t t = warp_scan_incl64(sh[lane_id()]);
-        sh[lane_id()] = t;
+
+struct Wish {  // what a sequence asks for
+    int64_t add, target;
+    int own;
+    bool valid;
+};
+__device__ __forceinline__ Wish wish_of(const int32_t* length, const int32_t* n_new, const whirl_block_tables& t, int s) {
+    Wish w{0, 0, 0, false};
+    if (s < t.seqs) {
+        const int64_t len = length[s], add = n_new[s];
+        const int own = t.owned[s];
+        const int64_t sum = len + add;
+        w.own = min(max(own, 0), t.max_blocks);
+        w.valid = len >= 0 && add >= 0 && sum <= INT32_MAX;
+        if (w.valid) w.target = (uint32_t(sum) + uint32_t(t.block_size) - 1) / uint32_t(t.block_size);
+        w.valid = w.valid && w.target <= t.max_blocks;
+        w.add = w.valid ? add : 0;
     }
-    __syncthreads();
-    const int64_t before = w ? sh[w - 1] : 0;
-    total = sh[kPlanThreads / 32 - 1];
-    __syncthreads();
-    return before + v;
+    return w;
 }
 
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* length, const int32_t* n_new, whirl_block_tables t, whirl_step_rows r,
                                                            void* ws) {
-    __shared__ int64_t sh[33];
+    __shared__ int64_t sh[3][32];
+    asm volatile("griddepcontrol.launch_dependents;");
     const Plan p = plan_of(ws, t.seqs);
     const int tid = threadIdx.x;
     const int count = min(max(*t.free_count, 0), t.num_blocks);
-    int64_t total;
-    // rows asked for -> who fits -> blocks given back
-    int64_t asked = 0, back = 0;
+    // As if everybody were granted: rows, blocks given back and blocks needed in one pass.  Where the sums stay inside max_rows and the
+    // blocks at hand, that is the answer.
+    int64_t rows = 0, back = 0, needs = 0;
     for (int base = 0; base < t.seqs; base += kPlanThreads) {
         const int s = base + tid;
-        const bool in = s < t.seqs;
-        const int64_t len = in ? length[s] : 0, add = in ? n_new[s] : 0;
-        const int64_t target = (len + add + t.block_size - 1) / t.block_size;
-        const bool valid = in && len >= 0 && add >= 0 && len + add <= INT32_MAX && target <= t.max_blocks;
-        const int64_t rows = asked + block_scan(valid ? add : 0, sh, total);
-        asked += total;
-        const bool fits = valid && (add == 0 || rows <= r.max_rows);
-        const int own = in ? min(max(t.owned[s], 0), t.max_blocks) : 0;
-        const int64_t give = fits && own > target ? own - target : 0;
-        const int64_t upto = back + block_scan(give, sh, total);
-        back += total;
-        if (in) {
-            r.status[s] = fits ? WHIRL_SEQ_OK : (valid ? WHIRL_SEQ_REFUSED : WHIRL_SEQ_INVALID);
-            p.owned[s] = own, p.target[s] = fits ? int(target) : own, p.back[s] = int(min(upto - give, int64_t(INT32_MAX)));
+        const Wish w = wish_of(length, n_new, t, s);
+        const int64_t give = w.valid && w.own > w.target ? w.own - w.target : 0, need = w.valid && w.target > w.own ? w.target - w.own : 0;
+        int64_t v[3] = {w.add, give, need}, total[3];
+        block_scan(v, total, sh);
+        if (s < t.seqs) {
+            r.status[s] = w.valid ? WHIRL_SEQ_OK : WHIRL_SEQ_INVALID;
+            p.owned[s] = w.own, p.target[s] = w.valid ? int(w.target) : w.own;
+            p.back[s] = int(min(back + v[1] - give, int64_t(INT32_MAX))), p.taken[s] = int(min(needs + v[2] - need, int64_t(INT32_MAX)));
+            r.row0[s] = int(min(rows + v[0] - w.add, int64_t(INT32_MAX)));
         }
+        rows += total[0], back += total[1], needs += total[2];
     }
-    // blocks needed -> who gets them -> rows  (each thread reads back what it wrote itself)
-    const int64_t have = count + back;
-    int64_t needs = 0, row = 0, used = 0;
-    for (int base = 0; base < t.seqs; base += kPlanThreads) {
-        const int s = base + tid;
-        const bool in = s < t.seqs;
-        const int own = in ? p.owned[s] : 0, target = in ? p.target[s] : 0;
-        const int64_t need = target > own ? target - own : 0;
-        const int64_t upto = needs + block_scan(need, sh, total);
-        needs += total;
-        const bool ok = in && r.status[s] == WHIRL_SEQ_OK && (need == 0 || upto <= have);
-        const int64_t add = ok ? n_new[s] : 0;
-        const int64_t end = row + block_scan(add, sh, total);
-        row += total;
-        block_scan(ok ? need : 0, sh, total);
-        used += total;
-        if (in) {
-            p.taken[s] = int(min(upto - need, int64_t(INT32_MAX)));
-            r.row0[s] = int(end - add);
-            if (ok) t.owned[s] = target;
-            else if (need) p.target[s] = own, r.status[s] = WHIRL_SEQ_REFUSED;
+    int64_t have = count + back, used = needs;
+    if (rows <= r.max_rows && needs <= have) {
+        for (int s = tid; s < t.seqs; s += kPlanThreads) t.owned[s] = p.target[s];  // (each thread reads what it wrote itself)
+    } else {
+        // rows asked for -> who fits -> blocks given back
+        int64_t asked = 0;
+        back = 0;
+        for (int base = 0; base < t.seqs; base += kPlanThreads) {
+            const int s = base + tid;
+            const Wish w = wish_of(length, n_new, t, s);
+            int64_t v[1] = {w.add}, total[1];
+            block_scan(v, total, sh);
+            const bool fits = w.valid && (w.add == 0 || asked + v[0] <= r.max_rows);
+            asked += total[0];
+            const int64_t give = fits && w.own > w.target ? w.own - w.target : 0;
+            v[0] = give;
+            block_scan(v, total, sh);
+            if (s < t.seqs) {
+                if (!fits) p.target[s] = w.own;
+                if (!fits && w.valid) r.status[s] = WHIRL_SEQ_REFUSED;
+                p.back[s] = int(min(back + v[0] - give, int64_t(INT32_MAX)));
+            }
+            back += total[0];
+        }
+        // blocks needed -> who gets them -> rows
+        have = count + back;
+        needs = rows = used = 0;
+        for (int base = 0; base < t.seqs; base += kPlanThreads) {
+            const int s = base + tid;
+            const bool in = s < t.seqs;
+            const int own = in ? p.owned[s] : 0, target = in ? p.target[s] : 0;
+            const int64_t need = target > own ? target - own : 0;
+            int64_t v[1] = {need}, total[1];
+            block_scan(v, total, sh);
+            const bool ok = in && r.status[s] == WHIRL_SEQ_OK && (need == 0 || needs + v[0] <= have);
+            if (in) p.taken[s] = int(min(needs + v[0] - need, int64_t(INT32_MAX)));
+            needs += total[0];
+            const int64_t add = ok ? n_new[s] : 0;
+            int64_t u[2] = {add, ok ? need : 0}, sum[2];
+            block_scan(u, sum, sh);
+            if (in) {
+                r.row0[s] = int(rows + u[0] - add);
+                if (ok) t.owned[s] = target;
+                else if (need) p.target[s] = own, r.status[s] = WHIRL_SEQ_REFUSED;
+            }
+            rows += sum[0], used += sum[1];
         }
     }
     if (tid == 0) {
-        r.row0[t.seqs] = int(row);
+        r.row0[t.seqs] = int(rows);
         *t.free_count = int(min(have - used, int64_t(t.num_blocks)));
-        p.head->count = count, p.head->rows = int(row), p.head->have = have;
+        p.head->count = count, p.head->rows = int(rows), p.head->have = have;
     }
 }
 
@@ -144,6 +197,7 @@ __device__ __forceinline__ int block_taken(const whirl_block_tables& t, const Pl
 constexpr int kFillThreads = 256;
 
 __global__ void __launch_bounds__(kFillThreads) fill_kernel(const int32_t* length, whirl_block_tables t, whirl_step_rows r, void* ws) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // plan_kernel's results (the launch overlaps it)
     const Plan p = plan_of(ws, t.seqs);
     const int count = p.head->count, rows = p.head->rows;
     const int64_t have = p.head->have;
@@ -186,9 +240,15 @@ cudaError_t block_tables_launch(const int32_t* length, const int32_t* n_new, con
     if (e != cudaSuccess) return e;
     const int64_t want = std::max((int64_t(r.max_rows) + kFillThreads - 1) / kFillThreads, (int64_t(t.seqs) * 32 + kFillThreads - 1) / kFillThreads);
     if (want == 0) return cudaSuccess;
-    fill_kernel<<<unsigned(std::min<int64_t>(want, int64_t(sm_count) * 8)), kFillThreads, 0, st>>>(length, t, r, ws);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(std::min<int64_t>(want, int64_t(sm_count) * 8))), cfg.blockDim = dim3(kFillThreads), cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at, cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, fill_kernel, length, t, r, ws);
     count_launch(LAUNCH_BLOCKS);
-    return cudaGetLastError();
+    return e;
 }
 
 }  // namespace wb

@@ -11,6 +11,7 @@
 #include <atomic>
 #include <cfloat>
 #include <cstdlib>
+#include <cstdio>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -140,7 +141,7 @@ __device__ __forceinline__ void add_many(Soft& a, const float (&x)[N], const Sca
 struct ReduceShared {
     float m[32];
     float2 sq[32];
-    float4 part[2][16];  // one per CTA of the cluster; a second set for a second reduction
+    float4 part[2][16];  // one per CTA of the cluster; a second set for a far row's second reduction
 };
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -259,11 +260,47 @@ __device__ __forceinline__ int head_of(const T* p, int n) {
 
 constexpr double kLn2 = 0.6931471805599453;
 
+// The row's scalars are worked out by one thread while the CTA waits, once per row, in a kernel whose loops own the instruction cache: a
+// few short polynomials in 64 bits instead of the library's log, exp and expm1 (measured on the policy loss, 4096 x 151936 bf16: SCALARS).
+
+// log of a positive finite number: s = 2^k f with f in [sqrt 1/2, sqrt 2), log f = 2 atanh z, z = (f - 1) / (f + 1), |z| < 0.172; the
+// terms left out are below 1e-13.  NaN for what has no logarithm.
+__device__ __forceinline__ double ln_of(double s) {
+    if (!(s > 0.0 && s <= 1.7e308)) return NAN;
+    const int hi = __double2hiint(s), k = (hi - 0x3fe6a09e) >> 20;
+    const double f = __hiloint2double(hi - (k << 20), __double2loint(s)), b = f + 1.0;
+    double r = double(__frcp_rn(float(b)));
+    r = r * (2.0 - b * r);
+    const double z = (f - 1.0) * r, y = z * z;
+    double t = 1.0 / 13.0;
+    t = fma(t, y, 1.0 / 11.0), t = fma(t, y, 1.0 / 9.0), t = fma(t, y, 1.0 / 7.0), t = fma(t, y, 1.0 / 5.0), t = fma(t, y, 1.0 / 3.0);
+    return fma(double(k), kLn2, 2.0 * z * fma(t, y, 1.0));
+}
+// exp of |d| <= 25: d = n ln 2 + f, Taylor's sum to f^11 (what is left out is below 1e-14).  NaN stays.
+__device__ __forceinline__ double exp_of(double d) {
+    const double n = rint(d * 1.4426950408889634);
+    constexpr double hi = double(0.6931471805599453f), lo = kLn2 - hi;  // (n * hi is exact)
+    const double f = fma(n, -lo, fma(n, -hi, d));
+    double t = 1.0 / 39916800.0;
+    t = fma(t, f, 1.0 / 3628800.0), t = fma(t, f, 1.0 / 362880.0), t = fma(t, f, 1.0 / 40320.0), t = fma(t, f, 1.0 / 5040.0);
+    t = fma(t, f, 1.0 / 720.0), t = fma(t, f, 1.0 / 120.0), t = fma(t, f, 1.0 / 24.0), t = fma(t, f, 1.0 / 6.0);
+    t = fma(t, f, 0.5), t = fma(t, f, 1.0), t = fma(t, f, 1.0);
+    return d == d ? __hiloint2double(__double2hiint(t) + (int(n) << 20), __double2loint(t)) : d;
+}
+// exp k - k - 1 for |k| <= 25, without the cancellation around 0
+__device__ __forceinline__ double kl_of(double k) {
+    if (fabs(k) > 0.35) return exp_of(k) - 1.0 - k;
+    double t = 1.0 / 39916800.0;
+    t = fma(t, k, 1.0 / 3628800.0), t = fma(t, k, 1.0 / 362880.0), t = fma(t, k, 1.0 / 40320.0), t = fma(t, k, 1.0 / 5040.0);
+    t = fma(t, k, 1.0 / 720.0), t = fma(t, k, 1.0 / 120.0), t = fma(t, k, 1.0 / 24.0), t = fma(t, k, 1.0 / 6.0);
+    return k * k * fma(t, k, 0.5);
+}
+
 // 2^(e - m c): what the rounded reference e of a row with maximum m puts into its sum.  Doubles: m c has to be exact to the last bits
 // of e.
 __device__ __forceinline__ double shift_of(double m, double e, double c) {
     const double y = kLn2 * (e - m * c);
-    return fabs(y) < 1e-3 ? 1.0 + y * (1.0 + y * (0.5 + y * (1.0 / 6.0))) : exp(y);
+    return fabs(y) < 1e-3 ? 1.0 + y * (1.0 + y * (0.5 + y * (1.0 / 6.0))) : exp_of(y < 25.0 ? y : 25.0);  // (|m c| <= 1e37: e is within 1e30 of it)
 }
 
 // The row's gradient: dx_j = w_j * (a + b * t_j), + d on the token, with t_j = x_j c - e (far: (x_j - e) c) and w_j = 2^t_j, whose sum
@@ -283,7 +320,7 @@ __device__ __forceinline__ GradRow grad_row(float m, double sum, float inv_t, in
     q.far = !(m >= -most && m <= most);
     q.e = q.far ? m : m * q.c;
     const double s = q.far ? sum : sum / shift_of(m, q.e, q.c), k = double(inv_t) / s;
-    q.a = float(-k * (g + (h == 0.0 ? 0.0 : h * (entropy - log(s)))));
+    q.a = float(-k * (g + (h == 0.0 ? 0.0 : h * (entropy - ln_of(s)))));
     q.b = float(-k * h * kLn2);
     q.d = float(double(inv_t) * g);
     return q;
@@ -320,19 +357,38 @@ __device__ __forceinline__ uint4 grad_vec(const GradRow& q, uint4 v) {
 constexpr int kRowThreads = 256;
 constexpr int kSliceMost = 200 * 1024;  // bytes of a row's slice that a CTA can hold
 
-// the row as a user's call describes it, and whether it counts
+// A row as a user's call describes it, and whether it counts.
 struct RowOf {
     int token;
-    float inv_t;
+    float inv_t, weight;
+    float adv, old_logp, ref_logp;  // (policy loss; the preference loss has ref_logp)
+    float scale;                    // row_scale, where it was known when the row was read
     bool live;
 };
-__device__ __forceinline__ RowOf row_of(const LossArgs& a, int row) {
+// Read by a warp, one word per lane, so that a row costs one trip to memory; every lane gets the whole.
+template <int EPI>
+__device__ __forceinline__ RowOf row_of(const LossArgs& a, int row, bool with_scale) {
+    const int lane = lane_id();
+    const void* p = nullptr;
+    if (lane == 0) p = a.token + row;
+    else if (lane == 1 && a.inv_t_rows) p = a.inv_t_rows + row;
+    else if (lane == 2 && a.weight) p = a.weight + row;
+    else if (lane == 3 && EPI == EPI_POLICY) p = a.adv + row;
+    else if (lane == 4 && EPI == EPI_POLICY && a.old_logp) p = a.old_logp + row;
+    else if (lane == 5 && EPI != EPI_NONE && a.ref_logp) p = a.ref_logp + row;
+    else if (lane == 6 && EPI == EPI_POLICY && with_scale) p = a.row_scale + row;
+    else if (lane == 7 && a.seq_start) p = a.seq_start;
+    else if (lane == 8 && a.seq_start) p = a.seq_start + a.seqs;
+    const uint32_t got = p ? *static_cast<const uint32_t*>(p) : 0u;
+    auto word = [&](int l) { return __shfl_sync(0xffffffffu, got, l); };
+    auto real = [&](int l) { return __uint_as_float(word(l)); };
     RowOf r;
-    r.token = a.token[row];
-    r.inv_t = a.inv_t_rows ? a.inv_t_rows[row] : a.inv_t;
-    r.live = unsigned(r.token) < unsigned(a.n);
-    if (a.weight) r.live = r.live && a.weight[row] > 0.f;
-    if (a.seq_start) r.live = r.live && row >= a.seq_start[0] && row < a.seq_start[a.seqs];
+    r.token = int(word(0));
+    const float it = real(1), wt = real(2);
+    r.inv_t = a.inv_t_rows ? it : a.inv_t, r.weight = a.weight ? wt : 1.f;
+    r.adv = real(3), r.old_logp = real(4), r.ref_logp = real(5), r.scale = real(6);
+    const int first = int(word(7)), end = int(word(8));
+    r.live = unsigned(r.token) < unsigned(a.n) && r.weight > 0.f && (!a.seq_start || (row >= first && row < end));
     return r;
 }
 
@@ -340,16 +396,16 @@ __device__ __forceinline__ RowOf row_of(const LossArgs& a, int row) {
 struct PolicyRow {
     double loss, kl, dlogp;
 };
-__device__ PolicyRow policy_row(const LossArgs& a, int row, double logp, double entropy) {
+__device__ PolicyRow policy_row(const LossArgs& a, const RowOf& w, double logp, double entropy) {
     PolicyRow p;
-    const double adv = a.adv[row];
+    const double adv = w.adv;
     double ratio = 1.0, pg, dpg;
     bool free_d = true;
     if (a.old_logp) {
-        double d = logp - double(a.old_logp[row]);
+        double d = logp - double(w.old_logp);
         free_d = !(d <= -20.0 || d >= 20.0);
         d = d < -20.0 ? -20.0 : (d > 20.0 ? 20.0 : d);
-        ratio = exp(d);
+        ratio = exp_of(d);
     }
     const double lo = 1.0 - double(a.clip_low), hi = 1.0 + double(a.clip_high);
     const double plain = ratio * adv, clipped = (ratio < lo ? lo : (ratio > hi ? hi : ratio)) * adv;
@@ -359,13 +415,12 @@ __device__ PolicyRow policy_row(const LossArgs& a, int row, double logp, double 
     if (a.dual_clip > 0.f && adv < 0.0 && pg > -double(a.dual_clip) * adv) pg = -double(a.dual_clip) * adv, dpg = 0.0;
     p.kl = 0.0;
     if (a.ref_logp) {
-        double k = double(a.ref_logp[row]) - logp;
+        double k = double(w.ref_logp) - logp;
         const bool free_k = !(k <= -20.0 || k >= 20.0);
         k = k < -20.0 ? -20.0 : (k > 20.0 ? 20.0 : k);
-        const double e = expm1(k);
-        p.kl = e - k;
+        p.kl = kl_of(k);
         pg += double(a.kl_coef) * p.kl;
-        if (free_k) dpg -= double(a.kl_coef) * e;
+        if (free_k) dpg -= double(a.kl_coef) * (p.kl + k);
     }
     p.loss = pg - (a.ent_coef != 0.f ? double(a.ent_coef) * entropy : 0.0);
     p.dlogp = dpg;
@@ -378,16 +433,16 @@ struct RowDone {
     double sum, entropy, g, h;
 };
 template <int EPI, bool ENT>
-__device__ __noinline__ RowDone finish_row(const LossArgs& a, int row, bool write, bool live, int token, float inv_t, float x_token, float m, float e,
-                                           float s, float q, bool far) {
+__device__ __forceinline__ RowDone finish_row(const LossArgs& a, int row, bool write, const RowOf& w, float x_token, float m, float e, float s, float q,
+                                           bool far) {
     RowDone done{};
     double logp = 0.0, entropy = 0.0, sum = 0.0;
-    if (live) {
-        const double c = double(inv_t) * 1.4426950408889634;
+    if (w.live) {
+        const double c = double(w.inv_t) * 1.4426950408889634;
         // a row without a finite maximum has no distribution
         sum = (m >= -FLT_MAX && m <= FLT_MAX) ? (far ? double(s) : double(s) * shift_of(m, e, c)) : double(NAN);
-        const double ls = log(sum);
-        logp = (double(x_token) - double(m)) * double(inv_t) - ls;
+        const double ls = ln_of(sum);
+        logp = (double(x_token) - double(m)) * double(w.inv_t) - ls;
         // the terms' mean exponent is q / s from the reference, and e - m c more from the maximum
         if (ENT) entropy = ls - kLn2 * (double(q) / double(s) + (far ? 0.0 : double(e) - double(m) * c));
     } else {
@@ -401,19 +456,18 @@ __device__ __noinline__ RowDone finish_row(const LossArgs& a, int row, bool writ
     if (EPI == EPI_POLICY) {
         PolicyRow p{};
         float scale = 0.f;
-        if (live) scale = a.row_scale[row], p = policy_row(a, row, logp, entropy);
-        done.g = float(double(scale) * p.dlogp), done.h = live ? -a.ent_coef * scale : 0.f;
+        if (w.live) scale = w.scale, p = policy_row(a, w, logp, entropy);
+        done.g = float(double(scale) * p.dlogp), done.h = w.live ? -a.ent_coef * scale : 0.f;
         if (write) {
             if (a.kl) a.kl[row] = float(p.kl);
             if (a.row_loss) a.row_loss[row] = float(p.loss);
             if (a.g_logp) a.g_logp[row] = float(done.g);
             if (a.g_entropy) a.g_entropy[row] = float(done.h);
-            a.row_term[row] = live ? double(scale) * p.loss : 0.0;
+            a.row_term[row] = w.live ? double(scale) * p.loss : 0.0;
         }
     } else if (EPI == EPI_PREF) {
-        const float w = !live ? 0.f : (a.weight ? a.weight[row] : 1.f);
-        a.row_term[row] = live ? double(w) * (logp - (a.ref_logp ? double(a.ref_logp[row]) : 0.0)) : 0.0;
-        a.row_scale[row] = w;
+        a.row_term[row] = w.live ? double(w.weight) * (logp - (a.ref_logp ? double(w.ref_logp) : 0.0)) : 0.0;
+        a.row_scale[row] = w.live ? w.weight : 0.f;
         a.g_logp[row] = 0.f;  // (the rows of a pair get theirs from pairs_kernel)
     }
     return done;
@@ -432,14 +486,14 @@ __device__ double block_sum(double v, double* sh) {  // the same value in every 
 // was launched the ordinary way).
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// The CTA that finishes the last row adds up the rows' terms, in their order.  (Called by one CTA per row, after its thread 0 has
-// written the row's term.)
-__device__ void last_sum(const LossArgs& a) {
+// The CTA that comes last adds up the rows' terms, in their order.  (Called by `callers` CTAs in all, each after its thread 0 has written
+// the terms of its rows.)
+__device__ void last_sum(const LossArgs& a, unsigned callers) {
     __shared__ bool last;
     __shared__ double sh_d[32];
     if (threadIdx.x == 0) {
         __threadfence();
-        last = atomicAdd(a.ticket, 1u) + 1u == unsigned(a.rows);
+        last = atomicAdd(a.ticket, 1u) + 1u == callers;
     }
     __syncthreads();
     if (!last) return;
@@ -505,135 +559,328 @@ __device__ __noinline__ Soft far_sums(const uint4* v, int cnt, bool have_edge, f
 template <typename T>
 constexpr int kFwdRing = sizeof(T) == 4 ? 4 : 8;
 
-// One cluster per row, each CTA a contiguous slice of `per` 16-byte vectors; the scalars before the first and behind the last
-// boundary belong to rank 0, one per thread.  A thread reads only what it copied into shared memory itself, so that the copies
-// need no barrier.
-template <typename T, int EPI, bool ENT, bool GRAD>
-__global__ void __launch_bounds__(kRowThreads, GRAD ? 5 : 3) rows_kernel(const __grid_constant__ LossArgs a, int per) {
-    constexpr int E = 16 / sizeof(T), NT = kRowThreads, V = 16 / E;
-    extern __shared__ __align__(16) uint4 slice[];  // GRAD: this CTA's part of the row; else a ring of what is under way
+// Where a CTA's slice of a row lies: `per` 16-byte vectors of the row's body; the scalars before the first and behind the last boundary
+// belong to rank 0, one per thread.
+template <typename T>
+struct Slice {
+    const T* x;       // the row
+    int head, nv, v0, cnt;
+    int edge;         // this thread's scalar, -1 without one
+    __device__ __forceinline__ Slice(const LossArgs& a, int row, int rank, int per) {
+        constexpr int E = 16 / sizeof(T);
+        x = static_cast<const T*>(a.x) + int64_t(row) * a.ld;
+        head = head_of(x, a.n), nv = (a.n - head) / E;
+        v0 = min(rank * per, nv), cnt = min(per, nv - v0);
+        const int i = int(threadIdx.x);
+        edge = rank == 0 && i < a.n - nv * E ? (i < head ? i : i + nv * E) : -1;  // (fewer than 2 E scalars, one per thread)
+    }
+    __device__ __forceinline__ const uint4* body() const { return reinterpret_cast<const uint4*>(x + head) + v0; }
+};
+
+// The cluster's statistics of a row from its threads' sums; valid in warp 0 of every CTA.  data: the CTA's vectors, read again for a
+// far row.
+template <typename T, bool ENT>
+__device__ __forceinline__ Soft row_sum(Soft s, const Scale& c, ReduceShared& sh, int ctas, const uint4* data, int cnt, bool have_edge, float x_edge,
+                                        bool& far) {
+    s = reduce<ENT>(s, c, sh, ctas, 0);
+    far = threadIdx.x < 32 && is_far(s);
+    if (__syncthreads_or(far)) {  // (every CTA of the cluster has the same statistics)
+        if (threadIdx.x == 0) sh.m[0] = s.m;
+        __syncthreads();
+        const float m = sh.m[0];
+        __syncthreads();
+        s = reduce_far<ENT>(far_sums<T, ENT>(data, cnt, have_edge, x_edge, m, c.hi), m, sh, ctas);
+        far = true;
+    }
+    return s;
+}
+
+// Statistics: one cluster per row.  A thread reads what it copied into shared memory itself, so that the copies need no barrier.
+template <typename T, int EPI, bool ENT>
+__global__ void __launch_bounds__(kRowThreads, 3) forward_kernel(const __grid_constant__ LossArgs a, int per) {
+    constexpr int E = 16 / sizeof(T), NT = kRowThreads, V = 16 / E, D = kFwdRing<T>;
+    extern __shared__ __align__(16) uint4 ring[];
     __shared__ ReduceShared sh;
-    __shared__ GradRow s_q;
-    __shared__ bool s_zero;
-    __shared__ float s_m;
     const int ctas = int(cluster_size()), rank = int(cluster_rank()), tid = threadIdx.x;
     const int row = int(blockIdx.x / unsigned(ctas));
-    const RowOf w = row_of(a, row);
-    const T* x = static_cast<const T*>(a.x) + int64_t(row) * a.ld;
-    const int head = head_of(x, a.n), nv = (a.n - head) / E, edge = a.n - nv * E;
-    const int v0 = min(rank * per, nv), cnt = min(per, nv - v0);
-    const uint4* v = reinterpret_cast<const uint4*>(x + head) + v0;
-    const int my_edge = rank == 0 && tid < edge ? (tid < head ? tid : tid + nv * E) : -1;  // (edge < 2 E <= NT)
-    float x_edge = 0.f;
-    bool zero = true, far = false;
+    RowOf w = row_of<EPI>(a, row, false);
     if (w.live) {
+        const Slice<T> at(a, row, rank, per);
+        const uint4* v = at.body();
+        const int cnt = at.cnt;
         const Scale c = scale_of(w.inv_t);
         Soft s = soft_empty(c);
-        float x_token = 0.f;
-        if (GRAD) {
-#pragma unroll 4
-            for (int i = tid; i < cnt; i += NT) copy_async16(slice + i, v + i);
-            copies_commit();
-        } else {
 #pragma unroll 1
-            for (int k = 0; k < kFwdRing<T> - 1; ++k) {
+        for (int k = 0; k < D - 1; ++k) {
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const int i = (k * V + j) * NT + tid;
-                    if (i < cnt) copy_async16(slice + i, v + i);
-                }
-                copies_commit();
+            for (int j = 0; j < V; ++j) {
+                const int i = (k * V + j) * NT + tid;
+                if (i < cnt) copy_async16(ring + i, v + i);
             }
+            copies_commit();
         }
-        if (tid == 0) x_token = load_one(x + w.token);
-        if (my_edge >= 0) {
-            x_edge = load_one(x + my_edge);
+        const float x_token = tid == 0 ? load_one(at.x + w.token) : 0.f;
+        float x_edge = 0.f;
+        if (at.edge >= 0) {
+            x_edge = load_one(at.x + at.edge);
             const float e[1] = {x_edge};
             add_many<ENT, 1>(s, e, c);
         }
-        if (GRAD) {
+        int slot = 0;  // of the step at hand; the one before it is where the next copies go
+#pragma unroll 1
+        for (int i = tid; i < cnt; i += V * NT) {
+            const int to = slot == 0 ? D - 1 : slot - 1;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const int k = i + ((D - 1) * V + j) * NT;
+                if (k < cnt) copy_async16(ring + (to * V + j) * NT + tid, v + k);
+            }
+            copies_commit();
+            copies_but<D - 1>();
+            const uint4* b = ring + slot * V * NT + tid;
+            if (i + (V - 1) * NT < cnt) {
+                add_block<T, ENT>(s, b, NT, c);
+            } else {
+                for (int j = 0; i + j * NT < cnt; ++j) add_vec<T, ENT>(s, b[j * NT], c);
+            }
+            slot = slot + 1 == D ? 0 : slot + 1;
+        }
+        copies_but<0>();
+        bool far;
+        s = row_sum<T, ENT>(s, c, sh, ctas, v, cnt, at.edge >= 0, x_edge, far);
+        if (tid == 0 && rank == 0) {
+            grid_dependency_wait();  // row_scale_kernel's results
+            if (EPI == EPI_POLICY) w.scale = a.row_scale[row];
+            finish_row<EPI, ENT>(a, row, true, w, x_token, s.m, s.e, s.s, s.q, far);
+        }
+    } else if (tid == 0 && rank == 0) {
+        grid_dependency_wait();
+        finish_row<EPI, ENT>(a, row, true, w, 0.f, 0.f, 0.f, 0.f, 0.f, false);
+    }
+    if (EPI == EPI_POLICY && rank == 0) last_sum(a, unsigned(a.rows));
+}
+
+// A warp's partial statistics, on their way to every CTA of the cluster
+template <bool ENT>
+struct Part;
+template <>
+struct Part<false> {
+    float m, s;
+};
+template <>
+struct Part<true> {
+    float m, s, q, pad;
+};
+// stores to shared memory of CTA `cta` and counts the bytes on its barrier
+__device__ __forceinline__ void send(Part<false>* to, uint64_t* bar, int cta, float m, float s, float) {
+    asm volatile(
+        "{\n .reg .b32 d, b;\n mapa.shared::cluster.u32 d, %0, %2;\n mapa.shared::cluster.u32 b, %1, %2;\n"
+        " st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [d], {%3, %4}, [b];\n}\n" ::"r"(smem_u32(to)),
+        "r"(smem_u32(bar)), "r"(cta), "r"(__float_as_uint(m)), "r"(__float_as_uint(s))
+        : "memory");
+}
+__device__ __forceinline__ void send(Part<true>* to, uint64_t* bar, int cta, float m, float s, float q) {
+    asm volatile(
+        "{\n .reg .b32 d, b;\n mapa.shared::cluster.u32 d, %0, %2;\n mapa.shared::cluster.u32 b, %1, %2;\n"
+        " st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [d], {%3, %4, %5, %5}, [b];\n}\n" ::"r"(smem_u32(to)),
+        "r"(smem_u32(bar)), "r"(cta), "r"(__float_as_uint(m)), "r"(__float_as_uint(s)), "r"(__float_as_uint(q))
+        : "memory");
+}
+__device__ __forceinline__ void cluster_barrier() { asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+constexpr int kRowWarps = kRowThreads / 32;
+
+// Each warp's sums to every CTA of the cluster (its lane i tells CTA i).
+template <bool ENT>
+__device__ __forceinline__ void tell(Soft a, const Scale& c, Part<ENT>* parts, uint64_t* bar, int ctas, int rank) {
+    a.s -= a.k, a.k = 0.f;
+    const float m = warp_max_f(a.m);
+    raise<ENT>(a, m, c);
+    a.s = warp_sum_f(a.s);
+    if (ENT) a.q = warp_sum_f(a.q);
+    if (lane_id() < ctas) send(parts + rank * kRowWarps + (threadIdx.x >> 5), bar, lane_id(), m, a.s, a.q);
+}
+// The row's statistics from all warps' (one warp).  A barrier that does not complete in its time gives a row of NaN.
+template <bool ENT>
+__device__ __forceinline__ Soft hear(const Scale& c, const Part<ENT>* parts, uint64_t* bar, uint32_t parity, int ctas, uint32_t& limit) {
+    const int n = ctas * kRowWarps;
+    if (lane_id() == 0) mbar_expect_tx(bar, uint32_t(n * sizeof(Part<ENT>)));
+    const bool came = __all_sync(0xffffffffu, mbar_wait(bar, parity, limit));
+    if (!came) limit = 1;  // (and the rows after it do not wait that long again)
+    float m = -INFINITY;
+    for (int i = lane_id(); i < n; i += 32) m = fmaxf(m, parts[i].m);
+    m = warp_max_f(m);
+    Soft s{m, ref_of(m, c), 0.f, 0.f, 0.f};
+    for (int i = lane_id(); i < n; i += 32) {
+        Soft p{parts[i].m, ref_of(parts[i].m, c), parts[i].s, 0.f, 0.f};
+        if constexpr (ENT) p.q = parts[i].q;
+        raise<ENT>(p, m, c);
+        s.s += p.s;
+        if (ENT) s.q += p.q;
+    }
+    s.s = warp_sum_f(s.s);
+    if (ENT) s.q = warp_sum_f(s.q);
+    if (!came) s.s = NAN;
+    return s;
+}
+
+// The policy loss with its gradient.  The clusters stay and take rows in turn, each CTA holding its slice of a row in shared memory
+// from the read to the gradient: one read and one write of global memory.  As soon as a thread has written a vector's
+// gradient it starts the copy of the same vector of the cluster's next row into the same place, so that the memory is
+// busy while the statistics of that row wait for it; several CTAs per SM fill each other's waits (the exchange of the statistics, the row's
+// scalars).  The statistics travel by stores that count on the receiver's mbarrier: a cluster barrier would hold every row until the
+// gradient's stores of the row before it are acknowledged.
+template <typename T, int EPI, bool ENT>
+__global__ void __launch_bounds__(kRowThreads, 5) fused_kernel(const __grid_constant__ LossArgs a, int per) {
+    constexpr int E = 16 / sizeof(T), NT = kRowThreads, V = 16 / E;
+    extern __shared__ __align__(16) uint4 slice[];  // `per` vectors, then three sets of partial statistics (rows in turn; far rows)
+    __shared__ GradRow s_q;
+    __shared__ RowOf s_row[2];
+    __shared__ uint64_t s_bar[3];
+    __shared__ float s_m;
+    __shared__ bool s_zero, s_far;
+    const int ctas = int(cluster_size()), rank = int(cluster_rank()), tid = threadIdx.x;
+    const int clusters = int(gridDim.x / unsigned(ctas));
+    Part<ENT>* const parts = reinterpret_cast<Part<ENT>*>(slice + per);
+    int row = int(blockIdx.x / unsigned(ctas)), lives = 0, fars = 0;
+    uint32_t limit = kWaitLimit;
+    if (tid < 32) {
+        const RowOf w = row_of<EPI>(a, row, false);
+        if (tid == 0) {
+            s_row[0] = w;
+            for (int i = 0; i < 3; ++i) mbar_init(&s_bar[i], 1);
+            mbar_fence_init();
+        }
+    }
+    __syncthreads();
+    if (s_row[0].live) {
+        const Slice<T> at(a, row, rank, per);
+        const uint4* v = at.body();
+#pragma unroll 4
+        for (int i = tid; i < at.cnt; i += NT) copy_async16(slice + i, v + i);
+        copies_commit();
+    }
+    cluster_barrier();  // every CTA's barriers are ready
+#pragma unroll 1
+    for (int k = 0; row < a.rows; ++k, row += clusters) {
+        const RowOf& w = s_row[k & 1];
+        const bool more = a.rows - row > clusters;
+        if (more && tid >= NT - 32) {  // the next row's scalars; the wait is over at once but for the first row
+            grid_dependency_wait();
+            const RowOf r = row_of<EPI>(a, row + clusters, true);
+            if (tid == NT - 32) s_row[(k + 1) & 1] = r;
+        }
+        const Slice<T> at(a, row, rank, per);
+        const int cnt = at.cnt;
+        float x_edge = 0.f;
+        bool zero = true;
+        if (w.live) {
+            const Scale c = scale_of(w.inv_t);
+            Soft s = soft_empty(c);
+            const float x_token = tid == 0 ? load_one(at.x + w.token) : 0.f;
+            if (at.edge >= 0) {
+                x_edge = load_one(at.x + at.edge);
+                const float e[1] = {x_edge};
+                add_many<ENT, 1>(s, e, c);
+            }
             copies_but<0>();
             int i = tid;
 #pragma unroll 1
             for (; i + (V - 1) * NT < cnt; i += V * NT) add_block<T, ENT>(s, slice + i, NT, c);
 #pragma unroll 1
             for (; i < cnt; i += NT) add_vec<T, ENT>(s, slice[i], c);
-        } else {
-            constexpr int D = kFwdRing<T>;
-            int slot = 0;  // of the step at hand; the one before it is where the next copies go
-#pragma unroll 1
-            for (int i = tid; i < cnt; i += V * NT) {
-                const int to = slot == 0 ? D - 1 : slot - 1;
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const int k = i + ((D - 1) * V + j) * NT;
-                    if (k < cnt) copy_async16(slice + (to * V + j) * NT + tid, v + k);
+            const int set = lives & 1;
+            tell<ENT>(s, c, parts + set * ctas * kRowWarps, &s_bar[set], ctas, rank);
+            auto finish = [&](const Soft& r, bool far) {  // one thread
+                RowOf wr = w;
+                if (k == 0) {
+                    grid_dependency_wait();  // row_scale_kernel's results
+                    if (EPI == EPI_POLICY) wr.scale = a.row_scale[row];
                 }
-                copies_commit();
-                copies_but<D - 1>();
-                const uint4* b = slice + slot * V * NT + tid;
-                if (i + (V - 1) * NT < cnt) {
-                    add_block<T, ENT>(s, b, NT, c);
-                } else {
-                    for (int j = 0; i + j * NT < cnt; ++j) add_vec<T, ENT>(s, b[j * NT], c);
-                }
-                slot = slot + 1 == D ? 0 : slot + 1;
-            }
-            copies_but<0>();
-        }
-        s = reduce<ENT>(s, c, sh, ctas, 0);
-        if (tid < 32) far = is_far(s);
-        if (__syncthreads_or(tid == 0 && far)) {  // (every CTA of the cluster has the same statistics)
-            if (tid == 0) s_m = s.m;
-            __syncthreads();
-            const float m = s_m;
-            s = far_sums<T, ENT>(GRAD ? slice : v, cnt, my_edge >= 0, x_edge, m, c.hi);
-            s = reduce_far<ENT>(s, m, sh, ctas);
-            far = true;
-        }
-        if (tid == 0) {
-            grid_dependency_wait();  // row_scale_kernel's results; row_scale and the ticket are read below
-            const RowDone d = finish_row<EPI, ENT>(a, row, rank == 0, true, w.token, w.inv_t, x_token, s.m, s.e, s.s, s.q, far);
-            if (GRAD) {
+                const RowDone d = finish_row<EPI, ENT>(a, row, rank == 0, wr, x_token, r.m, r.e, r.s, r.q, far);
                 s_zero = d.g == 0.0 && d.h == 0.0;
-                s_q = grad_row(s.m, d.sum, w.inv_t, w.token, d.g, d.h, d.entropy);
+                s_q = grad_row(r.m, d.sum, wr.inv_t, wr.token, d.g, d.h, d.entropy);
+            };
+            if (tid < 32) {
+                s = hear<ENT>(c, parts + set * ctas * kRowWarps, &s_bar[set], uint32_t(lives >> 1) & 1, ctas, limit);
+                if (tid == 0) {
+                    s_far = is_far(s), s_m = s.m;
+                    if (!is_far(s)) finish(s, false);
+                }
             }
-        }
-        if (GRAD) {
+            ++lives;
             __syncthreads();
+            if (s_far) {  // (every CTA of the cluster has the same statistics)
+                const float m = s_m;
+                const Scale one{1.f, 0.f, FLT_MAX};
+                s = far_sums<T, ENT>(slice, cnt, at.edge >= 0, x_edge, m, c.hi);
+                s.m = 0.f, s.e = 0.f;  // (references alike: nothing is scaled on the way)
+                tell<ENT>(s, one, parts + 2 * ctas * kRowWarps, &s_bar[2], ctas, rank);
+                if (tid < 32) {
+                    s = hear<ENT>(one, parts + 2 * ctas * kRowWarps, &s_bar[2], uint32_t(fars) & 1, ctas, limit);
+                    s.m = m;
+                    if (tid == 0) finish(s, true);
+                }
+                ++fars;
+                __syncthreads();
+            }
             zero = s_zero;
+        } else {
+            if (tid == 0) {
+                if (k == 0) grid_dependency_wait();
+                if (rank == 0) finish_row<EPI, ENT>(a, row, true, w, 0.f, 0.f, 0.f, 0.f, 0.f, false);
+            }
+            __syncthreads();
         }
-    } else if (tid == 0) {
-        grid_dependency_wait();
-        if (rank == 0) finish_row<EPI, ENT>(a, row, true, false, w.token, w.inv_t, 0.f, 0.f, 0.f, 0.f, 0.f, false);
-    }
-    if (GRAD) {
+        // (s_row of the next row, s_q and s_zero are in place; their next writes come after every thread has read them: s_row's behind the
+        // next row's barrier but one, the others' behind all warps' `tell` of the next row)
         GradRow q{};
         if (!zero) q = s_q;
         T* dx = static_cast<T*>(a.dx) + int64_t(row) * a.ld_dx;
-        if (my_edge >= 0) store_one(dx + my_edge, zero ? 0.f : grad_of<ENT>(q, x_edge) + (my_edge == q.token ? q.d : 0.f));
-        const bool vec = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
-        T* body = dx + head + int64_t(v0) * E;
+        if (at.edge >= 0) store_one(dx + at.edge, zero ? 0.f : grad_of<ENT>(q, x_edge) + (at.edge == q.token ? q.d : 0.f));
+        const bool vec = ((reinterpret_cast<uintptr_t>(at.x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
+        T* body = dx + at.head + int64_t(at.v0) * E;
         uint4* out = reinterpret_cast<uint4*>(body);
+        // the token's own element is written again by the thread that wrote its vector
+        const int t = zero ? -1 : q.token - at.head - at.v0 * E;
+        const bool mine = t >= 0 && t < cnt * E && (t / E) % NT == tid;
+        const float x_mine = mine ? load_one(reinterpret_cast<const T*>(slice) + t) : 0.f;
+        const uint4* next = nullptr;
+        int refill = 0;
+        if (more && s_row[(k + 1) & 1].live) {
+            const Slice<T> n(a, row + clusters, rank, per);
+            next = n.body(), refill = n.cnt;
+        }
+        int i = tid;
         if (zero && vec) {
 #pragma unroll 4
-            for (int i = tid; i < cnt; i += NT) __stcs(out + i, make_uint4(0, 0, 0, 0));
+            for (; i < cnt; i += NT) __stcs(out + i, make_uint4(0, 0, 0, 0));
+            i = tid;  // (nothing refilled yet)
         } else if (vec && !q.far) {
+            const int both = min(cnt, refill);
 #pragma unroll 2
-            for (int i = tid; i < cnt; i += NT) __stcs(out + i, grad_vec<T, ENT>(q, slice[i]));
-        } else {
-            for (int i = tid; i < cnt; i += NT) {
-                float e[E];
-                unpack<T>(zero ? make_uint4(0, 0, 0, 0) : slice[i], e);
-#pragma unroll 1
-                for (int k = 0; k < E; ++k) store_one(body + int64_t(i) * E + k, zero ? 0.f : grad_of<ENT>(q, load_one(reinterpret_cast<const T*>(slice + i) + k)));
+            for (; i < both; i += NT) {
+                const uint4 g = grad_vec<T, ENT>(q, slice[i]);
+                __stcs(out + i, g);
+                copy_async16(slice + i, next + i);
             }
+            for (int j = i; j < cnt; j += NT) __stcs(out + j, grad_vec<T, ENT>(q, slice[j]));
+        } else {
+            for (; i < cnt; i += NT) {
+#pragma unroll 1
+                for (int j = 0; j < E; ++j)
+                    store_one(body + int64_t(i) * E + j, zero ? 0.f : grad_of<ENT>(q, load_one(reinterpret_cast<const T*>(slice + i) + j)));
+            }
+            i = tid;
         }
-        // the token's own element, by the thread that wrote it
-        const int at = zero ? -1 : q.token - head - v0 * E;
-        if (at >= 0 && at < cnt * E && (at / E) % NT == tid) store_one(body + at, grad_of<ENT>(q, load_one(reinterpret_cast<const T*>(slice) + at)) + q.d);
+        if (mine) store_one(body + t, grad_of<ENT>(q, x_mine) + q.d);
+#pragma unroll 4
+        for (; i < refill; i += NT) copy_async16(slice + i, next + i);
+        copies_commit();
     }
-    if (EPI == EPI_POLICY && rank == 0) last_sum(a);
+    copies_but<0>();
+    cluster_barrier();  // nobody leaves while another CTA's stores are under way to it
+    if (EPI == EPI_POLICY && rank == 0) last_sum(a, unsigned(clusters));
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -805,49 +1052,64 @@ __global__ void __launch_bounds__(kPairThreads) pairs_kernel(LossArgs a, PairArg
     }
 }
 
-// A launch of rows_kernel: `ctas` CTAs per row in a cluster, `per` vectors each.
-template <typename T, int EPI, bool ENT, bool GRAD>
-cudaError_t rows_launch(const LossArgs& a, int ctas, int per, cudaStream_t st) {
-    constexpr int kMost = kSliceMost;
-    static std::atomic<uint64_t> ready{0};  // bit per device: the function's limits are raised
+// A launch of forward_kernel / fused_kernel: `ctas` CTAs in a cluster, `per` vectors of a row each, at most `clusters` clusters.
+template <typename F>
+cudaError_t cluster_launch(F f, std::atomic<uint64_t>& ready, const LossArgs& a, int ctas, int per, size_t smem, bool persistent, bool follows, cudaStream_t st) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    auto* const f = rows_kernel<T, EPI, ENT, GRAD>;
-    if (dev > 63 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {
-        e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+    if (dev > 63 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {  // bit per device: the function's limits are raised
+        e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kSliceMost);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
         if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_release);
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(a.rows) * unsigned(ctas)), cfg.blockDim = dim3(kRowThreads), cfg.stream = st;
-    cfg.dynamicSmemBytes = GRAD ? size_t(per) * 16 : size_t(kFwdRing<T>) * 16 * sizeof(T) * kRowThreads;
+    cfg.blockDim = dim3(kRowThreads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = unsigned(ctas), at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
     at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at, cfg.numAttrs = EPI == EPI_POLICY ? 2 : 1;  // (the policy loss follows row_scale_kernel)
+    cfg.attrs = at, cfg.numAttrs = 1;
+    int clusters = a.rows;
+    if (persistent) {
+        int fit = 0;
+        cfg.gridDim = dim3(unsigned(ctas));
+        e = cudaOccupancyMaxActiveClusters(&fit, f, &cfg);
+        if (e != cudaSuccess) return e;
+        clusters = std::min(clusters, std::max(fit, 1));
+        if (getenv("WB_V")) fprintf(stderr, "fit %d ctas %d smem %zu\n", fit, ctas, smem);
+    }
+    cfg.gridDim = dim3(unsigned(clusters) * unsigned(ctas));
+    cfg.numAttrs = follows ? 2 : 1;  // (the policy loss follows row_scale_kernel)
     e = cudaLaunchKernelEx(&cfg, f, a, per);
     count_launch(LAUNCH_LOSS);
     return e;
 }
-template <int EPI, bool GRAD>
-cudaError_t rows_launch(const LossArgs& a, int dtype, bool ent, int ctas, int per, cudaStream_t st) {
-    if (dtype == WHIRL_F32) return ent ? rows_launch<float, EPI, true, GRAD>(a, ctas, per, st) : rows_launch<float, EPI, false, GRAD>(a, ctas, per, st);
-    return ent ? rows_launch<uint16_t, EPI, true, GRAD>(a, ctas, per, st) : rows_launch<uint16_t, EPI, false, GRAD>(a, ctas, per, st);
-}
 
 int vectors_of(int n, int dtype) { return int((int64_t(n) * (dtype == WHIRL_F32 ? 4 : 2) + 15) / 16); }
 
+template <typename T, int EPI, bool ENT>
+cudaError_t forward_typed(const LossArgs& a, int ctas, int per, cudaStream_t st) {
+    static std::atomic<uint64_t> ready{0};
+    return cluster_launch(forward_kernel<T, EPI, ENT>, ready, a, ctas, per, size_t(kFwdRing<T>) * 16 * sizeof(T) * kRowThreads, false, EPI == EPI_POLICY, st);
+}
 template <int EPI>
 cudaError_t forward_launch(const LossArgs& a, int dtype, bool ent, cudaStream_t st) {
     const int nv = vectors_of(a.n, dtype);
     int ctas = 1;
-    while (ctas < 16 && int64_t(a.rows) * ctas < 888 && nv / (2 * ctas) >= 2 * kRowThreads) ctas *= 2;
+    while (ctas < 16 && int64_t(a.rows) * ctas < 1776 && nv / (2 * ctas) >= 2 * kRowThreads) ctas *= 2;
     if (const char* v = getenv("WB_CF")) ctas = atoi(v);
-    return rows_launch<EPI, false>(a, dtype, ent, ctas, (nv + ctas - 1) / ctas, st);
+    const int per = (nv + ctas - 1) / ctas;
+    if (dtype == WHIRL_F32) return ent ? forward_typed<float, EPI, true>(a, ctas, per, st) : forward_typed<float, EPI, false>(a, ctas, per, st);
+    return ent ? forward_typed<uint16_t, EPI, true>(a, ctas, per, st) : forward_typed<uint16_t, EPI, false>(a, ctas, per, st);
+}
+
+template <typename T, bool ENT>
+cudaError_t fused_typed(const LossArgs& a, int ctas, int per, cudaStream_t st) {
+    static std::atomic<uint64_t> ready{0};
+    return cluster_launch(fused_kernel<T, EPI_POLICY, ENT>, ready, a, ctas, per, size_t(per) * 16 + 3 * size_t(ctas) * kRowWarps * sizeof(Part<ENT>), true, true, st);
 }
 
 }  // namespace
@@ -882,7 +1144,10 @@ cudaError_t policy_launch(const LossArgs& a, int dtype, int mean, cudaStream_t s
     while (ctas < 16 && int64_t(a.rows) * ctas < 592 && nv / (2 * ctas) >= kRowThreads) ctas *= 2;
     if (const char* v = getenv("WB_CG")) ctas = atoi(v);
     const int64_t per = (int64_t(nv) + ctas - 1) / ctas;
-    if (a.dx && per * 16 <= kSliceMost) return rows_launch<EPI_POLICY, true>(a, dtype, ent, ctas, int(per), st);
+    if (a.dx && per * 16 <= kSliceMost) {
+        if (dtype == WHIRL_F32) return ent ? fused_typed<float, true>(a, ctas, int(per), st) : fused_typed<float, false>(a, ctas, int(per), st);
+        return ent ? fused_typed<uint16_t, true>(a, ctas, int(per), st) : fused_typed<uint16_t, false>(a, ctas, int(per), st);
+    }
     e = forward_launch<EPI_POLICY>(a, dtype, ent, st);
     return e == cudaSuccess && a.dx ? logprobs_grad_launch(a, dtype, st) : e;
 }
