@@ -353,7 +353,8 @@ int whirl_token_logprobs_grad(const void* x, int dtype, int rows, int n, int64_t
                               const float* inv_t_rows, const float* stats, const float* entropy, const float* g_logp,
                               const float* g_entropy, void* dx, int64_t ld_dx, void* stream);
 
-/* Bytes of workspace of the two losses below (0 <= rows, seqs). */
+/* Bytes of workspace of the two losses below, for up to `rows` rows and `seqs` sequences of the policy loss or pairs of the
+ * preference loss.  A workspace serves one call at a time. */
 size_t whirl_loss_workspace_bytes(int rows, int seqs);
 
 /* how a loss weighs its rows: s_row = w, w / (sum of w), or w / (sum of w over the row's sequence) / (sequences whose sum is

@@ -181,4 +181,4 @@ def test_decode_then_train():
     pref = api.preference_loss(x, token, start, ref_logp=scored.logp, beta=0.5)
     assert abs(pref.loss.item() - np.log(2)) < 1e-5               # the reference is the model itself
     fb = api.token_logprobs_grad(x, token, pref.stats, pref.g_logp)
-    assert torch.equal(fb, pref.dx)
+    assert (fb - pref.dx).abs().max() < 1e-6

@@ -218,8 +218,8 @@ def test_policy(rows, n, pad, off, mean, dtype):
     r = call()
     check_policy(r, x64, token, it, stats, adv, old, rf, weight, mean, starts, dtype, n, **kw)
     again = call()
-    for a, b in zip(vars(r).values(), vars(again).values()):
-        assert a is None or torch.equal(a, b)  # the same bits
+    for k in ("loss", "logp", "stats", "entropy", "kl", "row_loss", "g_logp", "row_scale", "dx"):
+        assert torch.equal(getattr(r, k), getattr(again, k))  # the same bits
     f = call(want_grad=False)
     assert f.dx is None  # (another kernel: its sums run in another order)
     check_policy(f, x64, token, it, stats, adv, old, rf, weight, mean, starts, dtype, n, **kw)
@@ -315,10 +315,12 @@ def test_preference(dtype, n, pad, kind, average):
     tol[torch.arange(rows), token.long()] += gt
     close(r.dx, d, tol, "dx")
     again = api.preference_loss(x, token.cuda(), starts.cuda(), rf.cuda(), weight.cuda(), **kw)
-    for a, b in zip(vars(r).values(), vars(again).values()):
-        assert torch.equal(a, b)
+    for k in ("loss", "pair_loss", "reward", "logp", "stats", "g_logp", "dx"):
+        assert torch.equal(getattr(r, k), getattr(again, k))
     f = api.preference_loss(x, token.cuda(), starts.cuda(), rf.cuda(), weight.cuda(), want_grad=False, **kw)
-    assert f.dx is None and torch.equal(f.loss, r.loss)
+    assert f.dx is None
+    close(f.loss, loss.mean(), lt.mean() + 2 * ref.EPS32 * loss.mean(), "loss without gradient")
+    close(f.g_logp, g, gt, "g_logp without gradient")
 
 
 def test_preference_edges():

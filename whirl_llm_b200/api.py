@@ -644,13 +644,26 @@ def token_logprobs_grad(x, token, stats, g_logp, inv_t: float = 1.0, inv_t_rows=
 class PolicyResult:
     loss: torch.Tensor                # [] float32
     logp: torch.Tensor                # [rows] float32, and so on
-    stats: torch.Tensor               # [rows, 2]
     entropy: Optional[torch.Tensor]   # (with ent_coef or want_entropy)
     kl: Optional[torch.Tensor]        # (with ref_logp)
     row_loss: torch.Tensor
-    g_logp: torch.Tensor              # d loss / d logp
-    row_scale: torch.Tensor           # a row's share of the loss; the entropy's gradient is -ent_coef * row_scale
-    dx: Optional[torch.Tensor]        # d loss / d x
+    dx: Optional[torch.Tensor]        # d loss / d x: logits.backward(result.dx) goes on from there
+    aux: torch.Tensor                 # what the properties below are views of (an allocation of its own each would cost more than the view)
+
+    @property
+    def stats(self) -> torch.Tensor:  # [rows, 2]: max, sum exp((x - max) * inv_t)
+        n = self.logp.numel()
+        return self.aux[: 2 * n].view(n, 2)
+
+    @property
+    def g_logp(self) -> torch.Tensor:  # d loss / d logp
+        n = self.logp.numel()
+        return self.aux[2 * n: 3 * n]
+
+    @property
+    def row_scale(self) -> torch.Tensor:  # a row's share of the loss; the entropy's gradient is -ent_coef * row_scale
+        n = self.logp.numel()
+        return self.aux[3 * n: 4 * n]
 
 
 def policy_loss(x, token, adv, old_logp=None, ref_logp=None, weight=None, seq_start=None, inv_t: float = 1.0, inv_t_rows=None,
@@ -669,17 +682,17 @@ def policy_loss(x, token, adv, old_logp=None, ref_logp=None, weight=None, seq_st
                      None if seq_start is None else _vec(seq_start, "seq_start", i32, (seqs + 1,), dev), seqs, mean,
                      _vec(inv_t_rows, "inv_t_rows", f32, rs, dev), inv_t, clip_low, clip_high, dual_clip, kl_coef, ent_coef)
     ent, kl = want_entropy or ent_coef != 0.0, ref_logp is not None
-    new = lambda: torch.empty(rows, dtype=f32, device=dev)  # noqa: E731  (one allocation each: views of a common one cost more)
-    v = new(), new(), new(), new(), new() if ent else None, new() if kl else None
-    loss, stats = torch.empty((), dtype=f32, device=dev), torch.empty((rows, 2), dtype=f32, device=dev)
-    if want_grad:
-        dx = _grad_out(x, dx, ld)
-    r = PolicyResult(loss, v[0], stats, v[4], v[5], v[1], v[2], v[3], dx if want_grad else None)
-    o = PolicyOut(loss.data_ptr(), v[0].data_ptr(), stats.data_ptr(), _p(r.entropy), _p(r.kl), v[1].data_ptr(), v[2].data_ptr(), v[3].data_ptr(),
-                  _p(r.dx), _loss_rows(dx)[3] if want_grad else 0)
-    ws = torch.empty(lib.whirl_loss_workspace_bytes(rows, seqs), dtype=torch.uint8, device=dev)
-    _call(dev, lib.whirl_policy_loss, x.data_ptr(), dt, rows, n, ld, C.byref(p), C.byref(o), ws.data_ptr(), ws.numel())
-    return r
+    loss, logp, row_loss = torch.empty((), dtype=f32, device=dev), torch.empty(rows, dtype=f32, device=dev), torch.empty(rows, dtype=f32, device=dev)
+    entropy = torch.empty(rows, dtype=f32, device=dev) if ent else None
+    kl = torch.empty(rows, dtype=f32, device=dev) if kl else None
+    nbytes = lib.whirl_loss_workspace_bytes(rows, seqs)
+    aux = torch.empty(4 * rows + (nbytes + 3) // 4, dtype=f32, device=dev)  # stats, g_logp, row_scale, and the workspace behind them
+    base = aux.data_ptr()
+    dx = _grad_out(x, dx, ld) if want_grad else None
+    o = PolicyOut(loss.data_ptr(), logp.data_ptr(), base, _p(entropy), _p(kl), row_loss.data_ptr(), base + 8 * rows, base + 12 * rows, _p(dx),
+                  _loss_rows(dx)[3] if want_grad else 0)
+    _call(dev, lib.whirl_policy_loss, x.data_ptr(), dt, rows, n, ld, p, o, base + 16 * rows, nbytes)
+    return PolicyResult(loss, logp, entropy, kl, row_loss, dx, aux)
 
 
 @dataclass
@@ -688,9 +701,18 @@ class PreferenceResult:
     pair_loss: torch.Tensor     # [pairs]
     reward: torch.Tensor        # [pairs, 2]: chosen, rejected
     logp: torch.Tensor          # [rows]
-    stats: torch.Tensor         # [rows, 2]
-    g_logp: torch.Tensor        # [rows]
-    dx: Optional[torch.Tensor]  # d loss / d x
+    dx: Optional[torch.Tensor]  # d loss / d x: logits.backward(result.dx) goes on from there
+    aux: torch.Tensor
+
+    @property
+    def stats(self) -> torch.Tensor:  # [rows, 2]: max, sum exp((x - max) * inv_t)
+        n = self.logp.numel()
+        return self.aux[: 2 * n].view(n, 2)
+
+    @property
+    def g_logp(self) -> torch.Tensor:  # d loss / d logp
+        n = self.logp.numel()
+        return self.aux[2 * n: 3 * n]
 
 
 def preference_loss(x, token, seq_start, ref_logp=None, weight=None, inv_t: float = 1.0, inv_t_rows=None, beta: float = 0.1,
@@ -707,15 +729,16 @@ def preference_loss(x, token, seq_start, ref_logp=None, weight=None, inv_t: floa
     p = PreferenceParams(_vec(token, "token", i32, rs, dev), _vec(seq_start, "seq_start", i32, (2 * pairs + 1,), dev),
                          _vec(ref_logp, "ref_logp", f32, rs, dev), _vec(weight, "weight", f32, rs, dev), _vec(inv_t_rows, "inv_t_rows", f32, rs, dev),
                          pairs, kind, int(average), inv_t, beta, smoothing, margin)
-    logp, g_logp = torch.empty(rows, dtype=f32, device=dev), torch.empty(rows, dtype=f32, device=dev)
+    loss, logp = torch.empty((), dtype=f32, device=dev), torch.empty(rows, dtype=f32, device=dev)
     pair_loss, reward = torch.empty(pairs, dtype=f32, device=dev), torch.empty((pairs, 2), dtype=f32, device=dev)
-    loss, stats = torch.empty((), dtype=f32, device=dev), torch.empty((rows, 2), dtype=f32, device=dev)
+    nbytes = lib.whirl_loss_workspace_bytes(rows, pairs)
+    aux = torch.empty(3 * rows + (nbytes + 3) // 4, dtype=f32, device=dev)  # stats, g_logp, and the workspace behind them
+    base = aux.data_ptr()
     dx = _grad_out(x, dx, ld) if want_grad else None
-    o = PreferenceOut(loss.data_ptr(), pair_loss.data_ptr(), reward.data_ptr(), logp.data_ptr(), stats.data_ptr(), g_logp.data_ptr(), _p(dx),
+    o = PreferenceOut(loss.data_ptr(), pair_loss.data_ptr(), reward.data_ptr(), logp.data_ptr(), base, base + 8 * rows, _p(dx),
                       _loss_rows(dx)[3] if want_grad else 0)
-    ws = torch.empty(lib.whirl_loss_workspace_bytes(rows, pairs), dtype=torch.uint8, device=dev)
-    _call(dev, lib.whirl_preference_loss, x.data_ptr(), dt, rows, n, ld, C.byref(p), C.byref(o), ws.data_ptr(), ws.numel())
-    return PreferenceResult(loss, pair_loss, reward, logp, stats, g_logp, dx)
+    _call(dev, lib.whirl_preference_loss, x.data_ptr(), dt, rows, n, ld, p, o, base + 12 * rows, nbytes)
+    return PreferenceResult(loss, pair_loss, reward, logp, dx, aux)
 
 
 # ---- the rows of the next step --------------------------------------------------------------------------------------------

@@ -495,14 +495,9 @@ LossWs loss_ws(int rows, int seqs) {
     const size_t r = rows < 1 ? 1 : size_t(rows), s = seqs < 1 ? 1 : size_t(seqs);
     LossWs w;
     size_t o = 0;
-    w.row_term = o, o = align_up(o + r * 8, 256);
-    w.seq_term = o, o = align_up(o + s * 8, 256);
-    w.stats = o, o = align_up(o + r * 8, 256);
-    w.entropy = o, o = align_up(o + r * 4, 256);
-    w.g_logp = o, o = align_up(o + r * 4, 256);
-    w.g_entropy = o, o = align_up(o + r * 4, 256);
-    w.row_scale = o, o = align_up(o + r * 4, 256);
-    w.ticket = o, o += 256;
+    auto take = [&](size_t& off, size_t bytes) { off = o, o = align_up(o + bytes, 256); };
+    take(w.row_term, r * 8), take(w.seq_term, s * 8), take(w.stats, r * 8);
+    take(w.entropy, r * 4), take(w.g_logp, r * 4), take(w.g_entropy, r * 4), take(w.row_scale, r * 4), take(w.ticket, 256);
     w.total = o;
     return w;
 }
@@ -597,7 +592,8 @@ int whirl_preference_loss(const void* x, int dtype, int rows, int n, int64_t ld,
     a.row_term = reinterpret_cast<double*>(static_cast<uint8_t*>(base) + w.row_term);
     a.seq_term = reinterpret_cast<double*>(static_cast<uint8_t*>(base) + w.seq_term);
     wb::PairArgs q{p->pairs, p->kind, p->average, p->beta, p->smoothing, p->margin, o->pair_loss, o->reward};
-    const cudaError_t e = wb::preference_launch(a, q, dtype, o->loss, static_cast<cudaStream_t>(stream));
+    a.ticket = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(base) + w.ticket), a.loss = o->loss;
+    const cudaError_t e = wb::preference_launch(a, q, dtype, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? WHIRL_OK : fail_cuda(e, "preference_loss launch");
 }
 

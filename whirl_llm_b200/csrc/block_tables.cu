@@ -186,45 +186,73 @@ __device__ __forceinline__ int last_upto(const int32_t* v, int n, int at) {
     return lo;
 }
 
-// block k (counted over the step) that is taken from the stack
-__device__ __forceinline__ int block_taken(const whirl_block_tables& t, const Plan& p, int count, int64_t have, int k) {
+// Block k (counted over the step) that is taken from the stack.  giver: the last one met, tried first (neighbouring blocks come from the
+// same one; a search is ten dependent loads).
+__device__ __forceinline__ int block_taken(const whirl_block_tables& t, const Plan& p, int count, int64_t have, int k, int& giver) {
     const int64_t at = have - 1 - k;
     if (at < count) return at >= 0 ? t.free_ids[at] : -1;
-    const int g = int(at - count), s = last_upto(p.back, t.seqs, g);  // the giver: the last sequence before whom at most g were given
-    return t.table[int64_t(s) * t.max_blocks + p.target[s] + (g - p.back[s])];
+    const int g = int(at - count);
+    if (giver < 0 || g < p.back[giver] || g >= p.back[giver] + (p.owned[giver] - p.target[giver])) giver = last_upto(p.back, t.seqs, g);
+    return t.table[int64_t(giver) * t.max_blocks + p.target[giver] + (g - p.back[giver])];
 }
 
 constexpr int kFillThreads = 256;
 
-__global__ void __launch_bounds__(kFillThreads) fill_kernel(const int32_t* length, whirl_block_tables t, whirl_step_rows r, void* ws) {
+// group: threads per sequence, a power of two from 32 on
+__global__ void __launch_bounds__(kFillThreads) fill_kernel(const int32_t* length, whirl_block_tables t, whirl_step_rows r, void* ws, int group) {
     asm volatile("griddepcontrol.wait;" ::: "memory");  // plan_kernel's results (the launch overlaps it)
     const Plan p = plan_of(ws, t.seqs);
     const int count = p.head->count, rows = p.head->rows;
     const int64_t have = p.head->have;
     const int64_t tid = int64_t(blockIdx.x) * kFillThreads + threadIdx.x, threads = int64_t(gridDim.x) * kFillThreads;
-    for (int64_t i = tid; i < r.max_rows; i += threads) {
-        int64_t slot = -1;
-        int pos = 0, s = -1;
-        if (i < rows) {
-            s = last_upto(r.row0, t.seqs, int(i));
-            pos = length[s] + int(i) - r.row0[s];
-            const int b = pos / t.block_size, own = p.owned[s];
-            const int id = b < own ? t.table[int64_t(s) * t.max_blocks + b] : block_taken(t, p, count, have, p.taken[s] + b - own);
-            slot = int64_t(id) * t.block_size + pos % t.block_size;
+    // four rows a thread: one search, and 16-byte stores where the arrays allow them
+    const bool wide = ((reinterpret_cast<uintptr_t>(r.slot) | reinterpret_cast<uintptr_t>(r.position) | reinterpret_cast<uintptr_t>(r.seq)) & 15) == 0;
+    for (int64_t i0 = tid * 4; i0 < r.max_rows; i0 += threads * 4) {
+        int64_t slot[4];
+        int pos[4], seq[4], s = -1, b = -1, id = 0, giver = -1;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int64_t i = i0 + k;
+            slot[k] = -1, pos[k] = 0, seq[k] = -1;
+            if (i < rows) {
+                int now = s < 0 ? last_upto(r.row0, t.seqs, int(i)) : s;
+                while (r.row0[now + 1] <= i) ++now;  // (row0[seqs] = rows > i)
+                pos[k] = length[now] + int(i) - r.row0[now];
+                const int at = pos[k] / t.block_size;
+                if (now != s || at != b) {
+                    const int own = p.owned[now];
+                    id = at < own ? t.table[int64_t(now) * t.max_blocks + at] : block_taken(t, p, count, have, p.taken[now] + at - own, giver);
+                }
+                s = now, b = at;
+                slot[k] = int64_t(id) * t.block_size + pos[k] % t.block_size, seq[k] = now;
+            }
         }
-        r.slot[i] = slot;
-        if (r.position) r.position[i] = pos;
-        if (r.seq) r.seq[i] = s;
+        if (wide && i0 + 4 <= r.max_rows) {
+            reinterpret_cast<longlong2*>(r.slot + i0)[0] = make_longlong2(slot[0], slot[1]);
+            reinterpret_cast<longlong2*>(r.slot + i0)[1] = make_longlong2(slot[2], slot[3]);
+            if (r.position) *reinterpret_cast<int4*>(r.position + i0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+            if (r.seq) *reinterpret_cast<int4*>(r.seq + i0) = make_int4(seq[0], seq[1], seq[2], seq[3]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (i0 + k >= r.max_rows) break;
+                r.slot[i0 + k] = slot[k];
+                if (r.position) r.position[i0 + k] = pos[k];
+                if (r.seq) r.seq[i0 + k] = seq[k];
+            }
+        }
     }
-    // a warp per sequence: what changes hands
-    for (int64_t s = tid >> 5; s < t.seqs; s += threads >> 5) {
+    // what changes hands
+    const int lane = int(tid & (group - 1));
+    for (int64_t s = tid / group; s < t.seqs; s += threads / group) {
         const int own = p.owned[s], target = p.target[s];
         int32_t* row = t.table + s * t.max_blocks;
-        for (int j = target + lane_id(); j < own; j += 32) {
+        for (int j = target + lane; j < own; j += group) {
             const int64_t to = int64_t(count) + p.back[s] + (j - target);
             if (to < t.num_blocks) t.free_ids[to] = row[j];
         }
-        for (int j = own + lane_id(); j < target; j += 32) row[j] = block_taken(t, p, count, have, p.taken[s] + (j - own));
+        int giver = -1;
+        for (int j = own + lane; j < target; j += group) row[j] = block_taken(t, p, count, have, p.taken[s] + (j - own), giver);
     }
 }
 
@@ -238,15 +266,19 @@ cudaError_t block_tables_launch(const int32_t* length, const int32_t* n_new, con
     count_launch(LAUNCH_BLOCKS);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    const int64_t want = std::max((int64_t(r.max_rows) + kFillThreads - 1) / kFillThreads, (int64_t(t.seqs) * 32 + kFillThreads - 1) / kFillThreads);
+    // four rows a thread; a quarter of a CTA per sequence where there are CTAs enough, so that long lists of blocks move side by side
+    const int64_t want = std::max((int64_t(r.max_rows) + 4 * kFillThreads - 1) / (4 * kFillThreads), (int64_t(t.seqs) * 64 + kFillThreads - 1) / kFillThreads);
     if (want == 0) return cudaSuccess;
+    const int64_t ctas = std::min<int64_t>(want, int64_t(sm_count) * 8);
+    int group = 32;
+    while (group < kFillThreads && int64_t(t.seqs) * group * 2 <= ctas * kFillThreads) group *= 2;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(std::min<int64_t>(want, int64_t(sm_count) * 8))), cfg.blockDim = dim3(kFillThreads), cfg.stream = st;
+    cfg.gridDim = dim3(unsigned(ctas)), cfg.blockDim = dim3(kFillThreads), cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at, cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, fill_kernel, length, t, r, ws);
+    e = cudaLaunchKernelEx(&cfg, fill_kernel, length, t, r, ws, group);
     count_launch(LAUNCH_BLOCKS);
     return e;
 }

@@ -191,8 +191,8 @@ struct LossArgs {
     float* row_scale;  // [rows] s of the policy loss; the rows' weights of the preference loss
     double* row_term;  // [rows] scaled row losses / weighted log ratios
     double* seq_term;  // [seqs] weight sums / pair losses
-    uint32_t* ticket;  // policy loss: rows finished so far (zeroed by the call)
-    float* loss;       // policy loss
+    uint32_t* ticket;  // rows finished so far (zeroed by the call)
+    float* loss;
 };
 struct PairArgs {
     int pairs, kind, average;
@@ -203,7 +203,7 @@ struct PairArgs {
 cudaError_t logprobs_launch(const LossArgs& a, int dtype, cudaStream_t st);
 cudaError_t logprobs_grad_launch(const LossArgs& a, int dtype, cudaStream_t st);
 cudaError_t policy_launch(const LossArgs& a, int dtype, int mean, cudaStream_t st);
-cudaError_t preference_launch(const LossArgs& a, const PairArgs& p, int dtype, float* loss, cudaStream_t st);
+cudaError_t preference_launch(const LossArgs& a, const PairArgs& p, int dtype, cudaStream_t st);
 
 // ---- cache block tables (block_tables.cu)
 size_t block_tables_ws_bytes(int seqs);

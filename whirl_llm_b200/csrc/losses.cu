@@ -10,8 +10,6 @@
 #include <algorithm>
 #include <atomic>
 #include <cfloat>
-#include <cstdlib>
-#include <cstdio>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -78,12 +76,14 @@ __device__ __forceinline__ Scale scale_of(float inv_t) {
     r.most = fminf(1e37f / r.hi, FLT_MAX);
     return r;
 }
-// the reference exponent of a maximum
-__device__ __forceinline__ float ref_of(float m, const Scale& c) { return fminf(fmaxf(m, -c.most), c.most) * c.hi; }
+// The reference exponent of a maximum: a whole number, so that moving a sum from one reference to another scales it by a power of two, exactly
+// (ex2.approx is low by 5e-8 on average: three moves of every partial sum would show in the log-probability).
+__device__ __forceinline__ float ref_of(float m, const Scale& c) { return rintf(fminf(fmaxf(m, -c.most), c.most) * c.hi); }
 
 // Partial statistics of a set of logits: m their maximum (-inf without one), e = ref_of(m), s - k = sum 2^(x c - e) (k: what
-// Kahan's sum owes), q = sum of the same terms times their exponent.  The exponent is one fused multiply-add from the logit; that e is a
-// rounded product shifts all terms of a row by the same factor, which row_sum() takes out again.
+// Kahan's sum owes), q = sum of the same terms times their exponent.  The exponent is two fused multiply-adds from the logit (first hi: the
+// difference to e is small, and rounded as such, before lo comes to it); that e is not
+// the maximum's own exponent shifts all terms of a row by the same factor (shift_of).
 // A plain float sum is not enough: in the thread that meets the row's peak every later term is rounded to the peak's last
 // bits, 300 times in a row of 151936, all of it landing in the log-probability (measured: 4e-7).
 struct Soft {
@@ -108,7 +108,7 @@ __device__ __forceinline__ void add_many(Soft& a, const float (&x)[N], const Sca
     if (m > a.m) raise<ENT>(a, m, c);
     float sum, qs = 0.f;
     if (N == 1) {
-        const float t = fmaf(x[0], c.hi, fmaf(x[0], c.lo, -a.e));
+        const float t = fmaf(x[0], c.lo, fmaf(x[0], c.hi, -a.e));
         sum = ex2_approx(t);
         if (ENT) qs = sum * fmaxf(t, -1000.f);
     } else {
@@ -117,7 +117,7 @@ __device__ __forceinline__ void add_many(Soft& a, const float (&x)[N], const Sca
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) {
             const F2 v = f2(x[2 * i], x[2 * i + 1]);
-            const float2 t = split(fma2(v, hi, fma2(v, lo, ne)));
+            const float2 t = split(fma2(v, lo, fma2(v, hi, ne)));
             w[i] = f2(ex2_approx(t.x), ex2_approx(t.y));
             if (ENT) q = fma2(w[i], f2(fmaxf(t.x, -1000.f), fmaxf(t.y, -1000.f)), q);  // (0 * -inf is not what a forbidden token adds)
         }
@@ -135,9 +135,7 @@ __device__ __forceinline__ void add_many(Soft& a, const float (&x)[N], const Sca
     if (ENT) a.q += qs;
 }
 
-// The statistics of all threads of the CTA, then of all CTAs of the cluster; the result is valid in warp 0 of every CTA.  Every
-// thread's sum is brought to the common maximum once (a tree of pairwise merges would scale it several times over, and
-// ex2.approx errs downwards, 5e-8 on average, each time).
+// The statistics of all threads of the CTA, then of all CTAs of the cluster; the result is valid in warp 0 of every CTA.
 struct ReduceShared {
     float m[32];
     float2 sq[32];
@@ -260,15 +258,16 @@ __device__ __forceinline__ int head_of(const T* p, int n) {
 
 constexpr double kLn2 = 0.6931471805599453;
 
-// The row's scalars are worked out by one thread while the CTA waits, once per row, in a kernel whose loops own the instruction cache: a
-// few short polynomials in 64 bits instead of the library's log, exp and expm1 (measured on the policy loss, 4096 x 151936 bf16: SCALARS).
-
-// log of a positive finite number: s = 2^k f with f in [sqrt 1/2, sqrt 2), log f = 2 atanh z, z = (f - 1) / (f + 1), |z| < 0.172; the
-// terms left out are below 1e-13.  NaN for what has no logarithm.
-__device__ __forceinline__ double ln_of(double s) {
-    if (!(s > 0.0 && s <= 1.7e308)) return NAN;
-    const int hi = __double2hiint(s), k = (hi - 0x3fe6a09e) >> 20;
-    const double f = __hiloint2double(hi - (k << 20), __double2loint(s)), b = f + 1.0;
+// The row's scalars are one warp's work per row, in the time that the others need for a slice: single-precision functions of the hardware
+// with one correction each, and 64 bits where a last bit would add up over a sequence.  (The library's log, exp and expm1 in 64
+// bits, and the divisions around them, took 2.7 us a row.)
+// log of a sum s > 0 (NaN without one): s = 2^k f with f in [sqrt 1/2, sqrt 2), log f = 2 atanh z, z = (f - 1) / (f + 1), |z| < 0.172; the
+// terms left out are below 1e-13.  (lg2.approx and a step of Newton's method with ex2.approx is low by 4e-8.)
+__device__ __forceinline__ double ln_of(float s) {
+    if (!(s > 0.f && s <= FLT_MAX)) return NAN;
+    const double d = double(s);
+    const int hi = __double2hiint(d), k = (hi - 0x3fe6a09e) >> 20;
+    const double f = __hiloint2double(hi - (k << 20), __double2loint(d)), b = f + 1.0;
     double r = double(__frcp_rn(float(b)));
     r = r * (2.0 - b * r);
     const double z = (f - 1.0) * r, y = z * z;
@@ -276,69 +275,60 @@ __device__ __forceinline__ double ln_of(double s) {
     t = fma(t, y, 1.0 / 11.0), t = fma(t, y, 1.0 / 9.0), t = fma(t, y, 1.0 / 7.0), t = fma(t, y, 1.0 / 5.0), t = fma(t, y, 1.0 / 3.0);
     return fma(double(k), kLn2, 2.0 * z * fma(t, y, 1.0));
 }
-// exp of |d| <= 25: d = n ln 2 + f, Taylor's sum to f^11 (what is left out is below 1e-14).  NaN stays.
-__device__ __forceinline__ double exp_of(double d) {
-    const double n = rint(d * 1.4426950408889634);
-    constexpr double hi = double(0.6931471805599453f), lo = kLn2 - hi;  // (n * hi is exact)
-    const double f = fma(n, -lo, fma(n, -hi, d));
-    double t = 1.0 / 39916800.0;
-    t = fma(t, f, 1.0 / 3628800.0), t = fma(t, f, 1.0 / 362880.0), t = fma(t, f, 1.0 / 40320.0), t = fma(t, f, 1.0 / 5040.0);
-    t = fma(t, f, 1.0 / 720.0), t = fma(t, f, 1.0 / 120.0), t = fma(t, f, 1.0 / 24.0), t = fma(t, f, 1.0 / 6.0);
-    t = fma(t, f, 0.5), t = fma(t, f, 1.0), t = fma(t, f, 1.0);
-    return d == d ? __hiloint2double(__double2hiint(t) + (int(n) << 20), __double2loint(t)) : d;
+// exp of |d| <= 20, the exponent's rounding errors taken out
+__device__ __forceinline__ float exp_of(float d) {
+    const float hi = d * kLog2e, lo = fmaf(d, kLog2e, -hi) + d * 1.92596299e-8f;  // (log2 e = kLog2e + 1.926e-8)
+    const float e = ex2_approx(hi);
+    return fmaf(e, lo * float(kLn2), e);
 }
-// exp k - k - 1 for |k| <= 25, without the cancellation around 0
-__device__ __forceinline__ double kl_of(double k) {
-    if (fabs(k) > 0.35) return exp_of(k) - 1.0 - k;
-    double t = 1.0 / 39916800.0;
-    t = fma(t, k, 1.0 / 3628800.0), t = fma(t, k, 1.0 / 362880.0), t = fma(t, k, 1.0 / 40320.0), t = fma(t, k, 1.0 / 5040.0);
-    t = fma(t, k, 1.0 / 720.0), t = fma(t, k, 1.0 / 120.0), t = fma(t, k, 1.0 / 24.0), t = fma(t, k, 1.0 / 6.0);
-    return k * k * fma(t, k, 0.5);
+// exp k - k - 1, by its series where the terms cancel
+__device__ __forceinline__ float kl_of(float k) {
+    if (!(fabsf(k) <= 1.f)) return exp_of(k) - 1.f - k;
+    float t = 1.f / 39916800.f;
+    t = fmaf(t, k, 1.f / 3628800.f), t = fmaf(t, k, 1.f / 362880.f), t = fmaf(t, k, 1.f / 40320.f), t = fmaf(t, k, 1.f / 5040.f);
+    t = fmaf(t, k, 1.f / 720.f), t = fmaf(t, k, 1.f / 120.f), t = fmaf(t, k, 1.f / 24.f), t = fmaf(t, k, 1.f / 6.f);
+    return k * k * fmaf(t, k, 0.5f);
 }
 
-// 2^(e - m c): what the rounded reference e of a row with maximum m puts into its sum.  Doubles: m c has to be exact to the last bits
-// of e.
-__device__ __forceinline__ double shift_of(double m, double e, double c) {
-    const double y = kLn2 * (e - m * c);
-    return fabs(y) < 1e-3 ? 1.0 + y * (1.0 + y * (0.5 + y * (1.0 / 6.0))) : exp_of(y < 25.0 ? y : 25.0);  // (|m c| <= 1e37: e is within 1e30 of it)
-}
+// The natural logarithm of what the reference e of a row with maximum m puts into its sum, ln 2 (e - m c).  64 bits: m c has to be exact
+// to the last bits of e.
+__device__ __forceinline__ double shift_of(float m, float e, float inv_t) { return kLn2 * (double(e) - double(m) * (double(inv_t) * 1.4426950408889634)); }
+__device__ __forceinline__ float shifted(float s, double y) { return s * exp_of(float(y)); }  // s e^y
 
 // The row's gradient: dx_j = w_j * (a + b * t_j), + d on the token, with t_j = x_j c - e (far: (x_j - e) c) and w_j = 2^t_j, whose sum
 // over the row is s:
 //   -inv_t g p_j - inv_t h p_j (log p_j + H),  p_j = w_j / s,  log p_j = ln 2 t_j - log s
 //   => a = -(inv_t / s) (g + h (H - log s)),  b = -(inv_t / s) h ln 2
 struct GradRow {
-    float e, c, a, b, d;
-    int token;
-    bool far;
+    float e, c, c_lo, a, b, d;
+    int token, far;
 };
-// sum: over exp((x - m) inv_t), m the row's maximum
-__device__ __forceinline__ GradRow grad_row(float m, double sum, float inv_t, int token, double g, double h, double entropy) {
+__device__ __forceinline__ GradRow grad_row(float m, bool far, float s, float ln_s, const Scale& c, float inv_t, int token, float g, float h, float entropy) {
     GradRow q;
-    q.c = inv_t * kLog2e, q.token = token;
-    const float most = fminf(1e37f / q.c, FLT_MAX);
-    q.far = !(m >= -most && m <= most);
-    q.e = q.far ? m : m * q.c;
-    const double s = q.far ? sum : sum / shift_of(m, q.e, q.c), k = double(inv_t) / s;
-    q.a = float(-k * (g + (h == 0.0 ? 0.0 : h * (entropy - ln_of(s)))));
-    q.b = float(-k * h * kLn2);
-    q.d = float(double(inv_t) * g);
+    q.far = far, q.e = far ? m : ref_of(m, c), q.c = c.hi, q.c_lo = c.lo, q.token = token;
+    const float k = inv_t / s;
+    q.a = -k * (h == 0.f ? g : g + h * (entropy - ln_s));
+    q.b = -k * h * float(kLn2);
+    q.d = inv_t * g;
     return q;
 }
 template <bool ENT>
 __device__ __forceinline__ float grad_of(const GradRow& q, float x) {
-    const float t = q.far ? (x - q.e) * q.c : fmaf(x, q.c, -q.e), w = ex2_approx(t);
+    const float t = q.far ? (x - q.e) * q.c : fmaf(x, q.c_lo, fmaf(x, q.c, -q.e)), w = ex2_approx(t);
     return ENT ? w * fmaf(q.b, fmaxf(t, -1000.f), q.a) : w * q.a;
 }
-template <bool ENT, int N>
+// LOW: with the scale's second float (a result of 8 bits does not show it)
+template <bool ENT, bool LOW, int N>
 __device__ __forceinline__ void grad_many(const GradRow& q, float (&x)[N]) {  // (not for a far row)
-    const F2 ne = f2(-q.e, -q.e), c = f2(q.c, q.c), a = f2(q.a, q.a), b = f2(q.b, q.b);
+    const F2 ne = f2(-q.e, -q.e), c = f2(q.c, q.c), lo = f2(q.c_lo, q.c_lo), a = f2(q.a, q.a), b = f2(q.b, q.b);
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
-        const float2 t = split(fma2(f2(x[i], x[i + 1]), c, ne));
+        const F2 v = f2(x[i], x[i + 1]);
+        const F2 t0 = fma2(v, c, ne);
+        const float2 t = split(LOW ? fma2(v, lo, t0) : t0);
         const F2 w = f2(ex2_approx(t.x), ex2_approx(t.y));
-        const float2 v = split(ENT ? mul2(w, fma2(b, f2(fmaxf(t.x, -1000.f), fmaxf(t.y, -1000.f)), a)) : mul2(w, a));
-        x[i] = v.x, x[i + 1] = v.y;
+        const float2 r = split(ENT ? mul2(w, fma2(b, f2(fmaxf(t.x, -1000.f), fmaxf(t.y, -1000.f)), a)) : mul2(w, a));
+        x[i] = r.x, x[i + 1] = r.y;
     }
 }
 // one vector of a row's gradient
@@ -346,7 +336,7 @@ template <typename T, bool ENT>
 __device__ __forceinline__ uint4 grad_vec(const GradRow& q, uint4 v) {
     float e[16 / sizeof(T)];
     unpack<T>(v, e);
-    grad_many<ENT, 16 / sizeof(T)>(q, e);
+    grad_many<ENT, sizeof(T) == 4, 16 / sizeof(T)>(q, e);
     return pack<T>(e);
 }
 
@@ -355,7 +345,7 @@ __device__ __forceinline__ uint4 grad_vec(const GradRow& q, uint4 v) {
 // ---------------------------------------------------------------------------------------------------------------
 
 constexpr int kRowThreads = 256;
-constexpr int kSliceMost = 200 * 1024;  // bytes of a row's slice that a CTA can hold
+constexpr int kSharedMost = 225 * 1024;  // bytes of dynamic shared memory that a CTA may ask for
 
 // A row as a user's call describes it, and whether it counts.
 struct RowOf {
@@ -392,85 +382,75 @@ __device__ __forceinline__ RowOf row_of(const LossArgs& a, int row, bool with_sc
     return r;
 }
 
-// The policy loss of one row (all in 64 bits: differences of log-probabilities).
+// The policy loss of one row.
 struct PolicyRow {
-    double loss, kl, dlogp;
+    float loss, kl, dlogp;
 };
-__device__ PolicyRow policy_row(const LossArgs& a, const RowOf& w, double logp, double entropy) {
+__device__ __forceinline__ PolicyRow policy_row(const LossArgs& a, const RowOf& w, double logp, float entropy) {
     PolicyRow p;
-    const double adv = w.adv;
-    double ratio = 1.0, pg, dpg;
+    const float adv = w.adv;
+    float ratio = 1.f;
     bool free_d = true;
     if (a.old_logp) {
-        double d = logp - double(w.old_logp);
-        free_d = !(d <= -20.0 || d >= 20.0);
-        d = d < -20.0 ? -20.0 : (d > 20.0 ? 20.0 : d);
-        ratio = exp_of(d);
+        const float d = float(logp - double(w.old_logp));
+        free_d = !(d <= -20.f || d >= 20.f);
+        ratio = exp_of(d < -20.f ? -20.f : (d > 20.f ? 20.f : d));
     }
-    const double lo = 1.0 - double(a.clip_low), hi = 1.0 + double(a.clip_high);
-    const double plain = ratio * adv, clipped = (ratio < lo ? lo : (ratio > hi ? hi : ratio)) * adv;
+    const float lo = 1.f - a.clip_low, hi = 1.f + a.clip_high;
+    const float plain = ratio * adv, clipped = (ratio < lo ? lo : (ratio > hi ? hi : ratio)) * adv;
     const bool takes_plain = plain <= clipped;
-    pg = takes_plain ? -plain : -clipped;
-    dpg = takes_plain && free_d ? -plain : 0.0;
-    if (a.dual_clip > 0.f && adv < 0.0 && pg > -double(a.dual_clip) * adv) pg = -double(a.dual_clip) * adv, dpg = 0.0;
-    p.kl = 0.0;
+    float pg = takes_plain ? -plain : -clipped;
+    p.dlogp = takes_plain && free_d ? -plain : 0.f;
+    if (a.dual_clip > 0.f && adv < 0.f && pg > -a.dual_clip * adv) pg = -a.dual_clip * adv, p.dlogp = 0.f;
+    if (logp != logp) p.dlogp = float(logp);
+    p.kl = 0.f;
     if (a.ref_logp) {
-        double k = double(w.ref_logp) - logp;
-        const bool free_k = !(k <= -20.0 || k >= 20.0);
-        k = k < -20.0 ? -20.0 : (k > 20.0 ? 20.0 : k);
+        float k = float(double(w.ref_logp) - logp);
+        const bool free_k = !(k <= -20.f || k >= 20.f);
+        k = k < -20.f ? -20.f : (k > 20.f ? 20.f : k);
         p.kl = kl_of(k);
-        pg += double(a.kl_coef) * p.kl;
-        if (free_k) dpg -= double(a.kl_coef) * (p.kl + k);
+        pg = fmaf(a.kl_coef, p.kl, pg);
+        if (free_k) p.dlogp -= a.kl_coef * (p.kl + k);
     }
-    p.loss = pg - (a.ent_coef != 0.f ? double(a.ent_coef) * entropy : 0.0);
-    p.dlogp = dpg;
+    p.loss = a.ent_coef != 0.f ? pg - a.ent_coef * entropy : pg;
     return p;
 }
 
-// What a row comes to; with `write`, what the call wants of it is written.  One thread.  s: the row's statistics, of which s.s may be
-// relative to a rounded reference (far: to the maximum itself).
+// What a row comes to, from its statistics: s relative to the reference e (far: to the maximum itself).
 struct RowDone {
-    double sum, entropy, g, h;
+    double logp, shift;
+    float m, s, ln_s, entropy, g, h;
+    PolicyRow p;
 };
 template <int EPI, bool ENT>
-__device__ __forceinline__ RowDone finish_row(const LossArgs& a, int row, bool write, const RowOf& w, float x_token, float m, float e, float s, float q,
-                                           bool far) {
-    RowDone done{};
-    double logp = 0.0, entropy = 0.0, sum = 0.0;
-    if (w.live) {
-        const double c = double(w.inv_t) * 1.4426950408889634;
-        // a row without a finite maximum has no distribution
-        sum = (m >= -FLT_MAX && m <= FLT_MAX) ? (far ? double(s) : double(s) * shift_of(m, e, c)) : double(NAN);
-        const double ls = ln_of(sum);
-        logp = (double(x_token) - double(m)) * double(w.inv_t) - ls;
-        // the terms' mean exponent is q / s from the reference, and e - m c more from the maximum
-        if (ENT) entropy = ls - kLn2 * (double(q) / double(s) + (far ? 0.0 : double(e) - double(m) * c));
-    } else {
-        m = 0.f;
-    }
-    done.sum = sum, done.entropy = entropy;
-    if (EPI != EPI_POLICY && !write) return done;
-    if (write && a.logp) a.logp[row] = float(logp);
-    if (write && a.stats) a.stats[2 * int64_t(row)] = m, a.stats[2 * int64_t(row) + 1] = float(sum);
-    if (write && ENT && a.entropy) a.entropy[row] = float(entropy);
+__device__ __forceinline__ RowDone row_done(const LossArgs& a, const RowOf& w, float x_token, float m, float e, float s, float q, bool far) {
+    RowDone r;
+    if (!(m >= -FLT_MAX && m <= FLT_MAX)) s = NAN;  // no distribution
+    const double ln_s = ln_of(s);
+    r.m = m, r.s = s, r.ln_s = float(ln_s), r.shift = far ? 0.0 : shift_of(m, e, w.inv_t);
+    r.logp = (double(x_token) - double(m)) * double(w.inv_t) - (ln_s + r.shift);
+    r.entropy = ENT ? float(ln_s - kLn2 * double(q / s)) : 0.f;
+    if (EPI == EPI_POLICY) r.p = policy_row(a, w, r.logp, r.entropy), r.g = w.scale * r.p.dlogp, r.h = -a.ent_coef * w.scale;
+    return r;
+}
+// Writes what the call wants of a row.  One thread.
+template <int EPI, bool ENT>
+__device__ __forceinline__ void write_row(const LossArgs& a, int row, const RowOf& w, const RowDone& r) {
+    const bool live = w.live;
+    if (a.logp) a.logp[row] = live ? float(r.logp) : 0.f;
+    if (a.stats) a.stats[2 * int64_t(row)] = live ? r.m : 0.f, a.stats[2 * int64_t(row) + 1] = live ? shifted(r.s, r.shift) : 0.f;
+    if (ENT && a.entropy) a.entropy[row] = live ? r.entropy : 0.f;
     if (EPI == EPI_POLICY) {
-        PolicyRow p{};
-        float scale = 0.f;
-        if (w.live) scale = w.scale, p = policy_row(a, w, logp, entropy);
-        done.g = float(double(scale) * p.dlogp), done.h = w.live ? -a.ent_coef * scale : 0.f;
-        if (write) {
-            if (a.kl) a.kl[row] = float(p.kl);
-            if (a.row_loss) a.row_loss[row] = float(p.loss);
-            if (a.g_logp) a.g_logp[row] = float(done.g);
-            if (a.g_entropy) a.g_entropy[row] = float(done.h);
-            a.row_term[row] = w.live ? double(scale) * p.loss : 0.0;
-        }
+        if (a.kl) a.kl[row] = live ? r.p.kl : 0.f;
+        if (a.row_loss) a.row_loss[row] = live ? r.p.loss : 0.f;
+        if (a.g_logp) a.g_logp[row] = live ? r.g : 0.f;
+        if (a.g_entropy) a.g_entropy[row] = live ? r.h : 0.f;
+        a.row_term[row] = live ? double(w.scale) * double(r.p.loss) : 0.0;
     } else if (EPI == EPI_PREF) {
-        a.row_term[row] = w.live ? double(w.weight) * (logp - (a.ref_logp ? double(w.ref_logp) : 0.0)) : 0.0;
-        a.row_scale[row] = w.live ? w.weight : 0.f;
+        a.row_term[row] = live ? double(w.weight) * (r.logp - (a.ref_logp ? double(w.ref_logp) : 0.0)) : 0.0;
+        a.row_scale[row] = live ? w.weight : 0.f;
         a.g_logp[row] = 0.f;  // (the rows of a pair get theirs from pairs_kernel)
     }
-    return done;
 }
 
 __device__ double block_sum(double v, double* sh) {  // the same value in every thread
@@ -486,22 +466,22 @@ __device__ double block_sum(double v, double* sh) {  // the same value in every 
 // was launched the ordinary way).
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// The CTA that comes last adds up the rows' terms, in their order.  (Called by `callers` CTAs in all, each after its thread 0 has written
-// the terms of its rows.)
-__device__ void last_sum(const LossArgs& a, unsigned callers) {
+// The CTA that comes last adds up the terms, in their order.  (Called by `callers` CTAs in all, each after its own terms are written.)
+__device__ void last_sum(uint32_t* ticket, unsigned callers, const double* terms, int count, double scale, float* loss) {
     __shared__ bool last;
     __shared__ double sh_d[32];
+    __syncthreads();
     if (threadIdx.x == 0) {
         __threadfence();
-        last = atomicAdd(a.ticket, 1u) + 1u == callers;
+        last = atomicAdd(ticket, 1u) + 1u == callers;
     }
     __syncthreads();
     if (!last) return;
     __threadfence();
     double t = 0.0;
-    for (int r = threadIdx.x; r < a.rows; r += blockDim.x) t += __ldcg(a.row_term + r);
+    for (int r = threadIdx.x; r < count; r += blockDim.x) t += __ldcg(terms + r);
     t = block_sum(t, sh_d);
-    if (threadIdx.x == 0) *a.loss = float(t);
+    if (threadIdx.x == 0) *loss = float(t * scale);
 }
 
 __device__ __forceinline__ void copy_async16(void* smem, const void* g) {
@@ -534,11 +514,11 @@ __device__ __forceinline__ void add_vec(Soft& s, uint4 v, const Scale& c) {
     add_many<ENT, 16 / sizeof(T)>(s, e, c);
 }
 // a far row's thread sums (see is_far); m: the row's maximum
-template <typename T, bool ENT>
+template <typename T, bool ENT, int NT>
 __device__ __noinline__ Soft far_sums(const uint4* v, int cnt, bool have_edge, float x_edge, float m, float c) {
     constexpr int E = 16 / sizeof(T);
     Soft a{m, 0.f, 0.f, 0.f, 0.f};
-    for (int i = threadIdx.x; i < cnt; i += blockDim.x) {
+    for (int i = threadIdx.x % NT; i < cnt; i += NT) {
         float x[E];
         unpack<T>(v[i], x);
         for (int j = 0; j < E; ++j) {
@@ -557,7 +537,7 @@ __device__ __noinline__ Soft far_sums(const uint4* v, int cnt, bool have_edge, f
 
 // vectors that a thread of the forward kernel has under way: kFwdRing steps of 16 logits each
 template <typename T>
-constexpr int kFwdRing = sizeof(T) == 4 ? 4 : 8;
+constexpr int kFwdRing = sizeof(T) == 4 ? 3 : 6;
 
 // Where a CTA's slice of a row lies: `per` 16-byte vectors of the row's body; the scalars before the first and behind the last boundary
 // belong to rank 0, one per thread.
@@ -589,7 +569,7 @@ __device__ __forceinline__ Soft row_sum(Soft s, const Scale& c, ReduceShared& sh
         __syncthreads();
         const float m = sh.m[0];
         __syncthreads();
-        s = reduce_far<ENT>(far_sums<T, ENT>(data, cnt, have_edge, x_edge, m, c.hi), m, sh, ctas);
+        s = reduce_far<ENT>(far_sums<T, ENT, kRowThreads>(data, cnt, have_edge, x_edge, m, c.hi), m, sh, ctas);
         far = true;
     }
     return s;
@@ -597,7 +577,7 @@ __device__ __forceinline__ Soft row_sum(Soft s, const Scale& c, ReduceShared& sh
 
 // Statistics: one cluster per row.  A thread reads what it copied into shared memory itself, so that the copies need no barrier.
 template <typename T, int EPI, bool ENT>
-__global__ void __launch_bounds__(kRowThreads, 3) forward_kernel(const __grid_constant__ LossArgs a, int per) {
+__global__ void __launch_bounds__(kRowThreads, 4) forward_kernel(const __grid_constant__ LossArgs a, int per) {
     constexpr int E = 16 / sizeof(T), NT = kRowThreads, V = 16 / E, D = kFwdRing<T>;
     extern __shared__ __align__(16) uint4 ring[];
     __shared__ ReduceShared sh;
@@ -651,73 +631,61 @@ __global__ void __launch_bounds__(kRowThreads, 3) forward_kernel(const __grid_co
         if (tid == 0 && rank == 0) {
             grid_dependency_wait();  // row_scale_kernel's results
             if (EPI == EPI_POLICY) w.scale = a.row_scale[row];
-            finish_row<EPI, ENT>(a, row, true, w, x_token, s.m, s.e, s.s, s.q, far);
+            write_row<EPI, ENT>(a, row, w, row_done<EPI, ENT>(a, w, x_token, s.m, s.e, s.s, s.q, far));
         }
     } else if (tid == 0 && rank == 0) {
         grid_dependency_wait();
-        finish_row<EPI, ENT>(a, row, true, w, 0.f, 0.f, 0.f, 0.f, 0.f, false);
+        write_row<EPI, ENT>(a, row, w, RowDone{});
     }
-    if (EPI == EPI_POLICY && rank == 0) last_sum(a, unsigned(a.rows));
+    if (EPI == EPI_POLICY && rank == 0) last_sum(a.ticket, unsigned(a.rows), a.row_term, a.rows, 1.0, a.loss);
 }
 
-// A warp's partial statistics, on their way to every CTA of the cluster
-template <bool ENT>
-struct Part;
-template <>
-struct Part<false> {
-    float m, s;
-};
-template <>
-struct Part<true> {
-    float m, s, q, pad;
+constexpr int kFusedThreads = 256, kFusedCtas = 5, kRowWarps = kFusedThreads / 32;
+
+// A warp's partial statistics of a row, on their way to every CTA of the cluster; x: the token's logit from the warp that has it, 0 from
+// the others (nobody reads it from memory: dx may be x, and another CTA may have written its part of the row by then).
+struct Part {
+    float m, s, q, x;
 };
 // stores to shared memory of CTA `cta` and counts the bytes on its barrier
-__device__ __forceinline__ void send(Part<false>* to, uint64_t* bar, int cta, float m, float s, float) {
+__device__ __forceinline__ void send(Part* to, uint64_t* bar, int cta, const Part& p) {
     asm volatile(
         "{\n .reg .b32 d, b;\n mapa.shared::cluster.u32 d, %0, %2;\n mapa.shared::cluster.u32 b, %1, %2;\n"
-        " st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [d], {%3, %4}, [b];\n}\n" ::"r"(smem_u32(to)),
-        "r"(smem_u32(bar)), "r"(cta), "r"(__float_as_uint(m)), "r"(__float_as_uint(s))
-        : "memory");
-}
-__device__ __forceinline__ void send(Part<true>* to, uint64_t* bar, int cta, float m, float s, float q) {
-    asm volatile(
-        "{\n .reg .b32 d, b;\n mapa.shared::cluster.u32 d, %0, %2;\n mapa.shared::cluster.u32 b, %1, %2;\n"
-        " st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [d], {%3, %4, %5, %5}, [b];\n}\n" ::"r"(smem_u32(to)),
-        "r"(smem_u32(bar)), "r"(cta), "r"(__float_as_uint(m)), "r"(__float_as_uint(s)), "r"(__float_as_uint(q))
+        " st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [d], {%3, %4, %5, %6}, [b];\n}\n" ::"r"(smem_u32(to)),
+        "r"(smem_u32(bar)), "r"(cta), "r"(__float_as_uint(p.m)), "r"(__float_as_uint(p.s)), "r"(__float_as_uint(p.q)), "r"(__float_as_uint(p.x))
         : "memory");
 }
 __device__ __forceinline__ void cluster_barrier() { asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-constexpr int kRowWarps = kRowThreads / 32;
-
 // Each warp's sums to every CTA of the cluster (its lane i tells CTA i).
 template <bool ENT>
-__device__ __forceinline__ void tell(Soft a, const Scale& c, Part<ENT>* parts, uint64_t* bar, int ctas, int rank) {
+__device__ __forceinline__ void tell(Soft a, float x_token, const Scale& c, Part* mine, uint64_t* bar, int ctas) {
     a.s -= a.k, a.k = 0.f;
     const float m = warp_max_f(a.m);
     raise<ENT>(a, m, c);
     a.s = warp_sum_f(a.s);
     if (ENT) a.q = warp_sum_f(a.q);
-    if (lane_id() < ctas) send(parts + rank * kRowWarps + (threadIdx.x >> 5), bar, lane_id(), m, a.s, a.q);
+    if (lane_id() < ctas) send(mine, bar, lane_id(), Part{m, a.s, a.q, x_token});
 }
-// The row's statistics from all warps' (one warp).  A barrier that does not complete in its time gives a row of NaN.
+// The row's statistics from n warps' (one warp).  A barrier that does not complete in its time gives a row of NaN.
 template <bool ENT>
-__device__ __forceinline__ Soft hear(const Scale& c, const Part<ENT>* parts, uint64_t* bar, uint32_t parity, int ctas, uint32_t& limit) {
-    const int n = ctas * kRowWarps;
-    if (lane_id() == 0) mbar_expect_tx(bar, uint32_t(n * sizeof(Part<ENT>)));
+__device__ __forceinline__ Soft hear(const Scale& c, const Part* parts, uint64_t* bar, uint32_t parity, int n, uint32_t& limit, float& x_token) {
+    if (lane_id() == 0) mbar_expect_tx(bar, uint32_t(n * sizeof(Part)));
     const bool came = __all_sync(0xffffffffu, mbar_wait(bar, parity, limit));
     if (!came) limit = 1;  // (and the rows after it do not wait that long again)
     float m = -INFINITY;
     for (int i = lane_id(); i < n; i += 32) m = fmaxf(m, parts[i].m);
     m = warp_max_f(m);
     Soft s{m, ref_of(m, c), 0.f, 0.f, 0.f};
+    float x = 0.f;
     for (int i = lane_id(); i < n; i += 32) {
-        Soft p{parts[i].m, ref_of(parts[i].m, c), parts[i].s, 0.f, 0.f};
-        if constexpr (ENT) p.q = parts[i].q;
-        raise<ENT>(p, m, c);
-        s.s += p.s;
-        if (ENT) s.q += p.q;
+        const Part p = parts[i];
+        Soft t{p.m, ref_of(p.m, c), p.s, 0.f, p.q};
+        raise<ENT>(t, m, c);
+        s.s += t.s, x += p.x;
+        if (ENT) s.q += t.q;
     }
+    x_token = warp_sum_f(x);
     s.s = warp_sum_f(s.s);
     if (ENT) s.q = warp_sum_f(s.q);
     if (!came) s.s = NAN;
@@ -730,9 +698,11 @@ __device__ __forceinline__ Soft hear(const Scale& c, const Part<ENT>* parts, uin
 // busy while the statistics of that row wait for it; several CTAs per SM fill each other's waits (the exchange of the statistics, the row's
 // scalars).  The statistics travel by stores that count on the receiver's mbarrier: a cluster barrier would hold every row until the
 // gradient's stores of the row before it are acknowledged.
-template <typename T, int EPI, bool ENT>
-__global__ void __launch_bounds__(kRowThreads, 5) fused_kernel(const __grid_constant__ LossArgs a, int per) {
-    constexpr int E = 16 / sizeof(T), NT = kRowThreads, V = 16 / E;
+
+template <typename T, bool ENT>
+__global__ void __launch_bounds__(kFusedThreads, kFusedCtas) fused_kernel(const __grid_constant__ LossArgs a, int per) {
+    constexpr int EPI = EPI_POLICY;
+    constexpr int E = 16 / sizeof(T), NT = kFusedThreads, V = 16 / E;
     extern __shared__ __align__(16) uint4 slice[];  // `per` vectors, then three sets of partial statistics (rows in turn; far rows)
     __shared__ GradRow s_q;
     __shared__ RowOf s_row[2];
@@ -741,7 +711,8 @@ __global__ void __launch_bounds__(kRowThreads, 5) fused_kernel(const __grid_cons
     __shared__ bool s_zero, s_far;
     const int ctas = int(cluster_size()), rank = int(cluster_rank()), tid = threadIdx.x;
     const int clusters = int(gridDim.x / unsigned(ctas));
-    Part<ENT>* const parts = reinterpret_cast<Part<ENT>*>(slice + per);
+    const int n_parts = ctas * kRowWarps, my_part = rank * kRowWarps + (tid >> 5);
+    Part* const parts = reinterpret_cast<Part*>(slice + per);
     int row = int(blockIdx.x / unsigned(ctas)), lives = 0, fars = 0;
     uint32_t limit = kWaitLimit;
     if (tid < 32) {
@@ -777,7 +748,6 @@ __global__ void __launch_bounds__(kRowThreads, 5) fused_kernel(const __grid_cons
         if (w.live) {
             const Scale c = scale_of(w.inv_t);
             Soft s = soft_empty(c);
-            const float x_token = tid == 0 ? load_one(at.x + w.token) : 0.f;
             if (at.edge >= 0) {
                 x_edge = load_one(at.x + at.edge);
                 const float e[1] = {x_edge};
@@ -789,20 +759,26 @@ __global__ void __launch_bounds__(kRowThreads, 5) fused_kernel(const __grid_cons
             for (; i + (V - 1) * NT < cnt; i += V * NT) add_block<T, ENT>(s, slice + i, NT, c);
 #pragma unroll 1
             for (; i < cnt; i += NT) add_vec<T, ENT>(s, slice[i], c);
+            // the token's logit goes along: one lane of the cluster has it
+            const int tok = w.token - at.head - at.v0 * E;
+            float x_token = at.edge >= 0 && w.token == at.edge ? x_edge : 0.f;
+            if (tok >= 0 && tok < cnt * E && (tok / E) % NT == tid) x_token = load_one(reinterpret_cast<const T*>(slice) + tok);
+            x_token = warp_sum_f(x_token);
             const int set = lives & 1;
-            tell<ENT>(s, c, parts + set * ctas * kRowWarps, &s_bar[set], ctas, rank);
-            auto finish = [&](const Soft& r, bool far) {  // one thread
+            tell<ENT>(s, x_token, c, parts + set * n_parts + my_part, &s_bar[set], ctas);
+            auto finish = [&](const Soft& r, bool far) {  // one thread: the CTA waits for it, so what it needs comes first
                 RowOf wr = w;
                 if (k == 0) {
                     grid_dependency_wait();  // row_scale_kernel's results
-                    if (EPI == EPI_POLICY) wr.scale = a.row_scale[row];
+                    wr.scale = a.row_scale[row];
                 }
-                const RowDone d = finish_row<EPI, ENT>(a, row, rank == 0, wr, x_token, r.m, r.e, r.s, r.q, far);
-                s_zero = d.g == 0.0 && d.h == 0.0;
-                s_q = grad_row(r.m, d.sum, wr.inv_t, wr.token, d.g, d.h, d.entropy);
+                const RowDone d = row_done<EPI, ENT>(a, wr, x_token, r.m, r.e, r.s, r.q, far);
+                s_zero = d.g == 0.f && d.h == 0.f;
+                s_q = grad_row(d.m, far, d.s, d.ln_s, c, wr.inv_t, wr.token, d.g, d.h, d.entropy);
+                if (rank == 0) write_row<EPI, ENT>(a, row, wr, d);
             };
             if (tid < 32) {
-                s = hear<ENT>(c, parts + set * ctas * kRowWarps, &s_bar[set], uint32_t(lives >> 1) & 1, ctas, limit);
+                s = hear<ENT>(c, parts + set * n_parts, &s_bar[set], uint32_t(lives >> 1) & 1, n_parts, limit, x_token);
                 if (tid == 0) {
                     s_far = is_far(s), s_m = s.m;
                     if (!is_far(s)) finish(s, false);
@@ -813,11 +789,12 @@ __global__ void __launch_bounds__(kRowThreads, 5) fused_kernel(const __grid_cons
             if (s_far) {  // (every CTA of the cluster has the same statistics)
                 const float m = s_m;
                 const Scale one{1.f, 0.f, FLT_MAX};
-                s = far_sums<T, ENT>(slice, cnt, at.edge >= 0, x_edge, m, c.hi);
+                s = far_sums<T, ENT, NT>(slice, cnt, at.edge >= 0, x_edge, m, c.hi);
                 s.m = 0.f, s.e = 0.f;  // (references alike: nothing is scaled on the way)
-                tell<ENT>(s, one, parts + 2 * ctas * kRowWarps, &s_bar[2], ctas, rank);
+                tell<ENT>(s, 0.f, one, parts + 2 * n_parts + my_part, &s_bar[2], ctas);
                 if (tid < 32) {
-                    s = hear<ENT>(one, parts + 2 * ctas * kRowWarps, &s_bar[2], uint32_t(fars) & 1, ctas, limit);
+                    float none;
+                    s = hear<ENT>(one, parts + 2 * n_parts, &s_bar[2], uint32_t(fars) & 1, n_parts, limit, none);
                     s.m = m;
                     if (tid == 0) finish(s, true);
                 }
@@ -828,7 +805,7 @@ __global__ void __launch_bounds__(kRowThreads, 5) fused_kernel(const __grid_cons
         } else {
             if (tid == 0) {
                 if (k == 0) grid_dependency_wait();
-                if (rank == 0) finish_row<EPI, ENT>(a, row, true, w, 0.f, 0.f, 0.f, 0.f, 0.f, false);
+                if (rank == 0) write_row<EPI, ENT>(a, row, w, RowDone{});
             }
             __syncthreads();
         }
@@ -880,7 +857,101 @@ __global__ void __launch_bounds__(kRowThreads, 5) fused_kernel(const __grid_cons
     }
     copies_but<0>();
     cluster_barrier();  // nobody leaves while another CTA's stores are under way to it
-    if (EPI == EPI_POLICY && rank == 0) last_sum(a, unsigned(clusters));
+    if (rank == 0) last_sum(a.ticket, unsigned(clusters), a.row_term, a.rows, 1.0, a.loss);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// short rows: a warp each
+// ---------------------------------------------------------------------------------------------------------------
+
+// A row of up to 8 KB fits the registers of one warp: it is read once, its statistics need no shared memory and no barrier, and (GRAD) its
+// gradient is written from the registers.  The kernels above spend 4 to 7 us of a CTA on a row however short it is: 8000 rows of
+// 2000 bf16 logits, policy loss with gradient, took 72 us with fused_kernel and take 50 here.
+constexpr int kSmallRowThreads = 256, kSmallVectors = 16;  // vectors a lane
+template <typename T, int EPI, bool ENT, bool GRAD>
+__global__ void __launch_bounds__(kSmallRowThreads, 2) small_rows_kernel(const __grid_constant__ LossArgs a) {
+    constexpr int E = 16 / sizeof(T), K = kSmallVectors;
+    const int lane = lane_id();
+    if (EPI == EPI_POLICY) grid_dependency_wait();  // row_scale_kernel's results
+    const int warps = int(gridDim.x) * (kSmallRowThreads / 32);
+#pragma unroll 1
+    for (int64_t row64 = int64_t(blockIdx.x) * (kSmallRowThreads / 32) + (threadIdx.x >> 5); row64 < a.rows; row64 += warps) {
+        const int row = int(row64);
+        const RowOf w = row_of<EPI>(a, row, true);
+        const T* x = static_cast<const T*>(a.x) + row64 * a.ld;
+        T* const dx = GRAD ? static_cast<T*>(a.dx) + row64 * a.ld_dx : nullptr;
+        const int head = head_of(x, a.n), nv = (a.n - head) / E, beside = a.n - nv * E;
+        const uint4* v = reinterpret_cast<const uint4*>(x + head);
+        const int edge = lane < beside ? (lane < head ? lane : lane + nv * E) : -1;  // (fewer than 2 E of them)
+        uint4 b[K];
+        float x_edge = 0.f;
+        GradRow q{};
+        if (w.live) {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                if (k * 32 < nv) b[k] = k * 32 + lane < nv ? v[k * 32 + lane] : make_uint4(0, 0, 0, 0);
+            const float x_token = load_one(x + w.token);
+            const Scale c = scale_of(w.inv_t);
+            Soft s = soft_empty(c);
+            if (edge >= 0) {
+                x_edge = load_one(x + edge);
+                const float e[1] = {x_edge};
+                add_many<ENT, 1>(s, e, c);
+            }
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                if (k * 32 + lane < nv) add_vec<T, ENT>(s, b[k], c);
+            __syncwarp();
+            s.s -= s.k, s.k = 0.f;
+            const float m = warp_max_f(s.m);
+            raise<ENT>(s, m, c);
+            s.s = warp_sum_f(s.s);
+            if (ENT) s.q = warp_sum_f(s.q);
+            const bool far = is_far(s);
+            if (far) {
+                Soft t = far_sums<T, ENT, 32>(v, nv, edge >= 0, x_edge, m, c.hi);
+                s.s = warp_sum_f(t.s), s.q = warp_sum_f(t.q);
+            }
+            const RowDone d = row_done<EPI, ENT>(a, w, x_token, s.m, s.e, s.s, s.q, far);
+            if (lane == 0) write_row<EPI, ENT>(a, row, w, d);
+            if (GRAD && !(d.g == 0.f && d.h == 0.f)) q = grad_row(d.m, far, d.s, d.ln_s, c, w.inv_t, w.token, d.g, d.h, d.entropy);
+        } else if (lane == 0) {
+            write_row<EPI, ENT>(a, row, w, RowDone{});
+        }
+        if (GRAD) {
+            __syncwarp();  // (every lane has read what it wants of the row: dx may be x)
+            const bool zero = q.a == 0.f && q.b == 0.f && q.d == 0.f;
+            const bool vec = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
+            const int t = zero ? -1 : q.token - head;  // the token's place among the vectors
+            if (edge >= 0) store_one(dx + edge, zero ? 0.f : grad_of<ENT>(q, x_edge) + (edge == q.token ? q.d : 0.f));
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const int i = k * 32 + lane;
+                if (i >= nv) continue;
+                float e[E];
+                if (zero) {
+#pragma unroll
+                    for (int j = 0; j < E; ++j) e[j] = 0.f;
+                } else {
+                    unpack<T>(b[k], e);
+                    if (!q.far) grad_many<ENT, sizeof(T) == 4, E>(q, e);
+                    else
+#pragma unroll
+                        for (int j = 0; j < E; ++j) e[j] = grad_of<ENT>(q, e[j]);
+                    if (t >= 0 && t / E == i)
+#pragma unroll
+                        for (int j = 0; j < E; ++j) e[j] += t % E == j ? q.d : 0.f;
+                }
+                if (vec) {
+                    __stcs(reinterpret_cast<uint4*>(dx + head) + i, pack<T>(e));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < E; ++j) store_one(dx + head + int64_t(i) * E + j, e[j]);
+                }
+            }
+        }
+    }
+    if (EPI == EPI_POLICY) last_sum(a.ticket, gridDim.x, a.row_term, a.rows, 1.0, a.loss);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -890,57 +961,75 @@ __global__ void __launch_bounds__(kRowThreads, 5) fused_kernel(const __grid_cons
 constexpr int kGradThreads = 256;
 
 template <typename T, bool ENT>
-__global__ void __launch_bounds__(kGradThreads) grad_kernel(const __grid_constant__ LossArgs a, int chunk) {
+__global__ void __launch_bounds__(kGradThreads, 6) grad_kernel(const __grid_constant__ LossArgs a, int chunk) {
     constexpr int E = 16 / sizeof(T), NT = kGradThreads;
     __shared__ GradRow s_q;
-    __shared__ bool s_zero;
     const int row = blockIdx.x, tid = threadIdx.x;
     const int64_t j0 = int64_t(blockIdx.y) * chunk;
     const int n = a.n - j0 < chunk ? int(a.n - j0) : chunk;
     const T* x = static_cast<const T*>(a.x) + int64_t(row) * a.ld + j0;
     T* dx = static_cast<T*>(a.dx) + int64_t(row) * a.ld_dx + j0;
-    if (tid == 0) {
-        const int token = a.token[row];
-        const float g = a.g_logp[row], h = ENT ? a.g_entropy[row] : 0.f;
-        s_zero = unsigned(token) >= unsigned(a.n) || (g == 0.f && h == 0.f);
-        if (!s_zero) {
-            const float inv_t = a.inv_t_rows ? a.inv_t_rows[row] : a.inv_t;
-            const float m = a.stats[2 * int64_t(row)], sum = a.stats[2 * int64_t(row) + 1];
-            s_q = grad_row(m, sum, inv_t, token, g, h, ENT ? a.entropy[row] : 0.f);
-        }
-    }
-    __syncthreads();
-    const bool zero = s_zero;
-    GradRow q{};
-    if (!zero) q = s_q;
-    const bool vec = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0 && !q.far;
-    const int head = vec ? head_of(x, n) : n, nv = (n - head) / E;
+    const int token = a.token[row];
+    const float g = a.g_logp[row], h = ENT ? a.g_entropy[row] : 0.f;
+    const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
+    const int head = same ? head_of(x, n) : n, nv = (n - head) / E;
     const uint4* v = reinterpret_cast<const uint4*>(x + head);
     uint4* dv = reinterpret_cast<uint4*>(dx + head);
-    const int64_t t64 = zero ? -1 : int64_t(q.token) - j0;
-    const int at = t64 >= 0 && t64 < n ? int(t64) : -1;
-    // the token's own logit, before anything is written (dx may be x)
-    const int t_vec = at - head;
-    const bool mine = at >= head && t_vec < nv * E && (t_vec / E) % NT == tid;
-    const float x_token = mine ? load_one(x + at) : 0.f;
-    if (zero) {
+    if (unsigned(token) >= unsigned(a.n) || (g == 0.f && h == 0.f)) {  // not read
 #pragma unroll 4
         for (int i = tid; i < nv; i += NT) __stcs(dv + i, make_uint4(0, 0, 0, 0));
-    } else {
-        int i = tid;
-#pragma unroll 1
-        for (; i + 3 * NT < nv; i += 4 * NT) {
-            const uint4 b[4] = {v[i], v[i + NT], v[i + 2 * NT], v[i + 3 * NT]};
+        for (int i = tid; i < n - nv * E; i += NT) store_one(dx + (i < head ? i : i + nv * E), 0.f);
+        return;
+    }
+    // the first vectors are under way while one thread makes the row's scalars
+    int i = tid;
+    uint4 b[4];
+    if (i + 3 * NT < nv) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) __stcs(dv + i + k * NT, grad_vec<T, ENT>(q, b[k]));
+        for (int k = 0; k < 4; ++k) b[k] = v[i + k * NT];
+    }
+    if (tid == 0) {
+        const float inv_t = a.inv_t_rows ? a.inv_t_rows[row] : a.inv_t;
+        const float m = a.stats[2 * int64_t(row)], sum = a.stats[2 * int64_t(row) + 1];
+        const Scale c = scale_of(inv_t);
+        const bool far = !(m >= -c.most && m <= c.most);
+        const double y = far ? 0.0 : shift_of(m, ref_of(m, c), inv_t);
+        s_q = grad_row(m, far, shifted(sum, -y), float(ln_of(sum) - y), c, inv_t, token, g, h, ENT ? a.entropy[row] : 0.f);
+    }
+    // the token's own logit, before anything is written (dx may be x)
+    const int64_t t64 = int64_t(token) - j0;
+    const int at = t64 >= 0 && t64 < n ? int(t64) : -1, t_vec = at - head;
+    const bool mine = at >= head && t_vec < nv * E && (t_vec / E) % NT == tid;
+    const float x_token = mine ? load_one(x + at) : 0.f;
+    __syncthreads();
+    const GradRow q = s_q;
+    if (!q.far) {
+#pragma unroll 1
+        while (i + 3 * NT < nv) {
+            uint4 o[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] = grad_vec<T, ENT>(q, b[k]);
+            const int next = i + 4 * NT;
+            if (next + 3 * NT < nv) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) b[k] = v[next + k * NT];
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) __stcs(dv + i + k * NT, o[k]);
+            i = next;
         }
 #pragma unroll 1
         for (; i < nv; i += NT) __stcs(dv + i, grad_vec<T, ENT>(q, v[i]));
+        if (mine) store_one(dx + at, grad_of<ENT>(q, x_token) + q.d);
+    } else {  // one by one
+        for (int k = tid; k < nv * E; k += NT) {
+            const int j = head + k;
+            store_one(dx + j, grad_of<ENT>(q, load_one(x + j)) + (j == at ? q.d : 0.f));
+        }
     }
-    if (mine) store_one(dx + at, grad_of<ENT>(q, x_token) + q.d);
-    for (int i = tid; i < head + (n - head - nv * E); i += NT) {
-        const int j = i < head ? i : i + nv * E;
-        store_one(dx + j, zero ? 0.f : grad_of<ENT>(q, load_one(x + j)) + (j == at ? q.d : 0.f));
+    for (int k = tid; k < n - nv * E; k += NT) {
+        const int j = k < head ? k : k + nv * E;
+        store_one(dx + j, grad_of<ENT>(q, load_one(x + j)) + (j == at ? q.d : 0.f));
     }
 }
 
@@ -963,11 +1052,8 @@ __device__ __forceinline__ int2 rows_of(const LossArgs& a, int s) {
 }
 
 // row_scale[rows] of the policy loss.  One CTA.
-__global__ void __launch_bounds__(kSmallThreads) row_scale_kernel(LossArgs a, int mean) {
-    __shared__ double sh[32];
+__device__ void row_scales(const LossArgs& a, int mean, double* sh) {
     const int tid = threadIdx.x;
-    asm volatile("griddepcontrol.launch_dependents;");
-    if (tid == 0) *a.ticket = 0;
     if (mean != WHIRL_MEAN_SEQS) {
         double k = 1.0;
         if (mean == WHIRL_MEAN_TOKENS) {
@@ -997,36 +1083,15 @@ __global__ void __launch_bounds__(kSmallThreads) row_scale_kernel(LossArgs a, in
         for (int r = b.x + lane_id(); r < b.y; r += 32) a.row_scale[r] = float(double(live_weight(a, r)) / t / have);
     }
 }
-
-// loss[0] = scale * sum of terms[count], in a fixed order.  One CTA.
-__global__ void __launch_bounds__(kSmallThreads) sum_kernel(const double* terms, int count, double scale, float* loss) {
+__global__ void __launch_bounds__(kSmallThreads) row_scale_kernel(const __grid_constant__ LossArgs a, int mean) {
     __shared__ double sh[32];
-    double t = 0.0;
-    for (int i = threadIdx.x; i < count; i += kSmallThreads) t += terms[i];
-    t = block_sum(t, sh);
-    if (threadIdx.x == 0) *loss = float(t * scale);
+    asm volatile("griddepcontrol.launch_dependents;");
+    if (threadIdx.x == 0) *a.ticket = 0;
+    row_scales(a, mean, sh);
 }
 
-// One CTA per pair: the sequences' sums, the pair's loss, and the rows' g_logp.
-constexpr int kPairThreads = 128;
-__global__ void __launch_bounds__(kPairThreads) pairs_kernel(LossArgs a, PairArgs p) {
-    __shared__ double sh[32];
-    const int i = blockIdx.x, tid = threadIdx.x;
-    int2 b[2];
-    double P[2], W[2];
-    for (int k = 0; k < 2; ++k) {
-        b[k] = rows_of(a, 2 * i + k);
-        double t = 0.0, w = 0.0;
-        for (int r = b[k].x + tid; r < b[k].y; r += kPairThreads) t += a.row_term[r], w += double(a.row_scale[r]);
-        P[k] = block_sum(t, sh);
-        W[k] = 1.0;
-        if (p.average) {
-            w = block_sum(w, sh);
-            W[k] = w > 0.0 ? 1.0 / w : 0.0;
-            P[k] = w > 0.0 ? P[k] / w : 0.0;
-        }
-    }
-    const double beta = p.beta, h = beta * (P[0] - P[1]) - double(p.margin);
+// Loss of a pair and its derivative by h.
+__device__ double2 pair_loss_of(const PairArgs& p, double h) {
     double loss, dh;
     if (p.kind == WHIRL_PREF_SIGMOID) {
         const double ls = p.smoothing, e = exp(-fabs(h)), l = log1p(e);
@@ -1037,35 +1102,68 @@ __global__ void __launch_bounds__(kPairThreads) pairs_kernel(LossArgs a, PairArg
         dh = ls * up - (1.0 - ls) * down;
     } else if (p.kind == WHIRL_PREF_HINGE) {
         loss = h != h ? h : (h < 1.0 ? 1.0 - h : 0.0);
-        dh = h < 1.0 ? -1.0 : 0.0;
+        dh = h != h ? h : (h < 1.0 ? -1.0 : 0.0);
     } else {
-        const double t = (h - 0.5) / beta;
-        loss = t * t, dh = 2.0 * t / beta;
+        const double t = (h - 0.5) / double(p.beta);
+        loss = t * t, dh = 2.0 * t / double(p.beta);
     }
-    const double coef = beta * dh / double(p.pairs);
-    for (int k = 0; k < 2; ++k)
-        for (int r = b[k].x + tid; r < b[k].y; r += kPairThreads) a.g_logp[r] = float((k ? -coef : coef) * W[k] * double(a.row_scale[r]));
-    if (tid == 0) {
-        a.seq_term[i] = loss;
-        if (p.pair_loss) p.pair_loss[i] = float(loss);
-        if (p.reward) p.reward[2 * i] = float(beta * P[0]), p.reward[2 * i + 1] = float(beta * P[1]);
+    return make_double2(loss, dh);
+}
+__device__ void write_pair(const LossArgs& a, const PairArgs& p, int i, double loss, double chosen, double rejected) {
+    a.seq_term[i] = loss;
+    if (p.pair_loss) p.pair_loss[i] = float(loss);
+    if (p.reward) p.reward[2 * i] = float(double(p.beta) * chosen), p.reward[2 * i + 1] = float(double(p.beta) * rejected);
+}
+// The sequences' sums of pair i, its loss, and the factor of every row's weight in g_logp (chosen, rejected).  The whole CTA.
+__device__ double2 pair_done(const LossArgs& a, const PairArgs& p, int i, int2 (&b)[2], double* sh) {
+    const int first = int(threadIdx.x), stride = int(blockDim.x);
+    double P[2], W[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        b[k] = rows_of(a, 2 * i + k);
+        double t = 0.0, w = 0.0;
+#pragma unroll 8
+        for (int r = b[k].x + first; r < b[k].y; r += stride) t += __ldcg(a.row_term + r), w += double(__ldcg(a.row_scale + r));
+        P[k] = block_sum(t, sh);
+        W[k] = 1.0;
+        if (p.average) {
+            w = block_sum(w, sh);
+            W[k] = w > 0.0 ? 1.0 / w : 0.0;
+            P[k] = w > 0.0 ? P[k] / w : 0.0;
+        }
     }
+    const double2 l = pair_loss_of(p, double(p.beta) * (P[0] - P[1]) - double(p.margin));
+    if (first == 0) write_pair(a, p, i, l.x, P[0], P[1]);
+    const double coef = double(p.beta) * l.y / double(p.pairs);
+    return make_double2(coef * W[0], -coef * W[1]);
 }
 
-// A launch of forward_kernel / fused_kernel: `ctas` CTAs in a cluster, `per` vectors of a row each, at most `clusters` clusters.
-template <typename F>
-cudaError_t cluster_launch(F f, std::atomic<uint64_t>& ready, const LossArgs& a, int ctas, int per, size_t smem, bool persistent, bool follows, cudaStream_t st) {
+// One CTA per pair: the sequences' sums, the pair's loss, and the rows' g_logp.
+constexpr int kPairThreads = 256;
+__global__ void __launch_bounds__(kPairThreads) pairs_kernel(const __grid_constant__ LossArgs a, const __grid_constant__ PairArgs p) {
+    __shared__ double sh[32];
+    int2 b[2];
+    const double2 c = pair_done(a, p, blockIdx.x, b, sh);
+    for (int k = 0; k < 2; ++k)
+        for (int r = b[k].x + int(threadIdx.x); r < b[k].y; r += kPairThreads) a.g_logp[r] = float((k ? c.y : c.x) * double(a.row_scale[r]));
+    last_sum(a.ticket, gridDim.x, a.seq_term, p.pairs, 1.0 / p.pairs, a.loss);
+}
+
+// A launch by clusters of `ctas` CTAs: one cluster per row, or (persistent) as many as fit at once.
+template <typename... P>
+cudaError_t cluster_launch(void (*f)(LossArgs, P...), std::atomic<uint64_t>& ready, const LossArgs& a, int ctas, int threads, size_t smem, bool persistent,
+                           bool follows, cudaStream_t st, P... rest) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev > 63 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {  // bit per device: the function's limits are raised
-        e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kSliceMost);
+        e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMost);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
         if (dev < 64) ready.fetch_or(uint64_t(1) << dev, std::memory_order_release);
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.blockDim = dim3(kRowThreads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
+    cfg.blockDim = dim3(unsigned(threads)), cfg.dynamicSmemBytes = smem, cfg.stream = st;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = unsigned(ctas), at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
@@ -1079,28 +1177,49 @@ cudaError_t cluster_launch(F f, std::atomic<uint64_t>& ready, const LossArgs& a,
         e = cudaOccupancyMaxActiveClusters(&fit, f, &cfg);
         if (e != cudaSuccess) return e;
         clusters = std::min(clusters, std::max(fit, 1));
-        if (getenv("WB_V")) fprintf(stderr, "fit %d ctas %d smem %zu\n", fit, ctas, smem);
     }
     cfg.gridDim = dim3(unsigned(clusters) * unsigned(ctas));
     cfg.numAttrs = follows ? 2 : 1;  // (the policy loss follows row_scale_kernel)
-    e = cudaLaunchKernelEx(&cfg, f, a, per);
+    e = cudaLaunchKernelEx(&cfg, f, a, rest...);
     count_launch(LAUNCH_LOSS);
     return e;
 }
 
 int vectors_of(int n, int dtype) { return int((int64_t(n) * (dtype == WHIRL_F32 ? 4 : 2) + 15) / 16); }
 
+bool is_small(int n, int dtype) { return vectors_of(n, dtype) <= 32 * kSmallVectors; }
+template <typename T, int EPI, bool ENT, bool GRAD>
+cudaError_t small_typed(const LossArgs& a, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    const int64_t want = (int64_t(a.rows) + kSmallRowThreads / 32 - 1) / (kSmallRowThreads / 32);
+    cfg.gridDim = dim3(unsigned(std::min<int64_t>(want, 148 * 8))), cfg.blockDim = dim3(kSmallRowThreads), cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at, cfg.numAttrs = EPI == EPI_POLICY ? 1 : 0;  // (the policy loss follows row_scale_kernel)
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, small_rows_kernel<T, EPI, ENT, GRAD>, a);
+    count_launch(LAUNCH_LOSS);
+    return e;
+}
+template <int EPI, bool GRAD>
+cudaError_t small_launch(const LossArgs& a, int dtype, bool ent, cudaStream_t st) {
+    if (dtype == WHIRL_F32) return ent ? small_typed<float, EPI, true, GRAD>(a, st) : small_typed<float, EPI, false, GRAD>(a, st);
+    return ent ? small_typed<uint16_t, EPI, true, GRAD>(a, st) : small_typed<uint16_t, EPI, false, GRAD>(a, st);
+}
+
 template <typename T, int EPI, bool ENT>
 cudaError_t forward_typed(const LossArgs& a, int ctas, int per, cudaStream_t st) {
     static std::atomic<uint64_t> ready{0};
-    return cluster_launch(forward_kernel<T, EPI, ENT>, ready, a, ctas, per, size_t(kFwdRing<T>) * 16 * sizeof(T) * kRowThreads, false, EPI == EPI_POLICY, st);
+    return cluster_launch(forward_kernel<T, EPI, ENT>, ready, a, ctas, kRowThreads, size_t(kFwdRing<T>) * 16 * sizeof(T) * kRowThreads, false, EPI == EPI_POLICY, st, per);
 }
 template <int EPI>
 cudaError_t forward_launch(const LossArgs& a, int dtype, bool ent, cudaStream_t st) {
+    if (is_small(a.n, dtype)) return small_launch<EPI, false>(a, dtype, ent, st);
     const int nv = vectors_of(a.n, dtype);
+    // Enough CTAs to fill the GPU three times over, 2 steps of the ring each at least: 1024 rows of 262144 f32 logits take 159 us with two
+    // CTAs a row, 164 with one, 182 with four.
     int ctas = 1;
     while (ctas < 16 && int64_t(a.rows) * ctas < 1776 && nv / (2 * ctas) >= 2 * kRowThreads) ctas *= 2;
-    if (const char* v = getenv("WB_CF")) ctas = atoi(v);
     const int per = (nv + ctas - 1) / ctas;
     if (dtype == WHIRL_F32) return ent ? forward_typed<float, EPI, true>(a, ctas, per, st) : forward_typed<float, EPI, false>(a, ctas, per, st);
     return ent ? forward_typed<uint16_t, EPI, true>(a, ctas, per, st) : forward_typed<uint16_t, EPI, false>(a, ctas, per, st);
@@ -1109,7 +1228,7 @@ cudaError_t forward_launch(const LossArgs& a, int dtype, bool ent, cudaStream_t 
 template <typename T, bool ENT>
 cudaError_t fused_typed(const LossArgs& a, int ctas, int per, cudaStream_t st) {
     static std::atomic<uint64_t> ready{0};
-    return cluster_launch(fused_kernel<T, EPI_POLICY, ENT>, ready, a, ctas, per, size_t(per) * 16 + 3 * size_t(ctas) * kRowWarps * sizeof(Part<ENT>), true, true, st);
+    return cluster_launch(fused_kernel<T, ENT>, ready, a, ctas, kFusedThreads, size_t(per) * 16 + 3 * size_t(ctas) * kRowWarps * sizeof(Part), true, true, st, per);
 }
 
 }  // namespace
@@ -1138,13 +1257,14 @@ cudaError_t policy_launch(const LossArgs& a, int dtype, int mean, cudaStream_t s
     if (e != cudaSuccess) return e;
     const bool ent = a.ent_coef != 0.f || a.entropy;
     const int nv = vectors_of(a.n, dtype);
-    int ctas = 1, most = 44 * 1024;
-    if (const char* v = getenv("WB_SL")) most = atoi(v) * 1024;
-    while (ctas < 16 && int64_t(nv + ctas - 1) / ctas * 16 > most) ctas *= 2;
-    while (ctas < 16 && int64_t(a.rows) * ctas < 592 && nv / (2 * ctas) >= kRowThreads) ctas *= 2;
-    if (const char* v = getenv("WB_CG")) ctas = atoi(v);
+    if (a.dx && is_small(a.n, dtype)) return small_launch<EPI_POLICY, true>(a, dtype, ent, st);
+    // The smallest cluster whose slices leave room for three CTAs an SM (rows of 1 MB: 16 CTAs 489 us, 8 CTAs 636; 512 KB: 8 CTAs 256, 16 CTAs
+    // 277, 4 CTAs 309; 300 KB: 8 CTAs 487, 4 CTAs 535, 16 CTAs 663), and a larger one where the rows would not fill the GPU.
+    int ctas = 1;
+    while (ctas < 16 && int64_t(nv + ctas - 1) / ctas * 16 > 70 * 1024) ctas *= 2;
+    while (ctas < 16 && int64_t(a.rows) * ctas < 592 && nv / (2 * ctas) >= kFusedThreads) ctas *= 2;
     const int64_t per = (int64_t(nv) + ctas - 1) / ctas;
-    if (a.dx && per * 16 <= kSliceMost) {
+    if (a.dx && per * 16 <= kSharedMost - 8192) {
         if (dtype == WHIRL_F32) return ent ? fused_typed<float, true>(a, ctas, int(per), st) : fused_typed<float, false>(a, ctas, int(per), st);
         return ent ? fused_typed<uint16_t, true>(a, ctas, int(per), st) : fused_typed<uint16_t, false>(a, ctas, int(per), st);
     }
@@ -1152,22 +1272,16 @@ cudaError_t policy_launch(const LossArgs& a, int dtype, int mean, cudaStream_t s
     return e == cudaSuccess && a.dx ? logprobs_grad_launch(a, dtype, st) : e;
 }
 
-cudaError_t preference_launch(const LossArgs& a, const PairArgs& p, int dtype, float* loss, cudaStream_t st) {
-    if (a.rows > 0) {
-        const cudaError_t e = forward_launch<EPI_PREF>(a, dtype, false, st);
-        if (e != cudaSuccess) return e;
-    }
+cudaError_t preference_launch(const LossArgs& a, const PairArgs& p, int dtype, cudaStream_t st) {
+    cudaError_t e = cudaMemsetAsync(p.pairs > 0 ? static_cast<void*>(a.ticket) : static_cast<void*>(a.loss), 0, 4, st);  // (no pairs: the loss is 0)
+    if (e == cudaSuccess && a.rows > 0) e = forward_launch<EPI_PREF>(a, dtype, false, st);
+    if (e != cudaSuccess) return e;
     if (p.pairs > 0) {
         pairs_kernel<<<p.pairs, kPairThreads, 0, st>>>(a, p);
         count_launch(LAUNCH_LOSS);
+        e = cudaGetLastError();
     }
-    if (a.dx && a.rows > 0) {
-        const cudaError_t e = logprobs_grad_launch(a, dtype, st);
-        if (e != cudaSuccess) return e;
-    }
-    sum_kernel<<<1, kSmallThreads, 0, st>>>(a.seq_term, p.pairs, p.pairs > 0 ? 1.0 / p.pairs : 0.0, loss);
-    count_launch(LAUNCH_LOSS);
-    return cudaGetLastError();
+    return e == cudaSuccess && a.dx && a.rows > 0 ? logprobs_grad_launch(a, dtype, st) : e;
 }
 
 }  // namespace wb
