@@ -355,9 +355,9 @@ struct RowOf {
     float scale;                    // row_scale, where it was known when the row was read
     bool live;
 };
-// Read by a warp, one word per lane, so that a row costs one trip to memory; every lane gets the whole.
+// Read by a warp, one word per lane, so that a row costs one trip to memory (row_word); every lane then gets the whole (row_from).
 template <int EPI>
-__device__ __forceinline__ RowOf row_of(const LossArgs& a, int row, bool with_scale) {
+__device__ __forceinline__ uint32_t row_word(const LossArgs& a, int row, bool with_scale) {
     const int lane = lane_id();
     const void* p = nullptr;
     if (lane == 0) p = a.token + row;
@@ -369,7 +369,9 @@ __device__ __forceinline__ RowOf row_of(const LossArgs& a, int row, bool with_sc
     else if (lane == 6 && EPI == EPI_POLICY && with_scale) p = a.row_scale + row;
     else if (lane == 7 && a.seq_start) p = a.seq_start;
     else if (lane == 8 && a.seq_start) p = a.seq_start + a.seqs;
-    const uint32_t got = p ? *static_cast<const uint32_t*>(p) : 0u;
+    return p ? *static_cast<const uint32_t*>(p) : 0u;
+}
+__device__ __forceinline__ RowOf row_from(const LossArgs& a, int row, uint32_t got) {
     auto word = [&](int l) { return __shfl_sync(0xffffffffu, got, l); };
     auto real = [&](int l) { return __uint_as_float(word(l)); };
     RowOf r;
@@ -381,6 +383,8 @@ __device__ __forceinline__ RowOf row_of(const LossArgs& a, int row, bool with_sc
     r.live = unsigned(r.token) < unsigned(a.n) && r.weight > 0.f && (!a.seq_start || (row >= first && row < end));
     return r;
 }
+template <int EPI>
+__device__ __forceinline__ RowOf row_of(const LossArgs& a, int row, bool with_scale) { return row_from(a, row, row_word<EPI>(a, row, with_scale)); }
 
 // The policy loss of one row.
 struct PolicyRow {
@@ -434,7 +438,7 @@ __device__ __forceinline__ RowDone row_done(const LossArgs& a, const RowOf& w, f
     return r;
 }
 // Writes what the call wants of a row.  One thread.
-template <int EPI, bool ENT>
+template <int EPI, bool ENT, bool TERM = true>
 __device__ __forceinline__ void write_row(const LossArgs& a, int row, const RowOf& w, const RowDone& r) {
     const bool live = w.live;
     if (a.logp) a.logp[row] = live ? float(r.logp) : 0.f;
@@ -445,7 +449,7 @@ __device__ __forceinline__ void write_row(const LossArgs& a, int row, const RowO
         if (a.row_loss) a.row_loss[row] = live ? r.p.loss : 0.f;
         if (a.g_logp) a.g_logp[row] = live ? r.g : 0.f;
         if (a.g_entropy) a.g_entropy[row] = live ? r.h : 0.f;
-        a.row_term[row] = live ? double(w.scale) * double(r.p.loss) : 0.0;
+        if (TERM) a.row_term[row] = live ? double(w.scale) * double(r.p.loss) : 0.0;
     } else if (EPI == EPI_PREF) {
         a.row_term[row] = live ? double(w.weight) * (r.logp - (a.ref_logp ? double(w.ref_logp) : 0.0)) : 0.0;
         a.row_scale[row] = live ? w.weight : 0.f;
@@ -479,7 +483,14 @@ __device__ void last_sum(uint32_t* ticket, unsigned callers, const double* terms
     if (!last) return;
     __threadfence();
     double t = 0.0;
-    for (int r = threadIdx.x; r < count; r += blockDim.x) t += __ldcg(terms + r);
+    const int stride = int(blockDim.x);
+    for (int r = threadIdx.x; r < count; r += 8 * stride) {  // (eight loads at a time: one CTA, and nobody to hide its waits)
+        double v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = int64_t(r) + k * stride < count ? __ldcg(terms + r + k * stride) : 0.0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t += v[k];
+    }
     t = block_sum(t, sh_d);
     if (threadIdx.x == 0) *loss = float(t * scale);
 }
@@ -867,17 +878,67 @@ __global__ void __launch_bounds__(kFusedThreads, kFusedCtas) fused_kernel(const 
 // A row of up to 8 KB fits the registers of one warp: it is read once, its statistics need no shared memory and no barrier, and (GRAD) its
 // gradient is written from the registers.  The kernels above spend 4 to 7 us of a CTA on a row however short it is: 8000 rows of
 // 2000 bf16 logits, policy loss with gradient, took 72 us with fused_kernel and take 50 here.
-constexpr int kSmallRowThreads = 256, kSmallVectors = 16;  // vectors a lane
-template <typename T, int EPI, bool ENT, bool GRAD>
-__global__ void __launch_bounds__(kSmallRowThreads, 2) small_rows_kernel(const __grid_constant__ LossArgs a) {
-    constexpr int E = 16 / sizeof(T), K = kSmallVectors;
+constexpr int kSmallRowThreads = 256, kSmallVectors = 16;  // vectors a lane, at most
+
+// writes the gradient of a row that a warp has in registers (q of zeros: zeros)
+template <typename T, bool ENT, int K>
+__device__ __forceinline__ void small_grad(const GradRow& q, const T* x, T* dx, int head, int nv, int edge, float x_edge, const uint4 (&b)[K]) {
+    constexpr int E = 16 / sizeof(T);
+    __syncwarp();  // (every lane has read what it wants of the row: dx may be x)
+    const bool zero = q.a == 0.f && q.b == 0.f && q.d == 0.f;
+    const bool vec = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
+    const int t = zero ? -1 : q.token - head;  // the token's place among the vectors
+    if (edge >= 0) store_one(dx + edge, zero ? 0.f : grad_of<ENT>(q, x_edge) + (edge == q.token ? q.d : 0.f));
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int i = k * 32 + lane_id();
+        if (i >= nv) continue;
+        float e[E];
+        if (zero) {
+#pragma unroll
+            for (int j = 0; j < E; ++j) e[j] = 0.f;
+        } else {
+            unpack<T>(b[k], e);
+            if (!q.far) grad_many<ENT, sizeof(T) == 4, E>(q, e);
+            else
+#pragma unroll
+                for (int j = 0; j < E; ++j) e[j] = grad_of<ENT>(q, e[j]);
+            if (t >= 0 && t / E == i)
+#pragma unroll
+                for (int j = 0; j < E; ++j) e[j] += t % E == j ? q.d : 0.f;
+        }
+        if (vec) {
+            __stcs(reinterpret_cast<uint4*>(dx + head) + i, pack<T>(e));
+        } else {
+#pragma unroll
+            for (int j = 0; j < E; ++j) store_one(dx + head + int64_t(i) * E + j, e[j]);
+        }
+    }
+}
+// the row's scalars from given statistics
+__device__ __forceinline__ GradRow grad_row_of(const LossArgs& a, int row, int token, float g, float h, bool ent) {
+    const float inv_t = a.inv_t_rows ? a.inv_t_rows[row] : a.inv_t;
+    const float m = a.stats[2 * int64_t(row)], sum = a.stats[2 * int64_t(row) + 1];
+    const Scale c = scale_of(inv_t);
+    const bool far = !(m >= -c.most && m <= c.most);
+    const double y = far ? 0.0 : shift_of(m, ref_of(m, c), inv_t);
+    return grad_row(m, far, shifted(sum, -y), float(ln_of(sum) - y), c, inv_t, token, g, h, ent ? a.entropy[row] : 0.f);
+}
+
+template <typename T, int EPI, bool ENT, bool GRAD, int K>
+__global__ void __launch_bounds__(kSmallRowThreads, K > 8 ? 2 : 3) small_rows_kernel(const __grid_constant__ LossArgs a) {
+    constexpr int E = 16 / sizeof(T);
     const int lane = lane_id();
     if (EPI == EPI_POLICY) grid_dependency_wait();  // row_scale_kernel's results
     const int warps = int(gridDim.x) * (kSmallRowThreads / 32);
+    double total = 0.0;  // policy loss: this warp's share (its rows are always the same, in the same order)
+    int64_t row64 = int64_t(blockIdx.x) * (kSmallRowThreads / 32) + (threadIdx.x >> 5);
+    uint32_t words = row64 < a.rows ? row_word<EPI>(a, int(row64), true) : 0u;
 #pragma unroll 1
-    for (int64_t row64 = int64_t(blockIdx.x) * (kSmallRowThreads / 32) + (threadIdx.x >> 5); row64 < a.rows; row64 += warps) {
+    for (; row64 < a.rows; row64 += warps) {
         const int row = int(row64);
-        const RowOf w = row_of<EPI>(a, row, true);
+        const RowOf w = row_from(a, row, words);
+        if (row64 + warps < a.rows) words = row_word<EPI>(a, int(row64 + warps), true);  // (here by the time it is wanted)
         const T* x = static_cast<const T*>(a.x) + row64 * a.ld;
         T* const dx = GRAD ? static_cast<T*>(a.dx) + row64 * a.ld_dx : nullptr;
         const int head = head_of(x, a.n), nv = (a.n - head) / E, beside = a.n - nv * E;
@@ -913,45 +974,27 @@ __global__ void __launch_bounds__(kSmallRowThreads, 2) small_rows_kernel(const _
                 s.s = warp_sum_f(t.s), s.q = warp_sum_f(t.q);
             }
             const RowDone d = row_done<EPI, ENT>(a, w, x_token, s.m, s.e, s.s, s.q, far);
-            if (lane == 0) write_row<EPI, ENT>(a, row, w, d);
+            if (lane == 0) write_row<EPI, ENT, EPI != EPI_POLICY>(a, row, w, d);
+            if (EPI == EPI_POLICY) total += double(w.scale) * double(d.p.loss);
             if (GRAD && !(d.g == 0.f && d.h == 0.f)) q = grad_row(d.m, far, d.s, d.ln_s, c, w.inv_t, w.token, d.g, d.h, d.entropy);
         } else if (lane == 0) {
-            write_row<EPI, ENT>(a, row, w, RowDone{});
+            write_row<EPI, ENT, EPI != EPI_POLICY>(a, row, w, RowDone{});
         }
         if (GRAD) {
-            __syncwarp();  // (every lane has read what it wants of the row: dx may be x)
-            const bool zero = q.a == 0.f && q.b == 0.f && q.d == 0.f;
-            const bool vec = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
-            const int t = zero ? -1 : q.token - head;  // the token's place among the vectors
-            if (edge >= 0) store_one(dx + edge, zero ? 0.f : grad_of<ENT>(q, x_edge) + (edge == q.token ? q.d : 0.f));
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-                const int i = k * 32 + lane;
-                if (i >= nv) continue;
-                float e[E];
-                if (zero) {
-#pragma unroll
-                    for (int j = 0; j < E; ++j) e[j] = 0.f;
-                } else {
-                    unpack<T>(b[k], e);
-                    if (!q.far) grad_many<ENT, sizeof(T) == 4, E>(q, e);
-                    else
-#pragma unroll
-                        for (int j = 0; j < E; ++j) e[j] = grad_of<ENT>(q, e[j]);
-                    if (t >= 0 && t / E == i)
-#pragma unroll
-                        for (int j = 0; j < E; ++j) e[j] += t % E == j ? q.d : 0.f;
-                }
-                if (vec) {
-                    __stcs(reinterpret_cast<uint4*>(dx + head) + i, pack<T>(e));
-                } else {
-#pragma unroll
-                    for (int j = 0; j < E; ++j) store_one(dx + head + int64_t(i) * E + j, e[j]);
-                }
-            }
+            small_grad<T, ENT, K>(q, x, dx, head, nv, edge, x_edge, b);
         }
     }
-    if (EPI == EPI_POLICY) last_sum(a.ticket, gridDim.x, a.row_term, a.rows, 1.0, a.loss);
+    if (EPI == EPI_POLICY) {
+        __shared__ double s_total[kSmallRowThreads / 32];
+        if (lane == 0) s_total[threadIdx.x >> 5] = total;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            double t = 0.0;
+            for (int i = 0; i < kSmallRowThreads / 32; ++i) t += s_total[i];
+            a.row_term[blockIdx.x] = t;  // (a term per CTA: there are fewer of them than rows)
+        }
+        last_sum(a.ticket, gridDim.x, a.row_term, int(gridDim.x), 1.0, a.loss);
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -988,14 +1031,7 @@ __global__ void __launch_bounds__(kGradThreads, 6) grad_kernel(const __grid_cons
 #pragma unroll
         for (int k = 0; k < 4; ++k) b[k] = v[i + k * NT];
     }
-    if (tid == 0) {
-        const float inv_t = a.inv_t_rows ? a.inv_t_rows[row] : a.inv_t;
-        const float m = a.stats[2 * int64_t(row)], sum = a.stats[2 * int64_t(row) + 1];
-        const Scale c = scale_of(inv_t);
-        const bool far = !(m >= -c.most && m <= c.most);
-        const double y = far ? 0.0 : shift_of(m, ref_of(m, c), inv_t);
-        s_q = grad_row(m, far, shifted(sum, -y), float(ln_of(sum) - y), c, inv_t, token, g, h, ENT ? a.entropy[row] : 0.f);
-    }
+    if (tid == 0) s_q = grad_row_of(a, row, token, g, h, ENT);
     // the token's own logit, before anything is written (dx may be x)
     const int64_t t64 = int64_t(token) - j0;
     const int at = t64 >= 0 && t64 < n ? int(t64) : -1, t_vec = at - head;
@@ -1033,6 +1069,34 @@ __global__ void __launch_bounds__(kGradThreads, 6) grad_kernel(const __grid_cons
     }
 }
 
+// Short rows (see small_rows_kernel): a warp each.  60000 rows of 2000 bf16 logits: grad_kernel 186 us, this one 88.
+template <typename T, bool ENT, int K>
+__global__ void __launch_bounds__(kSmallRowThreads, K > 8 ? 2 : 3) small_grad_kernel(const __grid_constant__ LossArgs a) {
+    constexpr int E = 16 / sizeof(T);
+    const int lane = lane_id();
+    const int64_t warps = int64_t(gridDim.x) * (kSmallRowThreads / 32);
+#pragma unroll 1
+    for (int64_t row64 = int64_t(blockIdx.x) * (kSmallRowThreads / 32) + (threadIdx.x >> 5); row64 < a.rows; row64 += warps) {
+        const int row = int(row64), token = a.token[row];
+        const float g = a.g_logp[row], h = ENT ? a.g_entropy[row] : 0.f;
+        const T* x = static_cast<const T*>(a.x) + row64 * a.ld;
+        const int head = head_of(x, a.n), nv = (a.n - head) / E, beside = a.n - nv * E;
+        const uint4* v = reinterpret_cast<const uint4*>(x + head);
+        const int edge = lane < beside ? (lane < head ? lane : lane + nv * E) : -1;
+        uint4 b[K];
+        float x_edge = 0.f;
+        GradRow q{};
+        if (unsigned(token) < unsigned(a.n) && !(g == 0.f && h == 0.f)) {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                if (k * 32 < nv) b[k] = k * 32 + lane < nv ? v[k * 32 + lane] : make_uint4(0, 0, 0, 0);
+            if (edge >= 0) x_edge = load_one(x + edge);
+            q = grad_row_of(a, row, token, g, h, ENT);
+        }
+        small_grad<T, ENT, K>(q, x, static_cast<T*>(a.dx) + row64 * a.ld_dx, head, nv, edge, x_edge, b);
+    }
+}
+
 // ---------------------------------------------------------------------------------------------------------------
 // weights, pairs, sums: small kernels
 // ---------------------------------------------------------------------------------------------------------------
@@ -1040,10 +1104,9 @@ __global__ void __launch_bounds__(kGradThreads, 6) grad_kernel(const __grid_cons
 constexpr int kSmallThreads = 1024;
 
 __device__ __forceinline__ float live_weight(const LossArgs& a, int row) {
-    if (unsigned(a.token[row]) >= unsigned(a.n)) return 0.f;
-    if (!a.weight) return 1.f;
-    const float w = a.weight[row];
-    return w > 0.f ? w : 0.f;
+    const int token = a.token[row];
+    const float w = a.weight ? a.weight[row] : 1.f;  // (both loads before the first is looked at)
+    return unsigned(token) < unsigned(a.n) && w > 0.f ? w : 0.f;
 }
 // the rows of sequence s, inside the batch whatever seq_start says
 __device__ __forceinline__ int2 rows_of(const LossArgs& a, int s) {
@@ -1058,10 +1121,12 @@ __device__ void row_scales(const LossArgs& a, int mean, double* sh) {
         double k = 1.0;
         if (mean == WHIRL_MEAN_TOKENS) {
             double t = 0.0;
+#pragma unroll 8
             for (int r = tid; r < a.rows; r += kSmallThreads) t += live_weight(a, r);
             t = block_sum(t, sh);
             k = t > 0.0 ? 1.0 / t : 0.0;
         }
+#pragma unroll 8
         for (int r = tid; r < a.rows; r += kSmallThreads) a.row_scale[r] = float(k * live_weight(a, r));
         return;
     }
@@ -1197,7 +1262,8 @@ cudaError_t small_typed(const LossArgs& a, cudaStream_t st) {
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at, cfg.numAttrs = EPI == EPI_POLICY ? 1 : 0;  // (the policy loss follows row_scale_kernel)
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, small_rows_kernel<T, EPI, ENT, GRAD>, a);
+    const bool half = vectors_of(a.n, sizeof(T) == 4 ? WHIRL_F32 : WHIRL_BF16) <= 32 * 8;  // rows of up to 4 KB: half the registers, half as many warps more
+    const cudaError_t e = half ? cudaLaunchKernelEx(&cfg, small_rows_kernel<T, EPI, ENT, GRAD, 8>, a) : cudaLaunchKernelEx(&cfg, small_rows_kernel<T, EPI, ENT, GRAD, 16>, a);
     count_launch(LAUNCH_LOSS);
     return e;
 }
@@ -1235,7 +1301,21 @@ cudaError_t fused_typed(const LossArgs& a, int ctas, int per, cudaStream_t st) {
 
 cudaError_t logprobs_launch(const LossArgs& a, int dtype, cudaStream_t st) { return forward_launch<EPI_NONE>(a, dtype, a.entropy != nullptr, st); }
 
+template <typename T, bool ENT>
+static cudaError_t small_grad_typed(const LossArgs& a, cudaStream_t st) {
+    const dim3 grid(unsigned(std::min<int64_t>((int64_t(a.rows) + kSmallRowThreads / 32 - 1) / (kSmallRowThreads / 32), 148 * 8)));
+    const bool half = vectors_of(a.n, sizeof(T) == 4 ? WHIRL_F32 : WHIRL_BF16) <= 32 * 8;
+    if (half) small_grad_kernel<T, ENT, 8><<<grid, kSmallRowThreads, 0, st>>>(a);
+    else small_grad_kernel<T, ENT, 16><<<grid, kSmallRowThreads, 0, st>>>(a);
+    count_launch(LAUNCH_LOSS);
+    return cudaGetLastError();
+}
+
 cudaError_t logprobs_grad_launch(const LossArgs& a, int dtype, cudaStream_t st) {
+    if (is_small(a.n, dtype)) {
+        if (dtype == WHIRL_F32) return a.g_entropy ? small_grad_typed<float, true>(a, st) : small_grad_typed<float, false>(a, st);
+        return a.g_entropy ? small_grad_typed<uint16_t, true>(a, st) : small_grad_typed<uint16_t, false>(a, st);
+    }
     // (a chunk per CTA; at most 65535 of them per row)
     const int chunk = int(std::max<int64_t>(16384, (int64_t(a.n) + 65534) / 65535));
     const dim3 grid(unsigned(a.rows), unsigned((int64_t(a.n) + chunk - 1) / chunk)), block(kGradThreads);
