@@ -451,3 +451,28 @@ def test_streams_threads_and_graphs():
     torch.cuda.synchronize()
     for k in range(2):
         assert all(torch.equal(a, b) for a, b in zip(outs[k], want[1 - k]))
+
+
+@pytest.mark.parametrize("rows,n,pad,dtype", [(2500, 4103, 1, "bf16"), (2500, 2049, 0, "f32"), (2400, 8200, 0, "f32"), (2400, 16385, 7, "bf16")])
+def test_many_rows_of_middle_length(rows, n, pad, dtype):
+    """Rows that a warp streams through its registers; some do not count."""
+    from whirl_llm_b200 import api
+    x, x64, token, it, stats, adv, old, rf, weight = policy_inputs(rows, n, dtype, seed=77, pad=pad, inv_t=0.8)
+    token[5], token[100] = -1, n
+    r = api.token_logprobs(x, token.cuda(), inv_t=0.8, want_entropy=True)
+    ok = (token >= 0) & (token < n)
+    want = torch.where(ok, stats[2], 0.0)
+    close(r.logp, want, ref.logp_tol(n, want))
+    close(r.entropy, torch.where(ok, stats[3], 0.0), ref.entropy_tol(n))
+    g = torch.randn(rows, generator=torch.Generator().manual_seed(3))
+    g[7] = 0.0
+    dx = api.token_logprobs_grad(x, token.cuda(), r.stats, g.cuda(), inv_t=0.8)
+    d, p, lp = ref.dlogits(x64, token, it, (stats[0], stats[1]), g.double())
+    close(dx, d, ref.dx_tol(p, lp, g.double(), it, DT[dtype], d, n=n), "dx")
+    assert (dx[[5, 7, 100]] == 0).all()
+    out = torch.empty((rows, n), dtype=DT[dtype], device="cuda")
+    assert torch.equal(api.token_logprobs_grad(x, token.cuda(), r.stats, g.cuda(), inv_t=0.8, dx=out), dx)
+    f = api.policy_loss(x, token.cuda(), adv.cuda(), old.cuda(), rf.cuda(), weight.cuda(), inv_t=0.8, kl_coef=0.1, want_grad=False)
+    check_policy(f, x64, token, it, stats, adv, old, rf, weight, 1, None, dtype, n, kl_coef=0.1)
+    f = api.policy_loss(x, token.cuda(), adv.cuda(), old.cuda(), rf.cuda(), weight.cuda(), inv_t=0.8, kl_coef=0.1)
+    check_policy(f, x64, token, it, stats, adv, old, rf, weight, 1, None, dtype, n, kl_coef=0.1)

@@ -312,12 +312,12 @@ __device__ __forceinline__ GradRow grad_row(float m, bool far, float s, float ln
     q.d = inv_t * g;
     return q;
 }
-template <bool ENT>
+// LOW: with the scale's second float (a result of 8 bits does not show it)
+template <bool ENT, bool LOW>
 __device__ __forceinline__ float grad_of(const GradRow& q, float x) {
-    const float t = q.far ? (x - q.e) * q.c : fmaf(x, q.c_lo, fmaf(x, q.c, -q.e)), w = ex2_approx(t);
+    const float t0 = fmaf(x, q.c, -q.e), t = q.far ? (x - q.e) * q.c : (LOW ? fmaf(x, q.c_lo, t0) : t0), w = ex2_approx(t);
     return ENT ? w * fmaf(q.b, fmaxf(t, -1000.f), q.a) : w * q.a;
 }
-// LOW: with the scale's second float (a result of 8 bits does not show it)
 template <bool ENT, bool LOW, int N>
 __device__ __forceinline__ void grad_many(const GradRow& q, float (&x)[N]) {  // (not for a far row)
     const F2 ne = f2(-q.e, -q.e), c = f2(q.c, q.c), lo = f2(q.c_lo, q.c_lo), a = f2(q.a, q.a), b = f2(q.b, q.b);
@@ -825,7 +825,7 @@ __global__ void __launch_bounds__(kFusedThreads, kFusedCtas) fused_kernel(const 
         GradRow q{};
         if (!zero) q = s_q;
         T* dx = static_cast<T*>(a.dx) + int64_t(row) * a.ld_dx;
-        if (at.edge >= 0) store_one(dx + at.edge, zero ? 0.f : grad_of<ENT>(q, x_edge) + (at.edge == q.token ? q.d : 0.f));
+        if (at.edge >= 0) store_one(dx + at.edge, zero ? 0.f : grad_of<ENT, sizeof(T) == 4>(q, x_edge) + (at.edge == q.token ? q.d : 0.f));
         const bool vec = ((reinterpret_cast<uintptr_t>(at.x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
         T* body = dx + at.head + int64_t(at.v0) * E;
         uint4* out = reinterpret_cast<uint4*>(body);
@@ -857,11 +857,11 @@ __global__ void __launch_bounds__(kFusedThreads, kFusedCtas) fused_kernel(const 
             for (; i < cnt; i += NT) {
 #pragma unroll 1
                 for (int j = 0; j < E; ++j)
-                    store_one(body + int64_t(i) * E + j, zero ? 0.f : grad_of<ENT>(q, load_one(reinterpret_cast<const T*>(slice + i) + j)));
+                    store_one(body + int64_t(i) * E + j, zero ? 0.f : grad_of<ENT, sizeof(T) == 4>(q, load_one(reinterpret_cast<const T*>(slice + i) + j)));
             }
             i = tid;
         }
-        if (mine) store_one(body + t, grad_of<ENT>(q, x_mine) + q.d);
+        if (mine) store_one(body + t, grad_of<ENT, sizeof(T) == 4>(q, x_mine) + q.d);
 #pragma unroll 4
         for (; i < refill; i += NT) copy_async16(slice + i, next + i);
         copies_commit();
@@ -880,18 +880,18 @@ __global__ void __launch_bounds__(kFusedThreads, kFusedCtas) fused_kernel(const 
 // 2000 bf16 logits, policy loss with gradient, took 72 us with fused_kernel and take 50 here.
 constexpr int kSmallRowThreads = 256, kSmallVectors = 16;  // vectors a lane, at most
 
-// writes the gradient of a row that a warp has in registers (q of zeros: zeros)
+// writes the gradient of a row's vectors from `first` on that a warp has in registers (q of zeros: zeros)
 template <typename T, bool ENT, int K>
-__device__ __forceinline__ void small_grad(const GradRow& q, const T* x, T* dx, int head, int nv, int edge, float x_edge, const uint4 (&b)[K]) {
+__device__ __forceinline__ void small_grad(const GradRow& q, const T* x, T* dx, int head, int first, int nv, int edge, float x_edge, const uint4 (&b)[K]) {
     constexpr int E = 16 / sizeof(T);
     __syncwarp();  // (every lane has read what it wants of the row: dx may be x)
     const bool zero = q.a == 0.f && q.b == 0.f && q.d == 0.f;
     const bool vec = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
     const int t = zero ? -1 : q.token - head;  // the token's place among the vectors
-    if (edge >= 0) store_one(dx + edge, zero ? 0.f : grad_of<ENT>(q, x_edge) + (edge == q.token ? q.d : 0.f));
+    if (edge >= 0) store_one(dx + edge, zero ? 0.f : grad_of<ENT, sizeof(T) == 4>(q, x_edge) + (edge == q.token ? q.d : 0.f));
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const int i = k * 32 + lane_id();
+        const int i = first + k * 32 + lane_id();
         if (i >= nv) continue;
         float e[E];
         if (zero) {
@@ -902,7 +902,7 @@ __device__ __forceinline__ void small_grad(const GradRow& q, const T* x, T* dx, 
             if (!q.far) grad_many<ENT, sizeof(T) == 4, E>(q, e);
             else
 #pragma unroll
-                for (int j = 0; j < E; ++j) e[j] = grad_of<ENT>(q, e[j]);
+                for (int j = 0; j < E; ++j) e[j] = grad_of<ENT, sizeof(T) == 4>(q, e[j]);
             if (t >= 0 && t / E == i)
 #pragma unroll
                 for (int j = 0; j < E; ++j) e[j] += t % E == j ? q.d : 0.f;
@@ -948,9 +948,12 @@ __global__ void __launch_bounds__(kSmallRowThreads, K > 8 ? 2 : 3) small_rows_ke
         float x_edge = 0.f;
         GradRow q{};
         if (w.live) {
+auto load = [&](int first) {
 #pragma unroll
-            for (int k = 0; k < K; ++k)
-                if (k * 32 < nv) b[k] = k * 32 + lane < nv ? v[k * 32 + lane] : make_uint4(0, 0, 0, 0);
+                for (int k = 0; k < K; ++k)
+                    if (first + k * 32 < nv) b[k] = first + k * 32 + lane < nv ? v[first + k * 32 + lane] : make_uint4(0, 0, 0, 0);
+            };
+            load(0);
             const float x_token = load_one(x + w.token);
             const Scale c = scale_of(w.inv_t);
             Soft s = soft_empty(c);
@@ -959,9 +962,15 @@ __global__ void __launch_bounds__(kSmallRowThreads, K > 8 ? 2 : 3) small_rows_ke
                 const float e[1] = {x_edge};
                 add_many<ENT, 1>(s, e, c);
             }
+#pragma unroll 1
+            for (int first = 0;;) {
 #pragma unroll
-            for (int k = 0; k < K; ++k)
-                if (k * 32 + lane < nv) add_vec<T, ENT>(s, b[k], c);
+                for (int k = 0; k < K; ++k)
+                    if (first + k * 32 + lane < nv) add_vec<T, ENT>(s, b[k], c);
+                first += 32 * K;
+                if (GRAD || first >= nv) break;  // (with GRAD the row is in the registers as a whole)
+                load(first);
+            }
             __syncwarp();
             s.s -= s.k, s.k = 0.f;
             const float m = warp_max_f(s.m);
@@ -981,7 +990,7 @@ __global__ void __launch_bounds__(kSmallRowThreads, K > 8 ? 2 : 3) small_rows_ke
             write_row<EPI, ENT, EPI != EPI_POLICY>(a, row, w, RowDone{});
         }
         if (GRAD) {
-            small_grad<T, ENT, K>(q, x, dx, head, nv, edge, x_edge, b);
+            small_grad<T, ENT, K>(q, x, dx, head, 0, nv, edge, x_edge, b);
         }
     }
     if (EPI == EPI_POLICY) {
@@ -1056,16 +1065,16 @@ __global__ void __launch_bounds__(kGradThreads, 6) grad_kernel(const __grid_cons
         }
 #pragma unroll 1
         for (; i < nv; i += NT) __stcs(dv + i, grad_vec<T, ENT>(q, v[i]));
-        if (mine) store_one(dx + at, grad_of<ENT>(q, x_token) + q.d);
+        if (mine) store_one(dx + at, grad_of<ENT, sizeof(T) == 4>(q, x_token) + q.d);
     } else {  // one by one
         for (int k = tid; k < nv * E; k += NT) {
             const int j = head + k;
-            store_one(dx + j, grad_of<ENT>(q, load_one(x + j)) + (j == at ? q.d : 0.f));
+            store_one(dx + j, grad_of<ENT, sizeof(T) == 4>(q, load_one(x + j)) + (j == at ? q.d : 0.f));
         }
     }
     for (int k = tid; k < n - nv * E; k += NT) {
         const int j = k < head ? k : k + nv * E;
-        store_one(dx + j, grad_of<ENT>(q, load_one(x + j)) + (j == at ? q.d : 0.f));
+        store_one(dx + j, grad_of<ENT, sizeof(T) == 4>(q, load_one(x + j)) + (j == at ? q.d : 0.f));
     }
 }
 
@@ -1086,14 +1095,23 @@ __global__ void __launch_bounds__(kSmallRowThreads, K > 8 ? 2 : 3) small_grad_ke
         uint4 b[K];
         float x_edge = 0.f;
         GradRow q{};
-        if (unsigned(token) < unsigned(a.n) && !(g == 0.f && h == 0.f)) {
+        const bool zero = unsigned(token) >= unsigned(a.n) || (g == 0.f && h == 0.f);
+        T* const dx = static_cast<T*>(a.dx) + row64 * a.ld_dx;
+#pragma unroll 1
+        for (int first = 0;;) {
+            if (!zero) {
 #pragma unroll
-            for (int k = 0; k < K; ++k)
-                if (k * 32 < nv) b[k] = k * 32 + lane < nv ? v[k * 32 + lane] : make_uint4(0, 0, 0, 0);
-            if (edge >= 0) x_edge = load_one(x + edge);
-            q = grad_row_of(a, row, token, g, h, ENT);
+                for (int k = 0; k < K; ++k)
+                    if (first + k * 32 < nv) b[k] = first + k * 32 + lane < nv ? v[first + k * 32 + lane] : make_uint4(0, 0, 0, 0);
+                if (first == 0) {
+                    if (edge >= 0) x_edge = load_one(x + edge);
+                    q = grad_row_of(a, row, token, g, h, ENT);
+                }
+            }
+            small_grad<T, ENT, K>(q, x, dx, head, first, nv, first == 0 ? edge : -1, x_edge, b);
+            first += 32 * K;
+            if (first >= nv) break;
         }
-        small_grad<T, ENT, K>(q, x, static_cast<T*>(a.dx) + row64 * a.ld_dx, head, nv, edge, x_edge, b);
     }
 }
 
@@ -1252,7 +1270,11 @@ cudaError_t cluster_launch(void (*f)(LossArgs, P...), std::atomic<uint64_t>& rea
 
 int vectors_of(int n, int dtype) { return int((int64_t(n) * (dtype == WHIRL_F32 ? 4 : 2) + 15) / 16); }
 
+// A warp per row: where it holds the whole row in its registers; or, where a row is read and done with piece by piece, for rows of up to 32 KB
+// (statistics) or 16 KB (gradient) of which there are enough to fill the GPU with warps.  20000 rows of 4200 bf16 logits: statistics by CTAs 120 us, by warps
+// 64; gradient 97 and 75.  3000 rows of 16000: statistics 31 by warps and 33 by CTAs, gradient 48 and 36.
 bool is_small(int n, int dtype) { return vectors_of(n, dtype) <= 32 * kSmallVectors; }
+bool is_short(const LossArgs& a, int dtype, int vectors) { return is_small(a.n, dtype) || (a.rows >= 148 * 16 && vectors_of(a.n, dtype) <= vectors); }
 template <typename T, int EPI, bool ENT, bool GRAD>
 cudaError_t small_typed(const LossArgs& a, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
@@ -1280,7 +1302,7 @@ cudaError_t forward_typed(const LossArgs& a, int ctas, int per, cudaStream_t st)
 }
 template <int EPI>
 cudaError_t forward_launch(const LossArgs& a, int dtype, bool ent, cudaStream_t st) {
-    if (is_small(a.n, dtype)) return small_launch<EPI, false>(a, dtype, ent, st);
+    if (is_short(a, dtype, 2048)) return small_launch<EPI, false>(a, dtype, ent, st);
     const int nv = vectors_of(a.n, dtype);
     // Enough CTAs to fill the GPU three times over, 2 steps of the ring each at least: 1024 rows of 262144 f32 logits take 159 us with two
     // CTAs a row, 164 with one, 182 with four.
@@ -1312,7 +1334,7 @@ static cudaError_t small_grad_typed(const LossArgs& a, cudaStream_t st) {
 }
 
 cudaError_t logprobs_grad_launch(const LossArgs& a, int dtype, cudaStream_t st) {
-    if (is_small(a.n, dtype)) {
+    if (is_short(a, dtype, 1024)) {
         if (dtype == WHIRL_F32) return a.g_entropy ? small_grad_typed<float, true>(a, st) : small_grad_typed<float, false>(a, st);
         return a.g_entropy ? small_grad_typed<uint16_t, true>(a, st) : small_grad_typed<uint16_t, false>(a, st);
     }
