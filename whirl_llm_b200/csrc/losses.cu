@@ -2,9 +2,18 @@
 // logits (formulas: include/whirl_b200.h).
 //
 // Every row needs its softmax statistics before any of its gradient can be written.  The statistics are one online pass: a
-// thread keeps the largest logit it has met, the sum of exp((x - that) * inv_t) and (for the entropy) the sum of the
-// exponentials times their exponents, and brings all three to a new maximum when one comes along; partial results merge the
-// same way.  The gradient is one elementwise pass over the row.
+// thread keeps the largest logit it has met, the sum of exp((x - about that) * inv_t) and (for the entropy) the sum of the
+// exponentials times their exponents, and brings them to a new reference when a larger logit comes along; partial results merge
+// the same way.  The gradient is one elementwise pass over the row.
+//
+//   forward_kernel     statistics of long rows, a cluster of 1 to 16 CTAs each      1024 x 262144 f32: 158 us, 6.8 TB/s
+//   grad_kernel        gradient of long rows from given statistics                  1024 x 262144 bf16: 170 us, 6.3 TB/s
+//   fused_kernel       policy loss: both at once, the row held in shared memory     4096 x 151936 bf16, a third masked: 500 us, 4.1 TB/s
+//   small_rows_kernel, small_grad_kernel   the same for short rows, a warp each     60000 x 2000 bf16: 80, 181 and 88 us
+//
+// All are bound by memory in principle (a logit costs about 7 instructions for the statistics, 5 for the gradient, and one
+// exponential of the special function unit for each).  The preference loss needs its sequences' sums before any gradient: forward_kernel,
+// pairs_kernel, grad_kernel, two reads and one write.
 #include "../../include/whirl_b200.h"
 
 #include <algorithm>
@@ -430,7 +439,8 @@ template <int EPI, bool ENT>
 __device__ __forceinline__ RowDone row_done(const LossArgs& a, const RowOf& w, float x_token, float m, float e, float s, float q, bool far) {
     RowDone r;
     if (!(m >= -FLT_MAX && m <= FLT_MAX)) s = NAN;  // no distribution
-    const double ln_s = ln_of(s);
+    // (ex2.approx truncates: over exponents of -24 .. 0 it was measured low by 5.1e-8 on average, over -1 .. 0 by 2.9e-8; a bias of all log-probabilities)
+    const double ln_s = ln_of(s) + 4.5e-8;
     r.m = m, r.s = s, r.ln_s = float(ln_s), r.shift = far ? 0.0 : shift_of(m, e, w.inv_t);
     r.logp = (double(x_token) - double(m)) * double(w.inv_t) - (ln_s + r.shift);
     r.entropy = ENT ? float(ln_s - kLn2 * double(q / s)) : 0.f;
@@ -709,7 +719,10 @@ __device__ __forceinline__ Soft hear(const Scale& c, const Part* parts, uint64_t
 // busy while the statistics of that row wait for it; several CTAs per SM fill each other's waits (the exchange of the statistics, the row's
 // scalars).  The statistics travel by stores that count on the receiver's mbarrier: a cluster barrier would hold every row until the
 // gradient's stores of the row before it are acknowledged.
-
+// What bounds it is the clusters' lockstep: every row waits for the slowest of its CTAs (1480 x 151936 bf16: DRAM at 55 % of the copy rate, the special
+// function units at 56 %, warps at the barrier a third of their time).  Measured beside it on 4096 x 151936 bf16, a third of the rows masked (501 us with
+// two launches and two reads, 487 to 503 here): one CTA an SM with a ring of slices and a warp of its own for the scalars, 770; tasks of
+// statistics and of gradients drawn from one counter, the second read from L2, 520 to 600; 384 or 512 threads, 534 and 554.
 template <typename T, bool ENT>
 __global__ void __launch_bounds__(kFusedThreads, kFusedCtas) fused_kernel(const __grid_constant__ LossArgs a, int per) {
     constexpr int EPI = EPI_POLICY;
@@ -877,7 +890,7 @@ __global__ void __launch_bounds__(kFusedThreads, kFusedCtas) fused_kernel(const 
 
 // A row of up to 8 KB fits the registers of one warp: it is read once, its statistics need no shared memory and no barrier, and (GRAD) its
 // gradient is written from the registers.  The kernels above spend 4 to 7 us of a CTA on a row however short it is: 8000 rows of
-// 2000 bf16 logits, policy loss with gradient, took 72 us with fused_kernel and take 50 here.
+// 2000 bf16 logits, policy loss with gradient, took 72 us with fused_kernel and take 32 here.
 constexpr int kSmallRowThreads = 256, kSmallVectors = 16;  // vectors a lane, at most
 
 // writes the gradient of a row's vectors from `first` on that a warp has in registers (q of zeros: zeros)
