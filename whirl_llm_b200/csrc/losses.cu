@@ -270,11 +270,10 @@ constexpr double kLn2 = 0.6931471805599453;
 // The row's scalars are one warp's work per row, in the time that the others need for a slice: single-precision functions of the hardware
 // with one correction each, and 64 bits where a last bit would add up over a sequence.  (The library's log, exp and expm1 in 64
 // bits, and the divisions around them, took 2.7 us a row.)
-// log of a sum s > 0 (NaN without one): s = 2^k f with f in [sqrt 1/2, sqrt 2), log f = 2 atanh z, z = (f - 1) / (f + 1), |z| < 0.172; the
+// log of a sum > 0 (NaN without one): 2^k f with f in [sqrt 1/2, sqrt 2), log f = 2 atanh z, z = (f - 1) / (f + 1), |z| < 0.172; the
 // terms left out are below 1e-13.  (lg2.approx and a step of Newton's method with ex2.approx is low by 4e-8.)
-__device__ __forceinline__ double ln_of(float s) {
-    if (!(s > 0.f && s <= FLT_MAX)) return NAN;
-    const double d = double(s);
+__device__ __forceinline__ double ln_of(double d) {
+    if (!(d > 1e-300 && d < 1e300)) return NAN;
     const int hi = __double2hiint(d), k = (hi - 0x3fe6a09e) >> 20;
     const double f = __hiloint2double(hi - (k << 20), __double2loint(d)), b = f + 1.0;
     double r = double(__frcp_rn(float(b)));
@@ -303,6 +302,17 @@ __device__ __forceinline__ float kl_of(float k) {
 // to the last bits of e.
 __device__ __forceinline__ double shift_of(float m, float e, float inv_t) { return kLn2 * (double(e) - double(m) * (double(inv_t) * 1.4426950408889634)); }
 __device__ __forceinline__ float shifted(float s, double y) { return s * exp_of(float(y)); }  // s e^y
+// A row's sum s, relative to its reference e, less the errors of ex2.approx that show.  That of the maximum's own term is taken out exactly (it is all that
+// stands between a near-certain token's log-probability and 0); the others are low by 5e-8 on average (measured, exponents of -24 .. 0).
+__device__ __forceinline__ double mended(float s, float m, float e, const Scale& c, double shift) {
+    const double y = -shift;  // ln 2 (m c - e), within ln 2 / 2 unless m c has no fraction
+    if (!(fabs(y) < 0.36)) return double(s);
+    double t = 1.0 / 3628800.0;
+    t = fma(t, y, 1.0 / 362880.0), t = fma(t, y, 1.0 / 40320.0), t = fma(t, y, 1.0 / 5040.0), t = fma(t, y, 1.0 / 720.0), t = fma(t, y, 1.0 / 120.0);
+    t = fma(t, y, 1.0 / 24.0), t = fma(t, y, 1.0 / 6.0), t = fma(t, y, 0.5), t = fma(t, y, 1.0), t = fma(t, y, 1.0);
+    const double top = double(ex2_approx(fmaf(m, c.lo, fmaf(m, c.hi, -e))));  // as it went into the sum
+    return t + (double(s) - top) * (1.0 + 5e-8);
+}
 
 // The row's gradient: dx_j = w_j * (a + b * t_j), + d on the token, with t_j = x_j c - e (far: (x_j - e) c) and w_j = 2^t_j, whose sum
 // over the row is s:
@@ -436,14 +446,15 @@ struct RowDone {
     PolicyRow p;
 };
 template <int EPI, bool ENT>
-__device__ __forceinline__ RowDone row_done(const LossArgs& a, const RowOf& w, float x_token, float m, float e, float s, float q, bool far) {
+__device__ __forceinline__ RowDone row_done(const LossArgs& a, const RowOf& w, const Scale& c, float x_token, float m, float e, float s, float q, bool far) {
     RowDone r;
     if (!(m >= -FLT_MAX && m <= FLT_MAX)) s = NAN;  // no distribution
-    // (ex2.approx truncates: over exponents of -24 .. 0 it was measured low by 5.1e-8 on average, over -1 .. 0 by 2.9e-8; a bias of all log-probabilities)
-    const double ln_s = ln_of(s) + 4.5e-8;
-    r.m = m, r.s = s, r.ln_s = float(ln_s), r.shift = far ? 0.0 : shift_of(m, e, w.inv_t);
+    r.shift = far ? 0.0 : shift_of(m, e, w.inv_t);
+    const double sum = far ? double(s) : mended(s, m, e, c, r.shift), ln_s = ln_of(sum);
+    r.m = m, r.s = float(sum), r.ln_s = float(ln_s);
     r.logp = (double(x_token) - double(m)) * double(w.inv_t) - (ln_s + r.shift);
-    r.entropy = ENT ? float(ln_s - kLn2 * double(q / s)) : 0.f;
+    if (r.logp > 0.0) r.logp = 0.0;  // (by the last bits of the sum)
+    r.entropy = ENT ? float(ln_s - kLn2 * double(q / s)) : 0.f;  // (the terms' mean exponent is q / s)
     if (EPI == EPI_POLICY) r.p = policy_row(a, w, r.logp, r.entropy), r.g = w.scale * r.p.dlogp, r.h = -a.ent_coef * w.scale;
     return r;
 }
@@ -652,7 +663,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) forward_kernel(const __grid_co
         if (tid == 0 && rank == 0) {
             grid_dependency_wait();  // row_scale_kernel's results
             if (EPI == EPI_POLICY) w.scale = a.row_scale[row];
-            write_row<EPI, ENT>(a, row, w, row_done<EPI, ENT>(a, w, x_token, s.m, s.e, s.s, s.q, far));
+            write_row<EPI, ENT>(a, row, w, row_done<EPI, ENT>(a, w, c, x_token, s.m, s.e, s.s, s.q, far));
         }
     } else if (tid == 0 && rank == 0) {
         grid_dependency_wait();
@@ -796,7 +807,7 @@ __global__ void __launch_bounds__(kFusedThreads, kFusedCtas) fused_kernel(const 
                     grid_dependency_wait();  // row_scale_kernel's results
                     wr.scale = a.row_scale[row];
                 }
-                const RowDone d = row_done<EPI, ENT>(a, wr, x_token, r.m, r.e, r.s, r.q, far);
+                const RowDone d = row_done<EPI, ENT>(a, wr, c, x_token, r.m, r.e, r.s, r.q, far);
                 s_zero = d.g == 0.f && d.h == 0.f;
                 s_q = grad_row(d.m, far, d.s, d.ln_s, c, wr.inv_t, wr.token, d.g, d.h, d.entropy);
                 if (rank == 0) write_row<EPI, ENT>(a, row, wr, d);
@@ -935,7 +946,7 @@ __device__ __forceinline__ GradRow grad_row_of(const LossArgs& a, int row, int t
     const Scale c = scale_of(inv_t);
     const bool far = !(m >= -c.most && m <= c.most);
     const double y = far ? 0.0 : shift_of(m, ref_of(m, c), inv_t);
-    return grad_row(m, far, shifted(sum, -y), float(ln_of(sum) - y), c, inv_t, token, g, h, ent ? a.entropy[row] : 0.f);
+    return grad_row(m, far, shifted(sum, -y), float(ln_of(double(sum)) - y), c, inv_t, token, g, h, ent ? a.entropy[row] : 0.f);
 }
 
 template <typename T, int EPI, bool ENT, bool GRAD, int K>
@@ -995,7 +1006,7 @@ auto load = [&](int first) {
                 Soft t = far_sums<T, ENT, 32>(v, nv, edge >= 0, x_edge, m, c.hi);
                 s.s = warp_sum_f(t.s), s.q = warp_sum_f(t.q);
             }
-            const RowDone d = row_done<EPI, ENT>(a, w, x_token, s.m, s.e, s.s, s.q, far);
+            const RowDone d = row_done<EPI, ENT>(a, w, c, x_token, s.m, s.e, s.s, s.q, far);
             if (lane == 0) write_row<EPI, ENT, EPI != EPI_POLICY>(a, row, w, d);
             if (EPI == EPI_POLICY) total += double(w.scale) * double(d.p.loss);
             if (GRAD && !(d.g == 0.f && d.h == 0.f)) q = grad_row(d.m, far, d.s, d.ln_s, c, w.inv_t, w.token, d.g, d.h, d.entropy);
