@@ -476,3 +476,73 @@ def test_many_rows_of_middle_length(rows, n, pad, dtype):
     check_policy(f, x64, token, it, stats, adv, old, rf, weight, 1, None, dtype, n, kl_coef=0.1)
     f = api.policy_loss(x, token.cuda(), adv.cuda(), old.cuda(), rf.cuda(), weight.cuda(), inv_t=0.8, kl_coef=0.1)
     check_policy(f, x64, token, it, stats, adv, old, rf, weight, 1, None, dtype, n, kl_coef=0.1)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,n", [(40, 1003), (24, 33001), (70, 50000), (9, 151936)])
+def test_losses_in_place_and_temperatures_per_row(rows, n, dtype):
+    """dx = x, and inv_t per row, give the same bits as a dx of its own and the one inv_t."""
+    from whirl_llm_b200 import api
+    x, _, token, it, _, adv, old, rf, weight = policy_inputs(rows, n, dtype, seed=61, inv_t=0.8)
+    x = x.contiguous()
+    cuda = [v.cuda() for v in (token, adv, old, rf, weight)]
+    starts = torch.tensor([0, rows // 3, rows // 2, rows // 2, rows - 1], dtype=torch.int32, device="cuda")
+    per_row = torch.full((rows,), 0.8, device="cuda")
+
+    def both(y, dx, **t):
+        tok, a, o, r, w = cuda
+        return (lambda d: api.policy_loss(y, tok, a, o, r, w, kl_coef=0.1, ent_coef=0.02, dx=d, **t),
+                lambda d: api.preference_loss(y, tok, starts, r, w, dx=d, **t))
+    for k in range(2):
+        want = both(x, None, inv_t=0.8)[k](None)
+        y = x.clone()
+        got = both(y, y, inv_t=0.8)[k](y)
+        assert got.dx is y and torch.equal(got.dx, want.dx) and torch.equal(got.loss, want.loss) and torch.equal(got.logp, want.logp)
+        got = both(x, None, inv_t_rows=per_row)[k](None)
+        assert torch.equal(got.dx, want.dx) and torch.equal(got.loss, want.loss) and torch.equal(got.stats, want.stats)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [1003, 20001, 60000])
+def test_policy_rows_of_every_kind(n, dtype):
+    """Rows of the type's lowest value, rows without a distribution, huge logits and a single token left, through the policy loss."""
+    from whirl_llm_b200 import api
+    rows = 8
+    x, _, token = make(rows, n, dtype, seed=71)
+    x = x.clone().contiguous()
+    low, high = torch.finfo(DT[dtype]).min, torch.finfo(DT[dtype]).max
+    x[0] = low
+    x[1] = -math.inf
+    x[2, 5] = math.nan
+    x[3] = -math.inf
+    x[3, token[3].item()] = 1.0
+    x[4, 17] = high
+    x[5, : n // 2] = low
+    x[6] = high
+    x64, it = x.double().cpu(), ones(1.25, rows)
+    m, s, lp, h = ref.row_stats(x64, it)
+    want = lp.gather(1, token.long()[:, None])[:, 0].float().double()  # (as float32: -4e38 is -inf there)
+    for place in (False, True):
+        y = x.clone()
+        r = api.policy_loss(y, token.cuda(), torch.ones(rows, device="cuda"), inv_t=1.25, mean=0, want_entropy=True, dx=y if place else None)
+        close(r.logp, want, ref.logp_tol(n, want.clamp_min(-1e30)), "logp")
+        close(r.entropy, h, ref.entropy_tol(n), "entropy")
+        assert torch.isnan(r.loss)
+        g = torch.full((rows,), -1.0, dtype=torch.float64)
+        d, p, lpd = ref.dlogits(x64, token, it, (m, s), g)
+        good = torch.tensor([0, 3, 4, 5, 6, 7])
+        close(r.dx[good.cuda()], d[good], ref.dx_tol(p[good], lpd[good].clamp_min(-1e30), g[good], it[good], DT[dtype], d[good], n=n), "dx")
+        assert torch.isnan(r.dx[1:3]).all()
+        q = api.token_logprobs(x, token.cuda(), inv_t=1.25)
+        close(q.logp, want, ref.logp_tol(n, want.clamp_min(-1e30)), "logp alone")
+        dx = api.token_logprobs_grad(x, token.cuda(), q.stats, g.float().cuda(), inv_t=1.25)
+        close(dx[good.cuda()], d[good], ref.dx_tol(p[good], lpd[good].clamp_min(-1e30), g[good], it[good], DT[dtype], d[good], n=n), "dx alone")
+
+
+def test_rows_longer_than_a_cluster_holds():
+    from whirl_llm_b200 import api
+    rows, n = 3, 1000003
+    x, x64, token, it, stats, adv, old, rf, weight = policy_inputs(rows, n, "f32", seed=81, masked=0.0)
+    weight[1] = 0.0
+    r = api.policy_loss(x, token.cuda(), adv.cuda(), old.cuda(), rf.cuda(), weight.cuda(), kl_coef=0.1, ent_coef=0.01)
+    check_policy(r, x64, token, it, stats, adv, old, rf, weight, 1, None, "f32", n, kl_coef=0.1, ent_coef=0.01)

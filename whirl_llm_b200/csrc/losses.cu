@@ -425,7 +425,7 @@ __device__ __forceinline__ PolicyRow policy_row(const LossArgs& a, const RowOf& 
     float pg = takes_plain ? -plain : -clipped;
     p.dlogp = takes_plain && free_d ? -plain : 0.f;
     if (a.dual_clip > 0.f && adv < 0.f && pg > -a.dual_clip * adv) pg = -a.dual_clip * adv, p.dlogp = 0.f;
-    if (logp != logp) p.dlogp = float(logp);
+    if (logp != logp) pg = p.dlogp = float(logp);  // (a ratio of 1 does not see it)
     p.kl = 0.f;
     if (a.ref_logp) {
         float k = float(double(w.ref_logp) - logp);
