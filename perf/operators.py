@@ -348,10 +348,10 @@ def _policy_rows(logp, old, ref, adv, entropy, c):
 def _plain_policy(st):
     c, x = st["case"], st["x"]
     _, d, w, s = _softmax(x, st["inv_t"])
-    scale = _row_scale(st["weight"], st["seq_start"], c["mean"], c["rows"])
-    live = scale > 0
+    live = st["weight"] > 0
     logp = _at(d, st["token"]).double() - s.double().log()
     entropy = _entropy(d, w, s) if c["ent"] else None
+    scale = _row_scale(st["weight"], st["seq_start"], c["mean"], c["rows"])
     row, kl, dlogp = _policy_rows(logp, st["old_logp"], st["ref_logp"], st["adv"], None if entropy is None else entropy.double(), c)
     g = torch.where(live, scale * dlogp, 0.0).float()
     h = (-c["ent"] * scale).float() if c["ent"] else None
@@ -474,7 +474,7 @@ def exact(case, seed):
             row = row + case["kl"] * kl
         if case["ent"]:
             row = row - case["ent"] * entropy
-        live = (scale > 0).double()
+        live = (w > 0).double()
         (scale * live * row).sum().backward()
         row = row.detach() * live
         dx = _exact_dx(x, token, m, s, at.grad, -case["ent"] * scale if case["ent"] else None, entropy, inv_t)
