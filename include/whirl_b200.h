@@ -335,8 +335,8 @@ int whirl_spec_accept_residual(const void* target, const void* draft, int dtype,
  *     p_j = exp((x_j - max) * inv_t) / sum,  logp = log p[token],  H = - sum_j p_j log p_j   (an entry of p = 0 adds nothing)
  * Entries may be -inf or the type's lowest value (forbidden tokens: p = 0, gradient 0).  A row that holds a NaN or +inf, or
  * -inf alone, has no distribution: its outputs and its gradient are NaN.
- * A row COUNTS when its token lies in [0, n), its weight (where the call has weights) is > 0 and, where sequences matter, it
- * lies inside one.  Rows that do not count are not read: their outputs and statistics are 0, and so is their row of dx.
+ * A row COUNTS when its token lies in [0, n), its weight (where the call has weights) is > 0 and, in the preference loss, it
+ * lies inside a sequence.  Rows that do not count are not read: their outputs and statistics are 0, and so is their row of dx.
  * dx has the type of x, rows ld_dx apart; it may be x itself (with the same ld), and must not overlap x in another way.
  * Sums run in a fixed order: the same call gives the same bits.
  * ---------------------------------------------------------------------------------------------------------------- */
@@ -358,7 +358,8 @@ int whirl_token_logprobs_grad(const void* x, int dtype, int rows, int n, int64_t
 size_t whirl_loss_workspace_bytes(int rows, int seqs);
 
 /* how a loss weighs its rows: s_row = w, w / (sum of w), or w / (sum of w over the row's sequence) / (sequences whose sum is
- * > 0).  The sums run over the rows that count; a sum of 0 leaves s = 0. */
+ * > 0).  The sums run over the rows that count; a sum of 0 leaves s = 0.  With WHIRL_MEAN_SEQS a row that counts but lies in
+ * no sequence has s = 0: it has all its outputs, adds nothing to the loss, and its row of dx is 0. */
 enum { WHIRL_MEAN_SUM = 0, WHIRL_MEAN_TOKENS = 1, WHIRL_MEAN_SEQS = 2 };
 
 /* The clipped policy loss with a KL term, from the logits, and its gradient in the same pass.  Per row that counts:

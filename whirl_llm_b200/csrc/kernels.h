@@ -171,7 +171,7 @@ struct LossArgs {
     float inv_t;
     const float* inv_t_rows;
     const float* weight;       // null = 1
-    const int32_t* seq_start;  // null: rows need not lie in a sequence
+    const int32_t* seq_start;  // policy loss: null but with WHIRL_MEAN_SEQS
     int seqs;
     // forward outputs (null: not wanted); the gradient reads stats, entropy, g_logp and g_entropy
     float* logp;

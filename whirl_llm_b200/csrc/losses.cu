@@ -386,10 +386,11 @@ __device__ __forceinline__ uint32_t row_word(const LossArgs& a, int row, bool wi
     else if (lane == 4 && EPI == EPI_POLICY && a.old_logp) p = a.old_logp + row;
     else if (lane == 5 && EPI != EPI_NONE && a.ref_logp) p = a.ref_logp + row;
     else if (lane == 6 && EPI == EPI_POLICY && with_scale) p = a.row_scale + row;
-    else if (lane == 7 && a.seq_start) p = a.seq_start;
-    else if (lane == 8 && a.seq_start) p = a.seq_start + a.seqs;
+    else if (lane == 7 && EPI == EPI_PREF) p = a.seq_start;
+    else if (lane == 8 && EPI == EPI_PREF) p = a.seq_start + a.seqs;
     return p ? *static_cast<const uint32_t*>(p) : 0u;
 }
+template <int EPI>
 __device__ __forceinline__ RowOf row_from(const LossArgs& a, int row, uint32_t got) {
     auto word = [&](int l) { return __shfl_sync(0xffffffffu, got, l); };
     auto real = [&](int l) { return __uint_as_float(word(l)); };
@@ -398,12 +399,12 @@ __device__ __forceinline__ RowOf row_from(const LossArgs& a, int row, uint32_t g
     const float it = real(1), wt = real(2);
     r.inv_t = a.inv_t_rows ? it : a.inv_t, r.weight = a.weight ? wt : 1.f;
     r.adv = real(3), r.old_logp = real(4), r.ref_logp = real(5), r.scale = real(6);
-    const int first = int(word(7)), end = int(word(8));
-    r.live = unsigned(r.token) < unsigned(a.n) && r.weight > 0.f && (!a.seq_start || (row >= first && row < end));
+    r.live = unsigned(r.token) < unsigned(a.n) && r.weight > 0.f;
+    if (EPI == EPI_PREF) r.live = r.live && row >= int(word(7)) && row < int(word(8));  // (the policy loss leaves such rows s = 0)
     return r;
 }
 template <int EPI>
-__device__ __forceinline__ RowOf row_of(const LossArgs& a, int row, bool with_scale) { return row_from(a, row, row_word<EPI>(a, row, with_scale)); }
+__device__ __forceinline__ RowOf row_of(const LossArgs& a, int row, bool with_scale) { return row_from<EPI>(a, row, row_word<EPI>(a, row, with_scale)); }
 
 // The policy loss of one row.
 struct PolicyRow {
@@ -439,6 +440,9 @@ __device__ __forceinline__ PolicyRow policy_row(const LossArgs& a, const RowOf& 
     return p;
 }
 
+// A policy row's share of the loss (a row without a weight in it, s = 0, has none whatever its own loss is).
+__device__ __forceinline__ double share_of(const RowOf& w, const PolicyRow& p) { return w.scale > 0.f ? double(w.scale) * double(p.loss) : 0.0; }
+
 // What a row comes to, from its statistics: s relative to the reference e (far: to the maximum itself).
 struct RowDone {
     double logp, shift;
@@ -455,7 +459,7 @@ __device__ __forceinline__ RowDone row_done(const LossArgs& a, const RowOf& w, c
     r.logp = (double(x_token) - double(m)) * double(w.inv_t) - (ln_s + r.shift);
     if (r.logp > 0.0) r.logp = 0.0;  // (by the last bits of the sum)
     r.entropy = ENT ? float(ln_s - kLn2 * double(q / s)) : 0.f;  // (the terms' mean exponent is q / s)
-    if (EPI == EPI_POLICY) r.p = policy_row(a, w, r.logp, r.entropy), r.g = w.scale * r.p.dlogp, r.h = -a.ent_coef * w.scale;
+    if (EPI == EPI_POLICY) r.p = policy_row(a, w, r.logp, r.entropy), r.g = w.scale > 0.f ? w.scale * r.p.dlogp : 0.f, r.h = -a.ent_coef * w.scale;
     return r;
 }
 // Writes what the call wants of a row.  One thread.
@@ -470,7 +474,7 @@ __device__ __forceinline__ void write_row(const LossArgs& a, int row, const RowO
         if (a.row_loss) a.row_loss[row] = live ? r.p.loss : 0.f;
         if (a.g_logp) a.g_logp[row] = live ? r.g : 0.f;
         if (a.g_entropy) a.g_entropy[row] = live ? r.h : 0.f;
-        if (TERM) a.row_term[row] = live ? double(w.scale) * double(r.p.loss) : 0.0;
+        if (TERM) a.row_term[row] = live ? share_of(w, r.p) : 0.0;
     } else if (EPI == EPI_PREF) {
         a.row_term[row] = live ? double(w.weight) * (r.logp - (a.ref_logp ? double(w.ref_logp) : 0.0)) : 0.0;
         a.row_scale[row] = live ? w.weight : 0.f;
@@ -961,7 +965,7 @@ __global__ void __launch_bounds__(kSmallRowThreads, K > 8 ? 2 : 3) small_rows_ke
 #pragma unroll 1
     for (; row64 < a.rows; row64 += warps) {
         const int row = int(row64);
-        const RowOf w = row_from(a, row, words);
+        const RowOf w = row_from<EPI>(a, row, words);
         if (row64 + warps < a.rows) words = row_word<EPI>(a, int(row64 + warps), true);  // (here by the time it is wanted)
         const T* x = static_cast<const T*>(a.x) + row64 * a.ld;
         T* const dx = GRAD ? static_cast<T*>(a.dx) + row64 * a.ld_dx : nullptr;
@@ -1008,7 +1012,7 @@ auto load = [&](int first) {
             }
             const RowDone d = row_done<EPI, ENT>(a, w, c, x_token, s.m, s.e, s.s, s.q, far);
             if (lane == 0) write_row<EPI, ENT, EPI != EPI_POLICY>(a, row, w, d);
-            if (EPI == EPI_POLICY) total += double(w.scale) * double(d.p.loss);
+            if (EPI == EPI_POLICY) total += share_of(w, d.p);
             if (GRAD && !(d.g == 0.f && d.h == 0.f)) q = grad_row(d.m, far, d.s, d.ln_s, c, w.inv_t, w.token, d.g, d.h, d.entropy);
         } else if (lane == 0) {
             write_row<EPI, ENT, EPI != EPI_POLICY>(a, row, w, RowDone{});
