@@ -53,3 +53,103 @@ def test_policy_rows_outside_the_sequences(rows, n, pad, off, dtype, grad):
         assert math.isnan(q.logp[0].item()) and math.isnan(q.row_loss[0].item())
         assert torch.equal(q.loss, r.loss) and torch.equal(q.logp[1:], r.logp[1:])
         assert not grad or torch.equal(q.dx, r.dx)
+
+
+def far_rows(n, dtype):
+    """Rows whose largest logit times inv_t is far from what a float's reference resolves, and their temperatures."""
+    g = torch.Generator().manual_seed(n)
+    fill = [-1e9, -3e9, -1e10, -1e30, 1e10, 30.0, 1e36]
+    it = torch.tensor([1.0, 1.25, 1.0, 0.8, 1.0, 1e8, 10.0, 1.0, 1.25, 1.0, 1e9, 1.0, 1e-3], dtype=torch.float32)
+    rows = len(it)
+    x = torch.randn((rows, n), generator=g) * 3
+    token = torch.randint(0, n, (rows,), generator=g, dtype=torch.int32)
+    for r, v in enumerate(fill):
+        x[r] = v
+    x[7, token[7]] = 1e10                     # one huge logit, on the token
+    x[8, (token[8] + 1) % n] = 1e10           # ... and beside it
+    x[9, ::2], x[9, 1::2] = -1e30, -2e30      # a masked row of two levels
+    x[11, : n // 2] = -1e30                   # an ordinary row, half of it masked
+    x[12] = 1e12 + 4e11 * x[12]               # a wide row at a temperature that leaves it ordinary differences
+    x = x.to(DT[dtype])
+    return x, x.double(), token, it
+
+
+def check_dx(dx, x64, token, it, stats, g, dtype, n, what):
+    d, p, lp = ref.dlogits(x64, token, it.double(), stats, g)
+    close(dx, d, ref.dx_tol(p, lp.clamp_min(-1e30), g, it.double(), DT[dtype], d, n=n), what)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [64, 1003, 20001, 60000, 1000003])
+def test_far_rows_in_every_gradient(n, dtype):
+    """Rows filled with masks of -1e9 to -1e30, huge logits, temperatures near zero: the same statistics and the same gradient in every
+    path (given statistics, the policy loss, the preference loss; n = 1000003 f32: the policy loss in two launches)."""
+    from whirl_llm_b200 import api
+    x, x64, token, it = far_rows(n, dtype)
+    rows = len(it)
+    xd, tok, itd = x.cuda(), token.cuda(), it.cuda()
+    m, s, lp, h = ref.row_stats(x64, it.double())
+    want = lp.gather(1, token.long()[:, None])[:, 0]
+    tol = ref.logp_tol(n, want)
+    r = api.token_logprobs(xd, tok, inv_t_rows=itd, want_entropy=True)
+    close(r.logp, want, tol, "logp")
+    close(r.entropy, h, ref.entropy_tol(n), "entropy")
+    assert torch.equal(r.stats[:, 0].double().cpu(), m)
+    close(r.stats[:, 1], s, s * ref.sum_error(n), "sum")
+    g = torch.linspace(-1, 1.1, rows)
+    dx = api.token_logprobs_grad(xd, tok, r.stats, g.cuda(), inv_t_rows=itd)
+    stats = (r.stats[:, 0].double().cpu(), r.stats[:, 1].double().cpu())
+    check_dx(dx, x64, token, it, stats, g.double(), dtype, n, "dx of given statistics")
+    adv = g.cuda()
+    for kw in (dict(), dict(ent_coef=0.01)):
+        q = api.policy_loss(xd, tok, adv, inv_t_rows=itd, mean=api.MEAN_SUM, **kw)
+        close(q.logp, want, tol, "logp of the policy loss")
+        close(q.g_logp, -g.double(), ref.EPS32 * g.double().abs(), "g_logp")
+        if not kw:
+            check_dx(q.dx, x64, token, it, (m, s), -g.double(), dtype, n, "dx of the policy loss")
+        else:
+            hh = torch.full((rows,), -0.01).double()
+            d, p, lpd = ref.dlogits(x64, token, it.double(), (m, s), -g.double(), hh, h)
+            close(q.dx, d, ref.dx_tol(p, lpd.clamp_min(-1e30), g.double(), it.double(), DT[dtype], d, hh, h, n), "dx with entropy")
+    starts = torch.tensor([0, 4, 7, 9, rows], dtype=torch.int32, device="cuda")
+    # (the rows' own log-probabilities as reference: the pairs' losses stay ordinary)
+    f = api.preference_loss(xd, tok, starts, r.logp, inv_t_rows=itd, beta=0.5)
+    close(f.logp, want, tol, "logp of the preference loss")
+    assert (f.g_logp[:7].abs() > 1e-3).all()  # (a float of -1e10 is off by hundreds: the other pair is decided)
+    check_dx(f.dx, x64, token, it, (m, s), f.g_logp.double().cpu(), dtype, n, "dx of the preference loss")
+
+
+@pytest.mark.parametrize("dtype,n", [("f32", 2500), ("bf16", 4200), ("f32", 20011)])
+@pytest.mark.parametrize("place", ["apart", "in place", "misaligned"])
+def test_policy_many_rows_of_every_kind(dtype, n, place):
+    """Clusters that take many rows: every third far (lowest value, the type's maximum, masks), rows without a distribution, masked ones
+    and ordinary ones in turn, each against the definition."""
+    from whirl_llm_b200 import api
+    rows = 2000 if n < 10000 else 700
+    g = torch.Generator().manual_seed(n)
+    x = (torch.randn((rows, n), generator=g) * 3).to(DT[dtype])
+    token = torch.randint(0, n, (rows,), generator=g, dtype=torch.int32)
+    weight = torch.ones(rows)
+    k = torch.arange(rows)
+    lim = torch.finfo(DT[dtype])
+    x[k % 9 == 0] = lim.min
+    x[(k % 9 == 3).nonzero()[:, 0], token[k % 9 == 3].long()] = lim.max
+    x[k % 9 == 6] = -1e30
+    x[(k % 5 == 1) & (k % 3 != 0), 7] = math.nan
+    weight[k % 4 == 2] = 0.0
+    x64, it = x.double(), ones(1.25, rows)
+    m, s, lp, h = ref.row_stats(x64, it)
+    logp = lp.gather(1, token.long()[:, None])[:, 0].float().double()  # (as float32: -4e38 is -inf there)
+    adv = torch.randn(rows, generator=g)
+    xd = x.cuda()
+    out = {"apart": None, "in place": xd, "misaligned": torch.zeros((rows, n + 1), dtype=DT[dtype], device="cuda")[:, 1:]}[place]
+    r = api.policy_loss(xd, token.cuda(), adv.cuda(), weight=weight.cuda(), inv_t=1.25, mean=api.MEAN_SUM, dx=out)
+    live = weight > 0
+    want = torch.where(live, logp, 0.0)
+    close(r.logp, want, ref.logp_tol(n, want.clamp_min(-1e30)), "logp")
+    gl = torch.where(live, torch.where(torch.isnan(logp), torch.nan, -adv.double()), 0.0)
+    close(r.g_logp, gl, 1e-30, "g_logp")
+    good = ~(torch.isnan(logp) & live)
+    d, p, lpd = ref.dlogits(x64[good], torch.where(live, token, -1)[good], it[good], (m[good], s[good]), gl[good])
+    close(r.dx[good.cuda()], d, ref.dx_tol(p, lpd.clamp_min(-1e30), gl[good], it[good], DT[dtype], d, n=n), "dx")
+    assert torch.isnan(r.dx[~good.cuda()]).all()

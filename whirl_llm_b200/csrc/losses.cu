@@ -73,7 +73,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // c = inv_t log2 e in two floats, hi rounded down so that lo >= 0 (a logit of -inf keeps its sign in both products).  With one float
 // the exponents of a whole row are off in the same direction, by up to 6e-8 of their size: a bias of some 3e-7 in every
 // log-probability, which sums over a sequence do not average out.
-// most: logits are clamped to +-most where a reference is made of them, so that most * c stays finite.
+// most: logits are clamped to +-most where a reference is made of them.  The terms of logits below -most vanish then (a thread that has met
+// masks of -1e30 alone keeps a sum of 0); a row whose own maximum lies beyond is a far row.
+// An exponent m c of 22 bits or more leaves a float too few bits behind the point.
+constexpr float kFarExponent = 4194304.f;
 struct Scale {
     float hi, lo, most;
 };
@@ -82,7 +85,7 @@ __device__ __forceinline__ Scale scale_of(float inv_t) {
     Scale r;
     r.hi = __double2float_rd(c);
     r.lo = fmaxf(float(c - double(r.hi)), 1e-37f);
-    r.most = fminf(1e37f / r.hi, FLT_MAX);
+    r.most = fminf(kFarExponent / r.hi, FLT_MAX);
     return r;
 }
 // The reference exponent of a maximum: a whole number, so that moving a sum from one reference to another scales it by a power of two, exactly
@@ -217,9 +220,15 @@ __device__ __forceinline__ Soft reduce_far(Soft a, float m, ReduceShared& sh, in
     return a;
 }
 
-// A row whose maximum is so large that its reference was clamped, or so low (rows of the type's lowest value) that its terms
-// vanished: exponents from the differences to the maximum, which is known by then.  Thread sums only.
-__device__ __forceinline__ bool is_far(const Soft& a) { return a.m >= -FLT_MAX && a.m <= FLT_MAX && !(a.s > 0.f && a.s <= FLT_MAX); }
+// A row whose maximum (of any sign: rows of the type's lowest value or of -1e30 alone, temperatures near zero) is beyond the references:
+// its exponents are made of the differences to the maximum, which is known by then.  One rule, from the maximum alone, for the
+// statistics and for a gradient that starts from given ones.
+__device__ __forceinline__ bool is_far(float m, const Scale& c) { return fabsf(m) <= FLT_MAX && fabsf(m) * c.hi >= kFarExponent; }
+// the exponent of a far row's logit
+__device__ __forceinline__ float far_exponent(float x, float m, float hi, float lo) {
+    const float d = x - m;
+    return fmaf(d, lo, d * hi);
+}
 
 // ---------------------------------------------------------------------------------------------------------------
 // reading and writing logits
@@ -314,7 +323,7 @@ __device__ __forceinline__ double mended(float s, float m, float e, const Scale&
     return t + (double(s) - top) * (1.0 + 5e-8);
 }
 
-// The row's gradient: dx_j = w_j * (a + b * t_j), + d on the token, with t_j = x_j c - e (far: (x_j - e) c) and w_j = 2^t_j, whose sum
+// The row's gradient: dx_j = w_j * (a + b * t_j), + d on the token, with t_j = x_j c - e (far: (x_j - m) c) and w_j = 2^t_j, whose sum
 // over the row is s:
 //   -inv_t g p_j - inv_t h p_j (log p_j + H),  p_j = w_j / s,  log p_j = ln 2 t_j - log s
 //   => a = -(inv_t / s) (g + h (H - log s)),  b = -(inv_t / s) h ln 2
@@ -334,7 +343,7 @@ __device__ __forceinline__ GradRow grad_row(float m, bool far, float s, float ln
 // LOW: with the scale's second float (a result of 8 bits does not show it)
 template <bool ENT, bool LOW>
 __device__ __forceinline__ float grad_of(const GradRow& q, float x) {
-    const float t0 = fmaf(x, q.c, -q.e), t = q.far ? (x - q.e) * q.c : (LOW ? fmaf(x, q.c_lo, t0) : t0), w = ex2_approx(t);
+    const float t0 = fmaf(x, q.c, -q.e), t = q.far ? far_exponent(x, q.e, q.c, q.c_lo) : (LOW ? fmaf(x, q.c_lo, t0) : t0), w = ex2_approx(t);
     return ENT ? w * fmaf(q.b, fmaxf(t, -1000.f), q.a) : w * q.a;
 }
 template <bool ENT, bool LOW, int N>
@@ -551,20 +560,20 @@ __device__ __forceinline__ void add_vec(Soft& s, uint4 v, const Scale& c) {
 }
 // a far row's thread sums (see is_far); m: the row's maximum
 template <typename T, bool ENT, int NT>
-__device__ __noinline__ Soft far_sums(const uint4* v, int cnt, bool have_edge, float x_edge, float m, float c) {
+__device__ __noinline__ Soft far_sums(const uint4* v, int cnt, bool have_edge, float x_edge, float m, float hi, float lo) {
     constexpr int E = 16 / sizeof(T);
     Soft a{m, 0.f, 0.f, 0.f, 0.f};
     for (int i = threadIdx.x % NT; i < cnt; i += NT) {
         float x[E];
         unpack<T>(v[i], x);
         for (int j = 0; j < E; ++j) {
-            const float t = (x[j] - m) * c, w = ex2_approx(t);
+            const float t = far_exponent(x[j], m, hi, lo), w = ex2_approx(t);
             a.s += w;
             if (ENT) a.q = fmaf(w, fmaxf(t, -1000.f), a.q);
         }
     }
     if (have_edge) {
-        const float t = (x_edge - m) * c, w = ex2_approx(t);
+        const float t = far_exponent(x_edge, m, hi, lo), w = ex2_approx(t);
         a.s += w;
         if (ENT) a.q = fmaf(w, fmaxf(t, -1000.f), a.q);
     }
@@ -599,13 +608,13 @@ template <typename T, bool ENT>
 __device__ __forceinline__ Soft row_sum(Soft s, const Scale& c, ReduceShared& sh, int ctas, const uint4* data, int cnt, bool have_edge, float x_edge,
                                         bool& far) {
     s = reduce<ENT>(s, c, sh, ctas, 0);
-    far = threadIdx.x < 32 && is_far(s);
+    far = threadIdx.x < 32 && is_far(s.m, c);
     if (__syncthreads_or(far)) {  // (every CTA of the cluster has the same statistics)
         if (threadIdx.x == 0) sh.m[0] = s.m;
         __syncthreads();
         const float m = sh.m[0];
         __syncthreads();
-        s = reduce_far<ENT>(far_sums<T, ENT, kRowThreads>(data, cnt, have_edge, x_edge, m, c.hi), m, sh, ctas);
+        s = reduce_far<ENT>(far_sums<T, ENT, kRowThreads>(data, cnt, have_edge, x_edge, m, c.hi, c.lo), m, sh, ctas);
         far = true;
     }
     return s;
@@ -819,8 +828,8 @@ __global__ void __launch_bounds__(kFusedThreads, kFusedCtas) fused_kernel(const 
             if (tid < 32) {
                 s = hear<ENT>(c, parts + set * n_parts, &s_bar[set], uint32_t(lives >> 1) & 1, n_parts, limit, x_token);
                 if (tid == 0) {
-                    s_far = is_far(s), s_m = s.m;
-                    if (!is_far(s)) finish(s, false);
+                    s_far = is_far(s.m, c), s_m = s.m;
+                    if (!is_far(s.m, c)) finish(s, false);
                 }
             }
             ++lives;
@@ -828,7 +837,7 @@ __global__ void __launch_bounds__(kFusedThreads, kFusedCtas) fused_kernel(const 
             if (s_far) {  // (every CTA of the cluster has the same statistics)
                 const float m = s_m;
                 const Scale one{1.f, 0.f, FLT_MAX};
-                s = far_sums<T, ENT, NT>(slice, cnt, at.edge >= 0, x_edge, m, c.hi);
+                s = far_sums<T, ENT, NT>(slice, cnt, at.edge >= 0, x_edge, m, c.hi, c.lo);
                 s.m = 0.f, s.e = 0.f;  // (references alike: nothing is scaled on the way)
                 tell<ENT>(s, 0.f, one, parts + 2 * n_parts + my_part, &s_bar[2], ctas);
                 if (tid < 32) {
@@ -948,7 +957,7 @@ __device__ __forceinline__ GradRow grad_row_of(const LossArgs& a, int row, int t
     const float inv_t = a.inv_t_rows ? a.inv_t_rows[row] : a.inv_t;
     const float m = a.stats[2 * int64_t(row)], sum = a.stats[2 * int64_t(row) + 1];
     const Scale c = scale_of(inv_t);
-    const bool far = !(m >= -c.most && m <= c.most);
+    const bool far = is_far(m, c);
     const double y = far ? 0.0 : shift_of(m, ref_of(m, c), inv_t);
     return grad_row(m, far, shifted(sum, -y), float(ln_of(double(sum)) - y), c, inv_t, token, g, h, ent ? a.entropy[row] : 0.f);
 }
@@ -1005,9 +1014,9 @@ auto load = [&](int first) {
             raise<ENT>(s, m, c);
             s.s = warp_sum_f(s.s);
             if (ENT) s.q = warp_sum_f(s.q);
-            const bool far = is_far(s);
+            const bool far = is_far(m, c);
             if (far) {
-                Soft t = far_sums<T, ENT, 32>(v, nv, edge >= 0, x_edge, m, c.hi);
+                Soft t = far_sums<T, ENT, 32>(v, nv, edge >= 0, x_edge, m, c.hi, c.lo);
                 s.s = warp_sum_f(t.s), s.q = warp_sum_f(t.q);
             }
             const RowDone d = row_done<EPI, ENT>(a, w, c, x_token, s.m, s.e, s.s, s.q, far);
