@@ -153,3 +153,28 @@ def test_policy_many_rows_of_every_kind(dtype, n, place):
     d, p, lpd = ref.dlogits(x64[good], torch.where(live, token, -1)[good], it[good], (m[good], s[good]), gl[good])
     close(r.dx[good.cuda()], d, ref.dx_tol(p, lpd.clamp_min(-1e30), gl[good], it[good], DT[dtype], d, n=n), "dx")
     assert torch.isnan(r.dx[~good.cuda()]).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [1003, 20001, 60000])
+def test_masked_rows_of_a_pair_without_a_finite_factor(n, dtype):
+    """A pair whose loss is NaN (a row without a distribution) or infinite (squared loss, a forbidden token): its rows that do not count
+    get zeros, and so do the rows outside the pairs."""
+    from whirl_llm_b200 import api
+    x, _, token = make(10, n, dtype, seed=6)
+    x = x.clone()
+    starts = torch.tensor([0, 3, 5, 7, 9], dtype=torch.int32, device="cuda")
+    weight = torch.tensor([1.0, 0, 1, 0, 1, 1, 0, 1, 0, 1], device="cuda")
+    dead = weight == 0
+    dead[9] = True
+    x[2, 5] = math.nan
+    r = api.preference_loss(x, token.cuda(), starts, weight=weight)
+    assert math.isnan(r.pair_loss[0].item()) and math.isfinite(r.pair_loss[1].item())
+    assert (r.g_logp[dead] == 0).all() and (r.dx[dead] == 0).all() and (r.logp[dead] == 0).all()
+    assert torch.isnan(r.g_logp[[0, 2, 4]]).all() and torch.isnan(r.dx[[0, 2, 4]]).all()
+    assert torch.isfinite(r.dx[[5, 7]]).all() and (r.dx[[5, 7]] != 0).any()
+    x[2, 5] = 0.0
+    x[2, token[2]] = -math.inf
+    r = api.preference_loss(x, token.cuda(), starts, weight=weight, kind=api.PREF_SQUARED)
+    assert r.pair_loss[0].item() == math.inf and math.isfinite(r.pair_loss[1].item())
+    assert (r.g_logp[dead] == 0).all() and (r.dx[dead] == 0).all() and (r.logp[dead] == 0).all()

@@ -1265,7 +1265,10 @@ __global__ void __launch_bounds__(kPairThreads) pairs_kernel(const __grid_consta
     int2 b[2];
     const double2 c = pair_done(a, p, blockIdx.x, b, sh);
     for (int k = 0; k < 2; ++k)
-        for (int r = b[k].x + int(threadIdx.x); r < b[k].y; r += kPairThreads) a.g_logp[r] = float((k ? c.y : c.x) * double(a.row_scale[r]));
+        for (int r = b[k].x + int(threadIdx.x); r < b[k].y; r += kPairThreads) {
+            const float w = a.row_scale[r];  // 0: the row does not count, whatever the pair comes to (NaN, infinity)
+            a.g_logp[r] = w > 0.f ? float((k ? c.y : c.x) * double(w)) : 0.f;
+        }
     last_sum(a.ticket, gridDim.x, a.seq_term, p.pairs, 1.0 / p.pairs, a.loss);
 }
 
