@@ -178,3 +178,32 @@ def test_masked_rows_of_a_pair_without_a_finite_factor(n, dtype):
     r = api.preference_loss(x, token.cuda(), starts, weight=weight, kind=api.PREF_SQUARED)
     assert r.pair_loss[0].item() == math.inf and math.isfinite(r.pair_loss[1].item())
     assert (r.g_logp[dead] == 0).all() and (r.dx[dead] == 0).all() and (r.logp[dead] == 0).all()
+
+
+@pytest.mark.parametrize("n", [1003, 20001, 60000])
+@pytest.mark.parametrize("shift", [1e4, 1e5, -1e5, 1e6, -1e6])
+def test_gradient_of_logits_with_an_offset(n, shift):
+    """bf16 logits that all lie far from zero (by less than far rows): probabilities from differences of a few steps."""
+    from whirl_llm_b200 import api
+    rows = 6
+    g = torch.Generator().manual_seed(n + int(shift))
+    x = (shift + abs(shift) * torch.randint(-3, 3, (rows, n), generator=g) / 256).to(torch.bfloat16)
+    token = torch.randint(0, n, (rows,), generator=g, dtype=torch.int32)
+    it = torch.full((rows,), 300.0 / abs(shift))   # a step (shift / 256 or / 128) is worth one or two units
+    it[3:] = 1.25
+    x64 = x.double()
+    m, s, lp, h = ref.row_stats(x64, it.double())
+    xd, tok, itd = x.cuda(), token.cuda(), it.cuda()
+    r = api.token_logprobs(xd, tok, inv_t_rows=itd, want_entropy=True)
+    want = lp.gather(1, token.long()[:, None])[:, 0]
+    close(r.logp, want, ref.logp_tol(n, want), "logp")
+    gl, gh = torch.randn(rows, generator=g), torch.randn(rows, generator=g)
+    stats, e64 = (r.stats[:, 0].double().cpu(), r.stats[:, 1].double().cpu()), r.entropy.double().cpu()
+    for use_h in (False, True):
+        dx = api.token_logprobs_grad(xd, tok, r.stats, gl.cuda(), inv_t_rows=itd, entropy=r.entropy if use_h else None, g_entropy=gh.cuda() if use_h else None)
+        d, p, lpd = ref.dlogits(x64, token, it.double(), stats, gl.double(), gh.double() if use_h else None, e64)
+        close(dx, d, ref.dx_tol(p, lpd, gl.double(), it.double(), torch.bfloat16, d, gh.double() if use_h else None, e64, n), "dx")
+    q = api.policy_loss(xd, tok, gl.cuda(), inv_t_rows=itd, mean=api.MEAN_SUM, ent_coef=0.5)
+    hh = torch.full((rows,), -0.5).double()
+    d, p, lpd = ref.dlogits(x64, token, it.double(), (m, s), -gl.double(), hh, h)
+    close(q.dx, d, ref.dx_tol(p, lpd, gl.double(), it.double(), torch.bfloat16, d, hh, h, n), "dx of the policy loss")

@@ -340,20 +340,19 @@ __device__ __forceinline__ GradRow grad_row(float m, bool far, float s, float ln
     q.d = inv_t * g;
     return q;
 }
-// LOW: with the scale's second float (a result of 8 bits does not show it)
-template <bool ENT, bool LOW>
+// (The scale's second float is needed for results of 8 bits too: it is worth x c_lo in the exponent, 0.8 % of p at a logit of 1e5.)
+template <bool ENT>
 __device__ __forceinline__ float grad_of(const GradRow& q, float x) {
-    const float t0 = fmaf(x, q.c, -q.e), t = q.far ? far_exponent(x, q.e, q.c, q.c_lo) : (LOW ? fmaf(x, q.c_lo, t0) : t0), w = ex2_approx(t);
+    const float t0 = fmaf(x, q.c, -q.e), t = q.far ? far_exponent(x, q.e, q.c, q.c_lo) : fmaf(x, q.c_lo, t0), w = ex2_approx(t);
     return ENT ? w * fmaf(q.b, fmaxf(t, -1000.f), q.a) : w * q.a;
 }
-template <bool ENT, bool LOW, int N>
+template <bool ENT, int N>
 __device__ __forceinline__ void grad_many(const GradRow& q, float (&x)[N]) {  // (not for a far row)
     const F2 ne = f2(-q.e, -q.e), c = f2(q.c, q.c), lo = f2(q.c_lo, q.c_lo), a = f2(q.a, q.a), b = f2(q.b, q.b);
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
         const F2 v = f2(x[i], x[i + 1]);
-        const F2 t0 = fma2(v, c, ne);
-        const float2 t = split(LOW ? fma2(v, lo, t0) : t0);
+        const float2 t = split(fma2(v, lo, fma2(v, c, ne)));
         const F2 w = f2(ex2_approx(t.x), ex2_approx(t.y));
         const float2 r = split(ENT ? mul2(w, fma2(b, f2(fmaxf(t.x, -1000.f), fmaxf(t.y, -1000.f)), a)) : mul2(w, a));
         x[i] = r.x, x[i + 1] = r.y;
@@ -364,7 +363,7 @@ template <typename T, bool ENT>
 __device__ __forceinline__ uint4 grad_vec(const GradRow& q, uint4 v) {
     float e[16 / sizeof(T)];
     unpack<T>(v, e);
-    grad_many<ENT, sizeof(T) == 4, 16 / sizeof(T)>(q, e);
+    grad_many<ENT, 16 / sizeof(T)>(q, e);
     return pack<T>(e);
 }
 
@@ -862,7 +861,7 @@ __global__ void __launch_bounds__(kFusedThreads, kFusedCtas) fused_kernel(const 
         GradRow q{};
         if (!zero) q = s_q;
         T* dx = static_cast<T*>(a.dx) + int64_t(row) * a.ld_dx;
-        if (at.edge >= 0) store_one(dx + at.edge, zero ? 0.f : grad_of<ENT, sizeof(T) == 4>(q, x_edge) + (at.edge == q.token ? q.d : 0.f));
+        if (at.edge >= 0) store_one(dx + at.edge, zero ? 0.f : grad_of<ENT>(q, x_edge) + (at.edge == q.token ? q.d : 0.f));
         const bool vec = ((reinterpret_cast<uintptr_t>(at.x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
         T* body = dx + at.head + int64_t(at.v0) * E;
         uint4* out = reinterpret_cast<uint4*>(body);
@@ -894,11 +893,11 @@ __global__ void __launch_bounds__(kFusedThreads, kFusedCtas) fused_kernel(const 
             for (; i < cnt; i += NT) {
 #pragma unroll 1
                 for (int j = 0; j < E; ++j)
-                    store_one(body + int64_t(i) * E + j, zero ? 0.f : grad_of<ENT, sizeof(T) == 4>(q, load_one(reinterpret_cast<const T*>(slice + i) + j)));
+                    store_one(body + int64_t(i) * E + j, zero ? 0.f : grad_of<ENT>(q, load_one(reinterpret_cast<const T*>(slice + i) + j)));
             }
             i = tid;
         }
-        if (mine) store_one(body + t, grad_of<ENT, sizeof(T) == 4>(q, x_mine) + q.d);
+        if (mine) store_one(body + t, grad_of<ENT>(q, x_mine) + q.d);
 #pragma unroll 4
         for (; i < refill; i += NT) copy_async16(slice + i, next + i);
         copies_commit();
@@ -925,7 +924,7 @@ __device__ __forceinline__ void small_grad(const GradRow& q, const T* x, T* dx, 
     const bool zero = q.a == 0.f && q.b == 0.f && q.d == 0.f;
     const bool vec = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;
     const int t = zero ? -1 : q.token - head;  // the token's place among the vectors
-    if (edge >= 0) store_one(dx + edge, zero ? 0.f : grad_of<ENT, sizeof(T) == 4>(q, x_edge) + (edge == q.token ? q.d : 0.f));
+    if (edge >= 0) store_one(dx + edge, zero ? 0.f : grad_of<ENT>(q, x_edge) + (edge == q.token ? q.d : 0.f));
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const int i = first + k * 32 + lane_id();
@@ -936,10 +935,10 @@ __device__ __forceinline__ void small_grad(const GradRow& q, const T* x, T* dx, 
             for (int j = 0; j < E; ++j) e[j] = 0.f;
         } else {
             unpack<T>(b[k], e);
-            if (!q.far) grad_many<ENT, sizeof(T) == 4, E>(q, e);
+            if (!q.far) grad_many<ENT, E>(q, e);
             else
 #pragma unroll
-                for (int j = 0; j < E; ++j) e[j] = grad_of<ENT, sizeof(T) == 4>(q, e[j]);
+                for (int j = 0; j < E; ++j) e[j] = grad_of<ENT>(q, e[j]);
             if (t >= 0 && t / E == i)
 #pragma unroll
                 for (int j = 0; j < E; ++j) e[j] += t % E == j ? q.d : 0.f;
@@ -1102,16 +1101,16 @@ __global__ void __launch_bounds__(kGradThreads, 6) grad_kernel(const __grid_cons
         }
 #pragma unroll 1
         for (; i < nv; i += NT) __stcs(dv + i, grad_vec<T, ENT>(q, v[i]));
-        if (mine) store_one(dx + at, grad_of<ENT, sizeof(T) == 4>(q, x_token) + q.d);
+        if (mine) store_one(dx + at, grad_of<ENT>(q, x_token) + q.d);
     } else {  // one by one
         for (int k = tid; k < nv * E; k += NT) {
             const int j = head + k;
-            store_one(dx + j, grad_of<ENT, sizeof(T) == 4>(q, load_one(x + j)) + (j == at ? q.d : 0.f));
+            store_one(dx + j, grad_of<ENT>(q, load_one(x + j)) + (j == at ? q.d : 0.f));
         }
     }
     for (int k = tid; k < n - nv * E; k += NT) {
         const int j = k < head ? k : k + nv * E;
-        store_one(dx + j, grad_of<ENT, sizeof(T) == 4>(q, load_one(x + j)) + (j == at ? q.d : 0.f));
+        store_one(dx + j, grad_of<ENT>(q, load_one(x + j)) + (j == at ? q.d : 0.f));
     }
 }
 
