@@ -207,3 +207,26 @@ def test_gradient_of_logits_with_an_offset(n, shift):
     hh = torch.full((rows,), -0.5).double()
     d, p, lpd = ref.dlogits(x64, token, it.double(), (m, s), -gl.double(), hh, h)
     close(q.dx, d, ref.dx_tol(p, lpd, gl.double(), it.double(), torch.bfloat16, d, hh, h, n), "dx of the policy loss")
+
+
+@pytest.mark.parametrize("n", [1003, 20001])
+@pytest.mark.parametrize("inv_t", [1e-36, 3e-34, 1e-30])
+def test_smallest_inv_t(n, inv_t):
+    """Logits of up to 1e38 at an inverse temperature near the smallest normal number."""
+    from whirl_llm_b200 import api
+    g = torch.Generator().manual_seed(n)
+    rows = 5
+    it = torch.full((rows,), inv_t)
+    x = torch.randn((rows, n), generator=g) * float(3 / it[0])
+    x[1, ::3] = -math.inf
+    token = torch.randint(0, n, (rows,), generator=g, dtype=torch.int32)
+    m, s, lp, h = ref.row_stats(x.double(), it.double())
+    want = lp.gather(1, token.long()[:, None])[:, 0]
+    r = api.token_logprobs(x.cuda(), token.cuda(), inv_t=it[0].item(), want_entropy=True)
+    close(r.logp, want, ref.logp_tol(n, want), "logp")
+    close(r.stats[:, 1], s, s * ref.sum_error(n), "sum")
+    close(r.entropy, h, ref.entropy_tol(n), "entropy")
+    gl = torch.full((rows,), 1e36)
+    dx = api.token_logprobs_grad(x.cuda(), token.cuda(), r.stats, gl.cuda(), inv_t=it[0].item())
+    d, p, lpd = ref.dlogits(x.double(), token, it.double(), (r.stats[:, 0].double().cpu(), r.stats[:, 1].double().cpu()), gl.double())
+    close(dx, d, ref.dx_tol(p, lpd, gl.double(), it.double(), torch.float32, d, n=n), "dx")

@@ -84,7 +84,7 @@ __device__ __forceinline__ Scale scale_of(float inv_t) {
     const double c = double(inv_t) * 1.4426950408889634;
     Scale r;
     r.hi = __double2float_rd(c);
-    r.lo = fmaxf(float(c - double(r.hi)), 1e-37f);
+    r.lo = fmaxf(float(c - double(r.hi)), fmaxf(r.hi * 1e-12f, 1e-45f));  // (at the smallest inv_t too it may not outweigh hi)
     r.most = fminf(kFarExponent / r.hi, FLT_MAX);
     return r;
 }
