@@ -2,6 +2,7 @@
 such rows; against the 64-bit definitions (loss_ref.py)."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -230,3 +231,20 @@ def test_smallest_inv_t(n, inv_t):
     dx = api.token_logprobs_grad(x.cuda(), token.cuda(), r.stats, gl.cuda(), inv_t=it[0].item())
     d, p, lpd = ref.dlogits(x.double(), token, it.double(), (r.stats[:, 0].double().cpu(), r.stats[:, 1].double().cpu()), gl.double())
     close(dx, d, ref.dx_tol(p, lpd, gl.double(), it.double(), torch.float32, d, n=n), "dx")
+
+
+@pytest.mark.parametrize("rows,n,dtype,inv_t", [(4000, 1003, "f32", 1.0), (4000, 1003, "bf16", 1.25), (3000, 9000, "f32", 1.0), (4000, 20001, "bf16", 1.0), (2000, 60000, "f32", 0.8)])
+def test_errors_of_many_rows_do_not_add_up(rows, n, dtype, inv_t):
+    """The log-probability of a long sequence: a row's errors are roundings that fall either way (its sum's float, some ten partial sums
+    and the largest terms: less than one half step of a float in the mean square) and what is left of the mean error of the
+    hardware's exponential (less than 1e-8, see the kernels)."""
+    from whirl_llm_b200 import api
+    g = torch.Generator(device="cuda").manual_seed(n)
+    x = (torch.randn((rows, n), generator=g, device="cuda") * 3).to(DT[dtype])
+    token = torch.randint(0, n, (rows,), generator=g, device="cuda")
+    x.scatter_(1, token[:, None], (math.log(n) + 2 + 3 * torch.randn(rows, generator=g, device="cuda")).to(x.dtype)[:, None])
+    z = torch.cat([torch.log_softmax(v.double() * float(np.float32(inv_t)), 1).gather(1, t[:, None])[:, 0] for v, t in zip(x.split(500), token.split(500))])
+    starts = torch.tensor([0, rows, rows], dtype=torch.int32, device="cuda")
+    r = api.preference_loss(x, token.int(), starts, ref_logp=z.float(), inv_t=inv_t, beta=1.0)   # what is left is small: no rounding of its own
+    want = (z - z.float().double()).sum()
+    assert abs(r.reward[0, 0].double() - want) < 1e-8 * rows + 6 * ref.EPS32 * math.sqrt(rows), ((r.reward[0, 0].double() - want) / rows).item()

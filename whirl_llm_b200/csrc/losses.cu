@@ -70,31 +70,37 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-// c = inv_t log2 e in two floats, hi rounded down so that lo >= 0 (a logit of -inf keeps its sign in both products).  With one float
+// c = inv_t log2 e in two floats, hi rounded down so that lo > 0 (a logit of -inf keeps its sign in both products).  With one float
 // the exponents of a whole row are off in the same direction, by up to 6e-8 of their size: a bias of some 3e-7 in every
-// log-probability, which sums over a sequence do not average out.
+// log-probability, which sums over a sequence do not average out.  hi has 16 bits: with 24, x lo is less than half a step of the exponent that it
+// is added to, and the same rounding takes it away in term after term (measured: 3e-8 to 8e-8 in the sum).
 // most: logits are clamped to +-most where a reference is made of them.  The terms of logits below -most vanish then (a thread that has met
 // masks of -1e30 alone keeps a sum of 0); a row whose own maximum lies beyond is a far row.
-// An exponent m c of 22 bits or more leaves a float too few bits behind the point.
-constexpr float kFarExponent = 4194304.f;
+// From 2^18 on an exponent m c, less its reference, keeps a rest of m lo that takes bits from the result.
+constexpr float kFarExponent = 262144.f;
 struct Scale {
     float hi, lo, most;
 };
 __device__ __forceinline__ Scale scale_of(float inv_t) {
     const double c = double(inv_t) * 1.4426950408889634;
     Scale r;
-    r.hi = __double2float_rd(c);
+    r.hi = __uint_as_float(__float_as_uint(__double2float_rd(c)) & 0xffffff00u);
     r.lo = fmaxf(float(c - double(r.hi)), fmaxf(r.hi * 1e-12f, 1e-45f));  // (at the smallest inv_t too it may not outweigh hi)
     r.most = fminf(kFarExponent / r.hi, FLT_MAX);
     return r;
 }
 // The reference exponent of a maximum: a whole number, so that moving a sum from one reference to another scales it by a power of two, exactly
-// (ex2.approx is low by 5e-8 on average: three moves of every partial sum would show in the log-probability).
-__device__ __forceinline__ float ref_of(float m, const Scale& c) { return rintf(fminf(fmaxf(m, -c.most), c.most) * c.hi); }
+// (ex2.approx is low by 5e-8 on average: three moves of every partial sum would show in the log-probability).  It lies kAbove above the maximum's
+// own exponent, so that every term's is below -1: there ex2.approx has the same mean error at every exponent (mended).
+constexpr float kAbove = 2.f;
+__device__ __forceinline__ float ref_of(float m, const Scale& c) {
+    const float x = fminf(fmaxf(m, -c.most), c.most);
+    return rintf(fmaf(x, c.lo, fmaf(x, c.hi, kAbove)));
+}
 
 // Partial statistics of a set of logits: m their maximum (-inf without one), e = ref_of(m), s - k = sum 2^(x c - e) (k: what
 // Kahan's sum owes), q = sum of the same terms times their exponent.  The exponent is two fused multiply-adds from the logit (first hi: the
-// difference to e is small, and rounded as such, before lo comes to it); that e is not
+// difference to e is small, and rounded as such, before lo comes to it; both roundings fall anywhere); that e is not
 // the maximum's own exponent shifts all terms of a row by the same factor (shift_of).
 // A plain float sum is not enough: in the thread that meets the row's peak every later term is rounded to the peak's last
 // bits, 300 times in a row of 151936, all of it landing in the log-probability (measured: 4e-7).
@@ -214,7 +220,7 @@ __device__ __forceinline__ Soft reduce(Soft a, const Scale& c, ReduceShared& sh,
 template <bool ENT>
 __device__ __forceinline__ Soft reduce_far(Soft a, float m, ReduceShared& sh, int ctas) {
     Scale one{1.f, 0.f, FLT_MAX};
-    a.m = 0.f, a.e = 0.f;  // (references alike: nothing is scaled)
+    a.m = 0.f, a.e = ref_of(0.f, one);  // (references alike: nothing is scaled)
     a = reduce<ENT>(a, one, sh, ctas, 1);
     a.m = m;
     return a;
@@ -310,17 +316,22 @@ __device__ __forceinline__ float kl_of(float k) {
 // The natural logarithm of what the reference e of a row with maximum m puts into its sum, ln 2 (e - m c).  64 bits: m c has to be exact
 // to the last bits of e.
 __device__ __forceinline__ double shift_of(float m, float e, float inv_t) { return kLn2 * (double(e) - double(m) * (double(inv_t) * 1.4426950408889634)); }
-__device__ __forceinline__ float shifted(float s, double y) { return s * exp_of(float(y)); }  // s e^y
+__device__ __forceinline__ float shifted(float s, double y) {  // s e^y; the whole powers of two apart, they are exact
+    const float k = rintf(float(y) * kLog2e);
+    return s * exp_of(float(y - kLn2 * double(k))) * ex2_approx(k);
+}
 // A row's sum s, relative to its reference e, less the errors of ex2.approx that show.  That of the maximum's own term is taken out exactly (it is all that
-// stands between a near-certain token's log-probability and 0); the others are low by 5e-8 on average (measured, exponents of -24 .. 0).
+// stands between a near-certain token's log-probability and 0).  The others are low by 5e-8 on average: measured over exponents of -24 to -1, each
+// power of two between 4.9e-8 and 5.1e-8, a sixteenth of one between 3.3e-8 and 6.2e-8, a single term up to 1.4e-7.  So a row of
+// many terms keeps some 1e-9, a row of two or three up to 1e-7 of what stands beside the maximum.
 __device__ __forceinline__ double mended(float s, float m, float e, const Scale& c, double shift) {
-    const double y = -shift;  // ln 2 (m c - e), within ln 2 / 2 unless m c has no fraction
+    const double y = double(kAbove) * kLn2 - shift;  // ln 2 (m c - e + kAbove), within ln 2 / 2
     if (!(fabs(y) < 0.36)) return double(s);
     double t = 1.0 / 3628800.0;
     t = fma(t, y, 1.0 / 362880.0), t = fma(t, y, 1.0 / 40320.0), t = fma(t, y, 1.0 / 5040.0), t = fma(t, y, 1.0 / 720.0), t = fma(t, y, 1.0 / 120.0);
     t = fma(t, y, 1.0 / 24.0), t = fma(t, y, 1.0 / 6.0), t = fma(t, y, 0.5), t = fma(t, y, 1.0), t = fma(t, y, 1.0);
     const double top = double(ex2_approx(fmaf(m, c.lo, fmaf(m, c.hi, -e))));  // as it went into the sum
-    return t + (double(s) - top) * (1.0 + 5e-8);
+    return t * 0.25 + (double(s) - top) * (1.0 + 5e-8);                       // (2^-kAbove)
 }
 
 // The row's gradient: dx_j = w_j * (a + b * t_j), + d on the token, with t_j = x_j c - e (far: (x_j - m) c) and w_j = 2^t_j, whose sum
@@ -334,7 +345,8 @@ struct GradRow {
 __device__ __forceinline__ GradRow grad_row(float m, bool far, float s, float ln_s, const Scale& c, float inv_t, int token, float g, float h, float entropy) {
     GradRow q;
     q.far = far, q.e = far ? m : ref_of(m, c), q.c = c.hi, q.c_lo = c.lo, q.token = token;
-    const float k = inv_t / s;
+    float k = inv_t / s;
+    if (!far) k = fmaf(k, 5e-8f, k);  // (what ex2.approx is low by: see mended)
     q.a = -k * (h == 0.f ? g : g + h * (entropy - ln_s));
     q.b = -k * h * float(kLn2);
     q.d = inv_t * g;
@@ -837,7 +849,7 @@ __global__ void __launch_bounds__(kFusedThreads, kFusedCtas) fused_kernel(const 
                 const float m = s_m;
                 const Scale one{1.f, 0.f, FLT_MAX};
                 s = far_sums<T, ENT, NT>(slice, cnt, at.edge >= 0, x_edge, m, c.hi, c.lo);
-                s.m = 0.f, s.e = 0.f;  // (references alike: nothing is scaled on the way)
+                s.m = 0.f, s.e = ref_of(0.f, one);  // (references alike: nothing is scaled on the way)
                 tell<ENT>(s, 0.f, one, parts + 2 * n_parts + my_part, &s_bar[2], ctas);
                 if (tid < 32) {
                     float none;
