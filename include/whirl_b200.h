@@ -396,6 +396,11 @@ typedef struct whirl_policy_out { /* only loss is required */
 int whirl_policy_loss(const void* x, int dtype, int rows, int n, int64_t ld, const whirl_policy_params* params,
                       const whirl_policy_out* out, void* ws, size_t ws_bytes, void* stream);
 
+/* Reads the error word that the last loss on this workspace left (the call synchronises `stream`).  WHIRL_OK, or
+ * WHIRL_ERR_TIMEOUT with *where (may be null) = 1 when a bounded wait of the policy loss ran out (an exchange of a row's
+ * statistics between thread blocks): rows, and the loss with them, are NaN then that need not be. */
+int whirl_loss_check(const void* ws, size_t ws_bytes, void* stream, uint32_t* where);
+
 /* A preference loss over pairs of sequences: sequence 2 i is the chosen one of pair i, 2 i + 1 the rejected one, and sequence s
  * holds the rows seq_start[s] .. seq_start[s + 1).  With P_s = sum of w * (logp - ref_logp) over the rows of s that count
  * (divided by the sum of their w with average != 0; 0 for a sequence without such rows):
@@ -502,7 +507,8 @@ int whirl_check(const void* ws, size_t ws_bytes, int rows, void* stream, uint32_
 /* Testing aid, per calling thread: the following whirl_sample_rows / whirl_topk_rows calls give every wait of the
  * single-pass kernel a budget of about wait_us microseconds (0 = the default, about a second), and with lose_copy != 0
  * the first CTA leaves one bulk copy of its first row out, so that the waits on it run out and the error path above
- * can be exercised without a fault.  whirl_test_waits(0, 0) restores the defaults. */
+ * can be exercised without a fault.  The same for whirl_policy_loss with a gradient: the first cluster leaves one exchange of
+ * statistics out.  whirl_test_waits(0, 0) restores the defaults. */
 void whirl_test_waits(uint32_t wait_us, int lose_copy);
 
 /* The same call on HOST buffers: logits, parameters and outputs are host pointers; the call copies them to the device

@@ -135,6 +135,7 @@ def _load() -> C.CDLL:
         "whirl_token_logprobs_grad": (i, [vp, i, i, i, i64, vp, f, vp, vp, vp, vp, vp, vp, i64, vp]),
         "whirl_loss_workspace_bytes": (sz, [i, i]),
         "whirl_policy_loss": (i, [vp, i, i, i, i64, C.POINTER(PolicyParams), C.POINTER(PolicyOut), vp, sz, vp]),
+        "whirl_loss_check": (i, [vp, sz, vp, C.POINTER(C.c_uint32)]),
         "whirl_preference_loss": (i, [vp, i, i, i, i64, C.POINTER(PreferenceParams), C.POINTER(PreferenceOut), vp, sz, vp]),
         "whirl_block_workspace_bytes": (sz, [i]),
         "whirl_block_tables_step": (i, [vp, vp, C.POINTER(BlockTables), C.POINTER(StepRowsOut), vp, sz, vp]),
@@ -152,7 +153,7 @@ DECLARED = ["whirl_status_string", "whirl_last_error", "whirl_version", "whirl_w
             "whirl_topk_rows", "whirl_topk_rows_shard", "whirl_merge_sample_rows", "whirl_sample_rows", "whirl_sample_rows_host", "whirl_host_release", "whirl_host_last_error",
             "whirl_launch_counts", "whirl_check", "whirl_shard_block_words", "whirl_merge_sample_rows_packed", "whirl_test_waits", "whirl_accept_rows",
             "whirl_uniform_splitmix", "whirl_race_base", "whirl_philox4x32_10", "whirl_uniform_philox4x32", "whirl_fill_draws",
-            "whirl_token_logprobs", "whirl_token_logprobs_grad", "whirl_loss_workspace_bytes", "whirl_policy_loss", "whirl_preference_loss",
+            "whirl_token_logprobs", "whirl_token_logprobs_grad", "whirl_loss_workspace_bytes", "whirl_policy_loss", "whirl_loss_check", "whirl_preference_loss",
             "whirl_block_workspace_bytes", "whirl_block_tables_step"]
 
 
@@ -693,6 +694,17 @@ def policy_loss(x, token, adv, old_logp=None, ref_logp=None, weight=None, seq_st
                   _loss_rows(dx)[3] if want_grad else 0)
     _call(dev, lib.whirl_policy_loss, x.data_ptr(), dt, rows, n, ld, p, o, base + 16 * rows, nbytes)
     return PolicyResult(loss, logp, entropy, kl, row_loss, dx, aux)
+
+
+def loss_check(r: PolicyResult) -> int:
+    """whirl_loss_check: 1 if a wait of the policy_loss call that returned r ran out (rows are NaN that need not be), else 0.
+    Synchronises the stream."""
+    where, ws = C.c_uint32(0), r.aux[4 * r.logp.numel():]
+    with torch.cuda.device(r.aux.device):
+        st = lib.whirl_loss_check(ws.data_ptr(), 4 * ws.numel(), torch.cuda.current_stream().cuda_stream, C.byref(where))
+    if st not in (0, ERR_TIMEOUT):
+        _check(st)
+    return int(where.value)
 
 
 @dataclass

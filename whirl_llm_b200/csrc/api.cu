@@ -496,8 +496,9 @@ LossWs loss_ws(int rows, int seqs) {
     LossWs w;
     size_t o = 0;
     auto take = [&](size_t& off, size_t bytes) { off = o, o = align_up(o + bytes, 256); };
+    take(w.ticket, 256);  // (first: whirl_loss_check knows no sizes)
     take(w.row_term, r * 8), take(w.seq_term, s * 8), take(w.stats, r * 8);
-    take(w.entropy, r * 4), take(w.g_logp, r * 4), take(w.g_entropy, r * 4), take(w.row_scale, r * 4), take(w.ticket, 256);
+    take(w.entropy, r * 4), take(w.g_logp, r * 4), take(w.g_entropy, r * 4), take(w.row_scale, r * 4);
     w.total = o;
     return w;
 }
@@ -550,7 +551,8 @@ int whirl_policy_loss(const void* x, int dtype, int rows, int n, int64_t ld, con
     if (!ws || ws_bytes < w.total + 256) return fail(WHIRL_ERR_WORKSPACE, "policy_loss: workspace missing or too small (whirl_loss_workspace_bytes)");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (rows == 0) {
-        const cudaError_t e = cudaMemsetAsync(o->loss, 0, sizeof(float), st);
+        cudaError_t e = cudaMemsetAsync(o->loss, 0, sizeof(float), st);
+        if (e == cudaSuccess) e = cudaMemsetAsync(static_cast<uint8_t*>(base) + w.ticket, 0, 8, st);
         return e == cudaSuccess ? WHIRL_OK : fail_cuda(e, "cudaMemsetAsync");
     }
     const bool ent = p->ent_coef != 0.f;
@@ -566,6 +568,7 @@ int whirl_policy_loss(const void* x, int dtype, int rows, int n, int64_t ld, con
     a.row_term = reinterpret_cast<double*>(static_cast<uint8_t*>(base) + w.row_term);
     a.seq_term = reinterpret_cast<double*>(static_cast<uint8_t*>(base) + w.seq_term);
     a.ticket = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(base) + w.ticket), a.loss = o->loss;
+    a.wait_limit = g_wait_limit ? g_wait_limit : wb::kLossWaitLimit, a.lose_part = g_lose_copy;
     const cudaError_t e = wb::policy_launch(a, dtype, p->mean, st);
     return e == cudaSuccess ? WHIRL_OK : fail_cuda(e, "policy_loss launch");
 }
@@ -595,6 +598,19 @@ int whirl_preference_loss(const void* x, int dtype, int rows, int n, int64_t ld,
     a.ticket = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(base) + w.ticket), a.loss = o->loss;
     const cudaError_t e = wb::preference_launch(a, q, dtype, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? WHIRL_OK : fail_cuda(e, "preference_loss launch");
+}
+
+int whirl_loss_check(const void* ws, size_t ws_bytes, void* stream, uint32_t* where) {
+    if (!ws) return fail(WHIRL_ERR_INVALID, "loss_check: ws is null");
+    if (ws_bytes < whirl_loss_workspace_bytes(0, 0)) return fail(WHIRL_ERR_WORKSPACE, "loss_check: workspace too small");
+    const uintptr_t base = (reinterpret_cast<uintptr_t>(ws) + 255) & ~uintptr_t(255);
+    uint32_t word = 0;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaError_t e = cudaMemcpyAsync(&word, reinterpret_cast<const void*>(base + loss_ws(0, 0).ticket + 4), 4, cudaMemcpyDeviceToHost, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    if (e != cudaSuccess) return fail_cuda(e, "loss_check");
+    if (where) *where = word;
+    return word == 0 ? WHIRL_OK : fail(WHIRL_ERR_TIMEOUT, "a bounded wait of the policy loss ran out: rows are NaN");
 }
 
 size_t whirl_block_workspace_bytes(int seqs) { return wb::block_tables_ws_bytes(seqs < 1 ? 1 : seqs) + 256; }

@@ -191,9 +191,12 @@ struct LossArgs {
     float* row_scale;  // [rows] s of the policy loss; the rows' weights of the preference loss
     double* row_term;  // [rows] scaled row losses / weighted log ratios
     double* seq_term;  // [seqs] weight sums / pair losses
-    uint32_t* ticket;  // rows finished so far (zeroed by the call)
+    uint32_t* ticket;  // [2], zeroed by the call: rows finished so far; whether a wait ran out
     float* loss;
+    uint32_t wait_limit;  // policy loss: budget of every wait, in suspensions of about a microsecond
+    uint32_t lose_part;   // tests only: the last CTA of the first cluster leaves out one exchange of statistics, so that waits run out
 };
+constexpr uint32_t kLossWaitLimit = 1u << 20;
 struct PairArgs {
     int pairs, kind, average;
     float beta, smoothing, margin;

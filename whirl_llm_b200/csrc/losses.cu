@@ -723,16 +723,15 @@ __device__ __forceinline__ void tell(Soft a, float x_token, const Scale& c, Part
     if (ENT) a.q = warp_sum_f(a.q);
     if (lane_id() < ctas) send(mine, bar, lane_id(), Part{m, a.s, a.q, x_token});
 }
-// The row's statistics from n warps' (one warp).  A barrier that does not complete in its time gives a row of NaN.
+// The row's statistics from n warps' (one warp).  false: they did not come in their time.
 template <bool ENT>
-__device__ __forceinline__ Soft hear(const Scale& c, const Part* parts, uint64_t* bar, uint32_t parity, int n, uint32_t& limit, float& x_token) {
+__device__ __forceinline__ bool hear(const Scale& c, const Part* parts, uint64_t* bar, uint32_t parity, int n, uint32_t limit, Soft& s, float& x_token) {
     if (lane_id() == 0) mbar_expect_tx(bar, uint32_t(n * sizeof(Part)));
-    const bool came = __all_sync(0xffffffffu, mbar_wait(bar, parity, limit));
-    if (!came) limit = 1;  // (and the rows after it do not wait that long again)
+    if (!__all_sync(0xffffffffu, mbar_wait(bar, parity, limit))) return false;
     float m = -INFINITY;
     for (int i = lane_id(); i < n; i += 32) m = fmaxf(m, parts[i].m);
     m = warp_max_f(m);
-    Soft s{m, ref_of(m, c), 0.f, 0.f, 0.f};
+    s = Soft{m, ref_of(m, c), 0.f, 0.f, 0.f};
     float x = 0.f;
     for (int i = lane_id(); i < n; i += 32) {
         const Part p = parts[i];
@@ -744,8 +743,64 @@ __device__ __forceinline__ Soft hear(const Scale& c, const Part* parts, uint64_t
     x_token = warp_sum_f(x);
     s.s = warp_sum_f(s.s);
     if (ENT) s.q = warp_sum_f(s.q);
-    if (!came) s.s = NAN;
-    return s;
+    return true;
+}
+
+namespace fused {
+// What a CTA knows of its rows so far, in one register (there are 48), the same in every thread: which row of the two this is; not the first
+// row; exchanges so far, modulo 4; one exchange at least; second exchanges, modulo 2; a wait ran out
+enum : uint32_t { ODD = 1, LATER = 2, LIVE = 4, LIVES = 12, SEEN = 16, FAR = 32, GONE = 64 };
+}  // namespace fused
+
+// A row from its statistics (one thread): what its gradient is made of, and what the call wants of it.  The CTA waits for it, so what it needs
+// comes first.
+template <bool ENT>
+__device__ __forceinline__ void finish_row(const LossArgs& a, const RowOf& w, int row, int rank, bool first, const Scale& c, float x_token, const Soft& s, bool far,
+                                           GradRow& q, bool& zero) {
+    RowOf wr = w;
+    if (first) {
+        grid_dependency_wait();  // row_scale_kernel's results
+        wr.scale = a.row_scale[row];
+    }
+    const RowDone d = row_done<EPI_POLICY, ENT>(a, wr, c, x_token, s.m, s.e, s.s, s.q, far);
+    zero = d.g == 0.f && d.h == 0.f;
+    q = grad_row(d.m, far, d.s, d.ln_s, c, wr.inv_t, wr.token, d.g, d.h, d.entropy);
+    if (rank == 0) write_row<EPI_POLICY, ENT>(a, row, wr, d);
+}
+// A far row, whose sums are made again and exchanged once more, or a row of a CTA that is GONE.  The whole CTA, behind a barrier: a wait
+// that ran out says nothing about where the CTA's other warps are.
+template <typename T, bool ENT>
+__device__ __noinline__ uint32_t rare_row(const LossArgs& a, const RowOf& w, int row, int rank, int ctas, uint32_t st, Scale c, float x_token, const uint4* slice,
+                                          int cnt, bool have_edge, float x_edge, Part* parts, uint64_t* bar, const float& row_m, GradRow& q, bool& zero) {
+    using namespace fused;
+    const bool far = !(st & GONE);
+    const int n_parts = ctas * kRowWarps;
+    Soft s{0.f, ref_of(0.f, c), NAN, 0.f, NAN};
+    if (far) {  // (every CTA of the cluster has the same statistics)
+        const float m = row_m;
+        const Scale one{1.f, 0.f, FLT_MAX};
+        s = far_sums<T, ENT, kFusedThreads>(slice, cnt, have_edge, x_edge, m, c.hi, c.lo);
+        s.m = 0.f, s.e = ref_of(0.f, one);  // (references alike: nothing is scaled on the way)
+        tell<ENT>(s, 0.f, one, parts + 2 * n_parts + rank * kRowWarps + int(threadIdx.x >> 5), bar + 2, ctas);
+        bool out = false;
+        if (threadIdx.x < 32) {
+            float none;
+            out = !hear<ENT>(one, parts + 2 * n_parts, bar + 2, st & FAR ? 1 : 0, n_parts, a.wait_limit, s, none);
+            s.m = m;
+        }
+        st ^= FAR;
+        if (__syncthreads_or(out)) st |= GONE;
+    }
+    if (threadIdx.x == 0) {
+        if (st & GONE) {
+            grid_dependency_wait();  // (row_scale_kernel clears the word)
+            atomicExch(a.ticket + 1, 1u);
+            s = Soft{0.f, ref_of(0.f, c), NAN, 0.f, NAN};
+        }
+        finish_row<ENT>(a, w, row, rank, !(st & LATER), c, x_token, s, !(st & GONE), q, zero);
+    }
+    __syncthreads();
+    return st;
 }
 
 // The policy loss with its gradient.  The clusters stay and take rows in turn, each CTA holding its slice of a row in shared memory
@@ -754,6 +809,9 @@ __device__ __forceinline__ Soft hear(const Scale& c, const Part* parts, uint64_t
 // busy while the statistics of that row wait for it; several CTAs per SM fill each other's waits (the exchange of the statistics, the row's
 // scalars).  The statistics travel by stores that count on the receiver's mbarrier: a cluster barrier would hold every row until the
 // gradient's stores of the row before it are acknowledged.
+// Should a CTA's wait run out (it has a limit; nothing makes it run out but a store that is lost), the CTA says so in the workspace and is
+// GONE: this row and all its later ones are NaN, without another exchange, since the barriers' phases no longer
+// match.  The cluster's other CTAs then miss its statistics and go the same way.
 // What bounds it is the clusters' lockstep: every row waits for the slowest of its CTAs (1480 x 151936 bf16: DRAM at 55 % of the copy rate, the special
 // function units at 56 %, warps at the barrier a third of their time).  Measured beside it on 4096 x 151936 bf16, a third of the rows masked (501 us with
 // two launches and two reads, 487 to 503 here): one CTA an SM with a ring of slices and a warp of its own for the scalars, 770; tasks of
@@ -772,8 +830,9 @@ __global__ void __launch_bounds__(kFusedThreads, kFusedCtas) fused_kernel(const 
     const int clusters = int(gridDim.x / unsigned(ctas));
     const int n_parts = ctas * kRowWarps, my_part = rank * kRowWarps + (tid >> 5);
     Part* const parts = reinterpret_cast<Part*>(slice + per);
-    int row = int(blockIdx.x / unsigned(ctas)), lives = 0, fars = 0;
-    uint32_t limit = kWaitLimit;
+    int row = int(blockIdx.x / unsigned(ctas));
+    using namespace fused;
+    uint32_t st = 0;
     if (tid < 32) {
         const RowOf w = row_of<EPI>(a, row, false);
         if (tid == 0) {
@@ -792,13 +851,13 @@ __global__ void __launch_bounds__(kFusedThreads, kFusedCtas) fused_kernel(const 
     }
     cluster_barrier();  // every CTA's barriers are ready
 #pragma unroll 1
-    for (int k = 0; row < a.rows; ++k, row += clusters) {
-        const RowOf& w = s_row[k & 1];
+    for (; row < a.rows; st = (st ^ ODD) | LATER, row += clusters) {
+        const RowOf& w = s_row[st & ODD];
         const bool more = a.rows - row > clusters;
         if (more && tid >= NT - 32) {  // the next row's scalars; the wait is over at once but for the first row
             grid_dependency_wait();
             const RowOf r = row_of<EPI>(a, row + clusters, true);
-            if (tid == NT - 32) s_row[(k + 1) & 1] = r;
+            if (tid == NT - 32) s_row[(st ^ ODD) & ODD] = r;
         }
         const Slice<T> at(a, row, rank, per);
         const int cnt = at.cnt;
@@ -823,53 +882,31 @@ __global__ void __launch_bounds__(kFusedThreads, kFusedCtas) fused_kernel(const 
             float x_token = at.edge >= 0 && w.token == at.edge ? x_edge : 0.f;
             if (tok >= 0 && tok < cnt * E && (tok / E) % NT == tid) x_token = load_one(reinterpret_cast<const T*>(slice) + tok);
             x_token = warp_sum_f(x_token);
-            const int set = lives & 1;
-            tell<ENT>(s, x_token, c, parts + set * n_parts + my_part, &s_bar[set], ctas);
-            auto finish = [&](const Soft& r, bool far) {  // one thread: the CTA waits for it, so what it needs comes first
-                RowOf wr = w;
-                if (k == 0) {
-                    grid_dependency_wait();  // row_scale_kernel's results
-                    wr.scale = a.row_scale[row];
-                }
-                const RowDone d = row_done<EPI, ENT>(a, wr, c, x_token, r.m, r.e, r.s, r.q, far);
-                s_zero = d.g == 0.f && d.h == 0.f;
-                s_q = grad_row(d.m, far, d.s, d.ln_s, c, wr.inv_t, wr.token, d.g, d.h, d.entropy);
-                if (rank == 0) write_row<EPI, ENT>(a, row, wr, d);
-            };
-            if (tid < 32) {
-                s = hear<ENT>(c, parts + set * n_parts, &s_bar[set], uint32_t(lives >> 1) & 1, n_parts, limit, x_token);
-                if (tid == 0) {
+            const int set = st & LIVE ? 1 : 0;
+            const bool lose = a.lose_part && !(st & SEEN) && int(blockIdx.x) == ctas - 1 && tid < 32;
+            if (!(st & GONE) && !lose) tell<ENT>(s, x_token, c, parts + set * n_parts + my_part, &s_bar[set], ctas);
+            bool out = false;
+            if (tid < 32 && !(st & GONE)) {
+                out = !hear<ENT>(c, parts + set * n_parts, &s_bar[set], st & (2 * LIVE) ? 1 : 0, n_parts, a.wait_limit, s, x_token);
+                if (tid == 0 && !out) {
                     s_far = is_far(s.m, c), s_m = s.m;
-                    if (!is_far(s.m, c)) finish(s, false);
+                    if (!is_far(s.m, c)) finish_row<ENT>(a, w, row, rank, !(st & LATER), c, x_token, s, false, s_q, s_zero);
                 }
             }
-            ++lives;
-            __syncthreads();
-            if (s_far) {  // (every CTA of the cluster has the same statistics)
-                const float m = s_m;
-                const Scale one{1.f, 0.f, FLT_MAX};
-                s = far_sums<T, ENT, NT>(slice, cnt, at.edge >= 0, x_edge, m, c.hi, c.lo);
-                s.m = 0.f, s.e = ref_of(0.f, one);  // (references alike: nothing is scaled on the way)
-                tell<ENT>(s, 0.f, one, parts + 2 * n_parts + my_part, &s_bar[2], ctas);
-                if (tid < 32) {
-                    float none;
-                    s = hear<ENT>(one, parts + 2 * n_parts, &s_bar[2], uint32_t(fars) & 1, n_parts, limit, none);
-                    s.m = m;
-                    if (tid == 0) finish(s, true);
-                }
-                ++fars;
-                __syncthreads();
-            }
+            st = (st & ~LIVES) | ((st + LIVE) & LIVES) | SEEN;
+            if (__syncthreads_or(out)) st |= GONE;
+            if ((st & GONE) || s_far)
+                st = rare_row<T, ENT>(a, w, row, rank, ctas, st, c, x_token, slice, cnt, at.edge >= 0, x_edge, parts, s_bar, s_m, s_q, s_zero);
             zero = s_zero;
         } else {
             if (tid == 0) {
-                if (k == 0) grid_dependency_wait();
+                if (!(st & LATER)) grid_dependency_wait();
                 if (rank == 0) write_row<EPI, ENT>(a, row, w, RowDone{});
             }
             __syncthreads();
         }
         // (s_row of the next row, s_q and s_zero are in place; their next writes come after every thread has read them: s_row's behind the
-        // next row's barrier but one, the others' behind all warps' `tell` of the next row)
+        // next row's barrier but one, the others' behind all warps' `tell` of the next row, or behind its barrier if that is not heard)
         GradRow q{};
         if (!zero) q = s_q;
         T* dx = static_cast<T*>(a.dx) + int64_t(row) * a.ld_dx;
@@ -883,7 +920,7 @@ __global__ void __launch_bounds__(kFusedThreads, kFusedCtas) fused_kernel(const 
         const float x_mine = mine ? load_one(reinterpret_cast<const T*>(slice) + t) : 0.f;
         const uint4* next = nullptr;
         int refill = 0;
-        if (more && s_row[(k + 1) & 1].live) {
+        if (more && s_row[(st ^ ODD) & ODD].live) {
             const Slice<T> n(a, row + clusters, rank, per);
             next = n.body(), refill = n.cnt;
         }
@@ -915,7 +952,9 @@ __global__ void __launch_bounds__(kFusedThreads, kFusedCtas) fused_kernel(const 
         copies_commit();
     }
     copies_but<0>();
-    cluster_barrier();  // nobody leaves while another CTA's stores are under way to it
+    cluster_barrier();  // nobody leaves while another CTA has stores for it to send
+    if (st & GONE)      // ... or, where it did not wait for them, while they are under way
+        for (int i = 0; i < 200; ++i) __nanosleep(1000);
     if (rank == 0) last_sum(a.ticket, unsigned(clusters), a.row_term, a.rows, 1.0, a.loss);
 }
 
@@ -1217,7 +1256,7 @@ __device__ void row_scales(const LossArgs& a, int mean, double* sh) {
 __global__ void __launch_bounds__(kSmallThreads) row_scale_kernel(const __grid_constant__ LossArgs a, int mean) {
     __shared__ double sh[32];
     asm volatile("griddepcontrol.launch_dependents;");
-    if (threadIdx.x == 0) *a.ticket = 0;
+    if (threadIdx.x == 0) a.ticket[0] = a.ticket[1] = 0;
     row_scales(a, mean, sh);
 }
 
@@ -1426,7 +1465,8 @@ cudaError_t policy_launch(const LossArgs& a, int dtype, int mean, cudaStream_t s
 }
 
 cudaError_t preference_launch(const LossArgs& a, const PairArgs& p, int dtype, cudaStream_t st) {
-    cudaError_t e = cudaMemsetAsync(p.pairs > 0 ? static_cast<void*>(a.ticket) : static_cast<void*>(a.loss), 0, 4, st);  // (no pairs: the loss is 0)
+    cudaError_t e = cudaMemsetAsync(a.ticket, 0, 8, st);
+    if (e == cudaSuccess && p.pairs == 0) e = cudaMemsetAsync(a.loss, 0, 4, st);  // (no pairs: the loss is 0)
     if (e == cudaSuccess && a.rows > 0) e = forward_launch<EPI_PREF>(a, dtype, false, st);
     if (e != cudaSuccess) return e;
     if (p.pairs > 0) {
