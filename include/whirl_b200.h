@@ -328,7 +328,7 @@ int whirl_spec_accept_residual(const void* target, const void* draft, int dtype,
  * Training on sampled tokens: log-probabilities, losses and their gradients down to the logits.  No counterpart in the
  * reference, which only serves.
  *
- * Logits are rows [rows][n] whose row r starts at x + r * ld elements (ld >= n; a padded vocabulary leaves a gap), f32 or bf16,
+ * Logits are rows [rows][n] (rows <= WHIRL_MAX_LOSS_ROWS) whose row r starts at x + r * ld elements (ld >= n; a padded vocabulary leaves a gap), f32 or bf16,
  * aligned to their own size; rows aligned to 16 bytes are the fast case.  With z = x * inv_t (inv_t > 0: the scalar, or
  * inv_t_rows[row] where that is given):
  *     max = max_j x_j,  sum = sum_j exp((x_j - max) * inv_t)          (stats [rows][2], the convention of whirl_sample_rows)
@@ -340,6 +340,8 @@ int whirl_spec_accept_residual(const void* target, const void* draft, int dtype,
  * dx has the type of x, rows ld_dx apart; it may be x itself (with the same ld), and must not overlap x in another way.
  * Sums run in a fixed order: the same call gives the same bits.
  * ---------------------------------------------------------------------------------------------------------------- */
+
+#define WHIRL_MAX_LOSS_ROWS (1 << 30) /* of sequences too */
 
 /* logp [rows], stats [rows][2] and entropy [rows] of the given tokens; any of the three outputs may be null. */
 int whirl_token_logprobs(const void* x, int dtype, int rows, int n, int64_t ld, const int32_t* token, float inv_t,

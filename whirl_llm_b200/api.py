@@ -563,6 +563,13 @@ MEAN_SUM, MEAN_TOKENS, MEAN_SEQS = 0, 1, 2
 PREF_SIGMOID, PREF_HINGE, PREF_SQUARED = 0, 1, 2
 
 
+def _i32(v: int, name: str) -> int:
+    """v, refused where a C int does not hold it (ctypes would cut it)."""
+    if not -2 ** 31 <= v < 2 ** 31:
+        raise ValueError(f"{name} = {v} does not fit 32 bits")
+    return v
+
+
 def _loss_rows(x: torch.Tensor):
     """Logits [rows, n] whose rows may lie further apart than n (a padded vocabulary): (dtype, rows, n, ld)."""
     if not x.is_cuda:
@@ -573,7 +580,7 @@ def _loss_rows(x: torch.Tensor):
     s0, s1 = x.stride()
     if (n > 1 and s1 != 1) or (rows > 1 and s0 < n):
         raise ValueError(f"logits must be rows of consecutive elements that do not overlap, got strides {(s0, s1)}")
-    return _dtype(x), rows, n, (s0 if rows > 1 else n)
+    return _dtype(x), _i32(rows, "rows"), _i32(n, "n"), (s0 if rows > 1 else n)
 
 
 def _vec(t: Optional[torch.Tensor], name: str, dtype, shape, dev: int):
@@ -677,7 +684,7 @@ def policy_loss(x, token, adv, old_logp=None, ref_logp=None, weight=None, seq_st
     f32, i32, rs, dev = torch.float32, torch.int32, (rows,), x.get_device()
     if mean == MEAN_SEQS and (seq_start is None or seq_start.dim() != 1 or seq_start.numel() < 1):
         raise ValueError("policy_loss: MEAN_SEQS needs seq_start [seqs + 1]")
-    seqs = 0 if seq_start is None else seq_start.numel() - 1
+    seqs = 0 if seq_start is None else _i32(seq_start.numel() - 1, "seqs")
     p = PolicyParams(_vec(token, "token", i32, rs, dev), _vec(adv, "adv", f32, rs, dev), _vec(old_logp, "old_logp", f32, rs, dev),
                      _vec(ref_logp, "ref_logp", f32, rs, dev), _vec(weight, "weight", f32, rs, dev),
                      None if seq_start is None else _vec(seq_start, "seq_start", i32, (seqs + 1,), dev), seqs, mean,
@@ -737,7 +744,7 @@ def preference_loss(x, token, seq_start, ref_logp=None, weight=None, inv_t: floa
     f32, i32, rs, dev = torch.float32, torch.int32, (rows,), x.get_device()
     if seq_start.dim() != 1 or seq_start.numel() % 2 != 1:
         raise ValueError(f"preference_loss: seq_start is [2 * pairs + 1], got {tuple(seq_start.shape)}")
-    pairs = seq_start.numel() // 2
+    pairs = _i32(seq_start.numel() // 2, "pairs")
     p = PreferenceParams(_vec(token, "token", i32, rs, dev), _vec(seq_start, "seq_start", i32, (2 * pairs + 1,), dev),
                          _vec(ref_logp, "ref_logp", f32, rs, dev), _vec(weight, "weight", f32, rs, dev), _vec(inv_t_rows, "inv_t_rows", f32, rs, dev),
                          pairs, kind, int(average), inv_t, beta, smoothing, margin)
@@ -776,7 +783,8 @@ def block_tables_step(length, n_new, table, owned, free_ids, free_count, block_s
         raise ValueError("block_tables_step: table must be [seqs, max_blocks] on a CUDA device")
     i32, dev = torch.int32, table.get_device()
     seqs, width = table.shape
-    blocks, ss = free_ids.numel(), (seqs,)
+    blocks, ss = _i32(free_ids.numel(), "num_blocks"), (seqs,)
+    block_size, max_rows, seqs, width = (_i32(v, k) for v, k in ((block_size, "block_size"), (max_rows, "max_rows"), (seqs, "seqs"), (width, "max_blocks")))
     if rows is None:
         rows = StepRows(torch.empty(max_rows, dtype=torch.int64, device=dev), torch.empty(max_rows, dtype=i32, device=dev),
                         torch.empty(max_rows, dtype=i32, device=dev), torch.empty(seqs + 1, dtype=i32, device=dev),

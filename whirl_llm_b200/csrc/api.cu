@@ -472,6 +472,7 @@ namespace {
 int bad_rows(const char* who, const void* x, int dtype, int rows, int n, int64_t ld, const int32_t* token, float inv_t, const float* inv_t_rows) {
     const std::string w(who);
     if (rows < 0 || n <= 0 || bad_dtype(dtype) || ld < n) return fail(WHIRL_ERR_INVALID, (w + ": bad rows / n / dtype / ld").c_str());
+    if (rows > WHIRL_MAX_LOSS_ROWS) return fail(WHIRL_ERR_UNSUPPORTED, (w + ": rows above WHIRL_MAX_LOSS_ROWS").c_str());
     if (rows > 0 && (!x || !token)) return fail(WHIRL_ERR_INVALID, (w + ": x / token is null").c_str());
     if (reinterpret_cast<uintptr_t>(x) & (dtype == WHIRL_F32 ? 3 : 1)) return fail(WHIRL_ERR_INVALID, (w + ": x is not aligned to its type").c_str());
     if (!inv_t_rows && !(inv_t > 0.f && inv_t <= 3.4e38f)) return fail(WHIRL_ERR_INVALID, (w + ": inv_t has to be positive and finite").c_str());
@@ -542,6 +543,7 @@ int whirl_policy_loss(const void* x, int dtype, int rows, int n, int64_t ld, con
     if (rows > 0 && !p->adv) return fail(WHIRL_ERR_INVALID, "policy_loss: adv is null");
     if (p->mean != WHIRL_MEAN_SUM && p->mean != WHIRL_MEAN_TOKENS && p->mean != WHIRL_MEAN_SEQS) return fail(WHIRL_ERR_INVALID, "policy_loss: bad mean");
     if (p->mean == WHIRL_MEAN_SEQS && (p->seqs < 0 || !p->seq_start)) return fail(WHIRL_ERR_INVALID, "policy_loss: WHIRL_MEAN_SEQS needs seq_start / seqs");
+    if (p->mean == WHIRL_MEAN_SEQS && p->seqs > WHIRL_MAX_LOSS_ROWS) return fail(WHIRL_ERR_UNSUPPORTED, "policy_loss: seqs above WHIRL_MAX_LOSS_ROWS");
     if (!(p->clip_low >= 0.f) || !(p->clip_high >= 0.f) || !(p->dual_clip >= 0.f) || !(p->kl_coef == p->kl_coef) || !(p->ent_coef == p->ent_coef))
         return fail(WHIRL_ERR_INVALID, "policy_loss: a clip is negative, or a coefficient is NaN");
     if (o->dx)
