@@ -45,3 +45,41 @@ def test_binding_refuses_what_a_c_int_would_cut():
     for v in (2 ** 31, 2 ** 32 + 16, -2 ** 31 - 1):
         with pytest.raises(ValueError):
             api._i32(v, "block_size")
+
+
+def test_arrays_not_aligned_to_their_type():
+    """A load or store at such an address is a fault of the device; every array is looked at."""
+    from whirl_llm_b200 import api
+    ok = [P, 0, 4, 100, 100, P, 1.0, P, P, P, P, None]
+    for i in (0, 5, 7, 8, 9, 10):
+        a = list(ok)
+        a[i] = P + 2
+        s, msg = status("whirl_token_logprobs", *a)
+        assert s == 1 and "aligned" in msg, i
+    ok = [P, 0, 4, 100, 100, P, 1.0, P, P, P, P, P, P + 100000, 100, None]
+    for i in (0, 5, 7, 8, 9, 10, 11, 12):
+        a = list(ok)
+        a[i] += 2
+        s, msg = status("whirl_token_logprobs_grad", *a)
+        assert s == 1 and "aligned" in msg, i
+    for k in ("token", "adv", "old_logp", "ref_logp", "weight", "inv_t_rows"):
+        assert "aligned" in policy(**{k: P + 1})[1], k
+    assert "aligned" in policy(mean=2, seqs=1, seq_start=P + 2)[1]
+    for k in ("loss", "logp", "stats", "entropy", "kl", "row_loss", "g_logp", "row_scale"):
+        assert "aligned" in policy(out={k: P + 2})[1], k
+    assert "aligned" in policy(out=dict(dx=P + 100002, ld_dx=100))[1]
+    for k in ("token", "seq_start", "ref_logp", "weight", "inv_t_rows"):
+        assert "aligned" in preference(**{k: P + 2})[1], k
+    for k in ("loss", "pair_loss", "reward", "logp", "stats", "g_logp"):
+        assert "aligned" in preference(out={k: P + 2})[1], k
+
+    def blocks(length=P, n_new=P, **kw):
+        t = dict(table=P, owned=P, free_ids=P, free_count=P, seqs=4, max_blocks=8, num_blocks=16, block_size=16)
+        o = dict(slot=P, position=P, seq=P, row0=P, status=P, max_rows=32)
+        for k, v in kw.items():
+            (t if k in t else o)[k] = v
+        return status("whirl_block_tables_step", length, n_new, C.byref(api.BlockTables(**t)), C.byref(api.StepRowsOut(**o)), P, 1 << 40, None)
+    for k in ("length", "n_new", "table", "owned", "free_ids", "free_count", "position", "seq", "row0", "status"):
+        s, msg = blocks(**{k: P + 2})
+        assert s == 1 and "aligned" in msg, k
+    assert "aligned" in blocks(slot=P + 4)[1]

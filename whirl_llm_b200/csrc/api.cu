@@ -468,24 +468,35 @@ int whirl_merge_sample_rows_packed(const void* blocks, int shards, int rows, int
 
 namespace {
 
+// "who: what" without an allocation (an exception must not leave a C entry)
+int refuse(int code, const char* who, const char* what) {
+    char msg[160];
+    snprintf(msg, sizeof msg, "%s: %s", who, what);
+    return fail(code, msg);
+}
+// whether one of the arrays is not aligned to its type
+bool askew(std::initializer_list<const void*> arrays, uintptr_t size = 4) {
+    uintptr_t bits = 0;
+    for (const void* p : arrays) bits |= reinterpret_cast<uintptr_t>(p);
+    return bits & (size - 1);
+}
+
 // logits rows of the loss entry points
 int bad_rows(const char* who, const void* x, int dtype, int rows, int n, int64_t ld, const int32_t* token, float inv_t, const float* inv_t_rows) {
-    const std::string w(who);
-    if (rows < 0 || n <= 0 || bad_dtype(dtype) || ld < n) return fail(WHIRL_ERR_INVALID, (w + ": bad rows / n / dtype / ld").c_str());
-    if (rows > WHIRL_MAX_LOSS_ROWS) return fail(WHIRL_ERR_UNSUPPORTED, (w + ": rows above WHIRL_MAX_LOSS_ROWS").c_str());
-    if (rows > 0 && (!x || !token)) return fail(WHIRL_ERR_INVALID, (w + ": x / token is null").c_str());
-    if (reinterpret_cast<uintptr_t>(x) & (dtype == WHIRL_F32 ? 3 : 1)) return fail(WHIRL_ERR_INVALID, (w + ": x is not aligned to its type").c_str());
-    if (!inv_t_rows && !(inv_t > 0.f && inv_t <= 3.4e38f)) return fail(WHIRL_ERR_INVALID, (w + ": inv_t has to be positive and finite").c_str());
+    if (rows < 0 || n <= 0 || bad_dtype(dtype) || ld < n) return refuse(WHIRL_ERR_INVALID, who, "bad rows / n / dtype / ld");
+    if (rows > WHIRL_MAX_LOSS_ROWS) return refuse(WHIRL_ERR_UNSUPPORTED, who, "rows above WHIRL_MAX_LOSS_ROWS");
+    if (rows > 0 && (!x || !token)) return refuse(WHIRL_ERR_INVALID, who, "x / token is null");
+    if (askew({x}, dtype == WHIRL_F32 ? 4 : 2) || askew({token, inv_t_rows})) return refuse(WHIRL_ERR_INVALID, who, "x / token / inv_t_rows is not aligned to its type");
+    if (!inv_t_rows && !(inv_t > 0.f && inv_t <= 3.4e38f)) return refuse(WHIRL_ERR_INVALID, who, "inv_t has to be positive and finite");
     return WHIRL_OK;
 }
 int bad_dx(const char* who, const void* x, int dtype, int rows, int n, int64_t ld, const void* dx, int64_t ld_dx) {
-    const std::string w(who);
     const int64_t e = dtype == WHIRL_F32 ? 4 : 2;
-    if (ld_dx < n || (reinterpret_cast<uintptr_t>(dx) & (e - 1))) return fail(WHIRL_ERR_INVALID, (w + ": bad ld_dx, or dx is not aligned to its type").c_str());
+    if (ld_dx < n || askew({dx}, e)) return refuse(WHIRL_ERR_INVALID, who, "bad ld_dx, or dx is not aligned to its type");
     if (rows == 0 || (dx == x && ld_dx == ld)) return WHIRL_OK;
     const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(dx);
     if (a < b + uintptr_t(e * (int64_t(rows - 1) * ld_dx + n)) && b < a + uintptr_t(e * (int64_t(rows - 1) * ld + n)))
-        return fail(WHIRL_ERR_INVALID, (w + ": dx overlaps x without being it").c_str());
+        return refuse(WHIRL_ERR_INVALID, who, "dx overlaps x without being it");
     return WHIRL_OK;
 }
 
@@ -510,6 +521,7 @@ float* or_ws(float* user, void* ws, size_t off) { return user ? user : reinterpr
 int whirl_token_logprobs(const void* x, int dtype, int rows, int n, int64_t ld, const int32_t* token, float inv_t, const float* inv_t_rows,
                          float* logp, float* stats, float* entropy, void* stream) {
     if (const int st = bad_rows("token_logprobs", x, dtype, rows, n, ld, token, inv_t, inv_t_rows)) return st;
+    if (askew({logp, stats, entropy})) return fail(WHIRL_ERR_INVALID, "token_logprobs: an output is not aligned to its type");
     if (rows == 0 || (!logp && !stats && !entropy)) return WHIRL_OK;
     wb::LossArgs a{};
     a.x = x, a.ld = ld, a.rows = rows, a.n = n, a.token = token, a.inv_t = inv_t, a.inv_t_rows = inv_t_rows;
@@ -524,6 +536,7 @@ int whirl_token_logprobs_grad(const void* x, int dtype, int rows, int n, int64_t
     if (const int st = bad_rows("token_logprobs_grad", x, dtype, rows, n, ld, token, inv_t, inv_t_rows)) return st;
     if (rows == 0) return WHIRL_OK;
     if (!stats || !g_logp || !dx || (g_entropy && !entropy)) return fail(WHIRL_ERR_INVALID, "token_logprobs_grad: stats / g_logp / dx is null, or g_entropy without entropy");
+    if (askew({stats, entropy, g_logp, g_entropy})) return fail(WHIRL_ERR_INVALID, "token_logprobs_grad: an input is not aligned to its type");
     if (const int st = bad_dx("token_logprobs_grad", x, dtype, rows, n, ld, dx, ld_dx)) return st;
     wb::LossArgs a{};
     a.x = x, a.ld = ld, a.rows = rows, a.n = n, a.token = token, a.inv_t = inv_t, a.inv_t_rows = inv_t_rows;
@@ -540,6 +553,9 @@ int whirl_policy_loss(const void* x, int dtype, int rows, int n, int64_t ld, con
                       size_t ws_bytes, void* stream) {
     if (!p || !o || !o->loss) return fail(WHIRL_ERR_INVALID, "policy_loss: params / out / loss is null");
     if (const int st = bad_rows("policy_loss", x, dtype, rows, n, ld, p->token, p->inv_t, p->inv_t_rows)) return st;
+    if (askew({p->adv, p->old_logp, p->ref_logp, p->weight, p->seq_start}) ||
+        askew({o->loss, o->logp, o->stats, o->entropy, o->kl, o->row_loss, o->g_logp, o->row_scale}))
+        return fail(WHIRL_ERR_INVALID, "policy_loss: an array is not aligned to its type");
     if (rows > 0 && !p->adv) return fail(WHIRL_ERR_INVALID, "policy_loss: adv is null");
     if (p->mean != WHIRL_MEAN_SUM && p->mean != WHIRL_MEAN_TOKENS && p->mean != WHIRL_MEAN_SEQS) return fail(WHIRL_ERR_INVALID, "policy_loss: bad mean");
     if (p->mean == WHIRL_MEAN_SEQS && (p->seqs < 0 || !p->seq_start)) return fail(WHIRL_ERR_INVALID, "policy_loss: WHIRL_MEAN_SEQS needs seq_start / seqs");
@@ -579,6 +595,8 @@ int whirl_preference_loss(const void* x, int dtype, int rows, int n, int64_t ld,
                           void* ws, size_t ws_bytes, void* stream) {
     if (!p || !o || !o->loss) return fail(WHIRL_ERR_INVALID, "preference_loss: params / out / loss is null");
     if (const int st = bad_rows("preference_loss", x, dtype, rows, n, ld, p->token, p->inv_t, p->inv_t_rows)) return st;
+    if (askew({p->seq_start, p->ref_logp, p->weight, o->loss, o->pair_loss, o->reward, o->logp, o->stats, o->g_logp}))
+        return fail(WHIRL_ERR_INVALID, "preference_loss: an array is not aligned to its type");
     if (p->pairs < 0 || p->pairs > (1 << 29) || !p->seq_start) return fail(WHIRL_ERR_INVALID, "preference_loss: bad pairs, or seq_start is null");
     if (p->kind != WHIRL_PREF_SIGMOID && p->kind != WHIRL_PREF_HINGE && p->kind != WHIRL_PREF_SQUARED) return fail(WHIRL_ERR_INVALID, "preference_loss: bad kind");
     if (!(p->beta > 0.f && p->beta <= 3.4e38f) || !(p->smoothing >= 0.f && p->smoothing <= 1.f) || !(p->margin == p->margin))
@@ -626,6 +644,8 @@ int whirl_block_tables_step(const int32_t* length, const int32_t* n_new, const w
         return fail(WHIRL_ERR_INVALID, "block_tables_step: free_count / free_ids / row0 / slot is null");
     if (t->seqs > 0 && (!length || !n_new || !t->owned || !r->status || (t->max_blocks > 0 && !t->table)))
         return fail(WHIRL_ERR_INVALID, "block_tables_step: length / n_new / owned / status / table is null");
+    if (askew({length, n_new, t->table, t->owned, t->free_ids, t->free_count, r->position, r->seq, r->row0, r->status}) || askew({r->slot}, 8))
+        return fail(WHIRL_ERR_INVALID, "block_tables_step: an array is not aligned to its type");
     if (!ws || ws_bytes < whirl_block_workspace_bytes(t->seqs)) return fail(WHIRL_ERR_WORKSPACE, "block_tables_step: workspace missing or too small (whirl_block_workspace_bytes)");
     void* base = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(ws) + 255) & ~uintptr_t(255));
     const cudaError_t e = wb::block_tables_launch(length, n_new, *t, *r, base, sm_count(), static_cast<cudaStream_t>(stream));
