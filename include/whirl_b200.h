@@ -337,7 +337,8 @@ int whirl_spec_accept_residual(const void* target, const void* draft, int dtype,
  * -inf alone, has no distribution: its outputs and its gradient are NaN.
  * A row COUNTS when its token lies in [0, n), its weight (where the call has weights) is > 0 and, in the preference loss, it
  * lies inside a sequence.  Rows that do not count are not read: their outputs and statistics are 0, and so is their row of dx.
- * dx has the type of x, rows ld_dx apart; it may be x itself (with the same ld), and must not overlap x in another way.
+ * dx has the type of x, rows ld_dx apart; it may be x itself (with the same ld), and must not overlap x in another way (with the
+ * same ld the two may be columns of one buffer, with another the memory from first to last row counts).
  * Sums run in a fixed order: the same call gives the same bits.
  * ---------------------------------------------------------------------------------------------------------------- */
 

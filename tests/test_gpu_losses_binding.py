@@ -12,3 +12,23 @@ def test_sizes_that_a_c_int_would_cut():
         api.block_tables_step(e(1), e(1), e(1, 4), e(1), e(5), e(1), block_size=2 ** 32 + 16, max_rows=7)
     with pytest.raises(ValueError, match="max_rows"):
         api.block_tables_step(e(1), e(1), e(1, 4), e(1), e(5), e(1), block_size=16, max_rows=2 ** 32 + 7)
+
+
+@pytest.mark.parametrize("n,dtype", [(1003, torch.float32), (1000, torch.bfloat16), (40002, torch.float32), (40000, torch.bfloat16)])
+def test_dx_beside_x_in_one_buffer(n, dtype):
+    from whirl_llm_b200 import api
+    rows = 50
+    g = torch.Generator(device="cuda").manual_seed(n)
+    buf = torch.randn((rows, 2 * n + 8), device="cuda", generator=g).to(dtype)
+    x, dx, rest = buf[:, :n], buf[:, n + 8:], buf[:, n: n + 8].clone()
+    token = torch.randint(0, n, (rows,), device="cuda", generator=g, dtype=torch.int32)
+    adv = torch.randn(rows, device="cuda", generator=g)
+    x0 = x.clone()
+    want = api.policy_loss(x, token, adv).dx
+    r = api.policy_loss(x, token, adv, dx=dx)
+    assert torch.equal(r.dx, want) and torch.equal(x, x0) and torch.equal(buf[:, n: n + 8], rest)
+    s = api.token_logprobs(x, token)
+    want = api.token_logprobs_grad(x, token, s.stats, adv)
+    assert torch.equal(api.token_logprobs_grad(x, token, s.stats, adv, dx=dx), want) and torch.equal(x, x0) and torch.equal(buf[:, n: n + 8], rest)
+    with pytest.raises(api.WhirlError, match="overlaps"):
+        api.policy_loss(x, token, adv, dx=buf[:, n - 1: 2 * n - 1])

@@ -83,3 +83,16 @@ def test_arrays_not_aligned_to_their_type():
         s, msg = blocks(**{k: P + 2})
         assert s == 1 and "aligned" in msg, k
     assert "aligned" in blocks(slot=P + 4)[1]
+
+
+def test_dx_beside_x_in_one_buffer():
+    """Columns of one buffer do not overlap; one element in common does."""
+    def grad(x, dx, ld=200, ld_dx=200, n=100, rows=4):
+        return status("whirl_token_logprobs_grad", x, 0, rows, n, ld, P, 1.0, None, P, None, P, None, dx, ld_dx, None)
+    for x, dx in ((P, P + 400), (P + 400, P), (P, P + 400 + 800), (P + 400, P + 800)):
+        s, msg = grad(x, dx)
+        assert "overlaps" not in msg or s != 1, (x, dx)          # (no device here: the launch itself fails)
+    for x, dx in ((P, P + 396), (P + 396, P), (P, P + 404), (P, P + 800), (P, P + 4), (P + 4, P)):
+        s, msg = grad(x, dx)
+        assert s == 1 and "overlaps" in msg, (x, dx)
+    assert grad(P, P + 400, ld_dx=201)[0] == 1                   # (rows drift into one another)

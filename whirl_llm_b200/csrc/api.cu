@@ -495,6 +495,10 @@ int bad_dx(const char* who, const void* x, int dtype, int rows, int n, int64_t l
     if (ld_dx < n || askew({dx}, e)) return refuse(WHIRL_ERR_INVALID, who, "bad ld_dx, or dx is not aligned to its type");
     if (rows == 0 || (dx == x && ld_dx == ld)) return WHIRL_OK;
     const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(dx);
+    if (ld == ld_dx) {  // columns of one buffer side by side: every row of the one lies between two of the other
+        const int64_t d = int64_t(b - a) / e % ld, gap = d < 0 ? d + ld : d;
+        if (gap >= n && gap <= ld - n) return WHIRL_OK;
+    }
     if (a < b + uintptr_t(e * (int64_t(rows - 1) * ld_dx + n)) && b < a + uintptr_t(e * (int64_t(rows - 1) * ld + n)))
         return refuse(WHIRL_ERR_INVALID, who, "dx overlaps x without being it");
     return WHIRL_OK;
