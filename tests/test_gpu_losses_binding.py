@@ -32,3 +32,17 @@ def test_dx_beside_x_in_one_buffer(n, dtype):
     assert torch.equal(api.token_logprobs_grad(x, token, s.stats, adv, dx=dx), want) and torch.equal(x, x0) and torch.equal(buf[:, n: n + 8], rest)
     with pytest.raises(api.WhirlError, match="overlaps"):
         api.policy_loss(x, token, adv, dx=buf[:, n - 1: 2 * n - 1])
+
+
+def test_gradient_of_rows_far_apart_takes_no_more_than_its_rows():
+    """The last position of every sequence of a batch: rows a whole sequence of logits apart."""
+    from whirl_llm_b200 import api
+    for n in (5000, 5003):
+        x = torch.randn((6, 100, n), device="cuda")[:, -1]
+        token = torch.arange(6, device="cuda", dtype=torch.int32)
+        adv = torch.ones(6, device="cuda")
+        s = api.token_logprobs(x, token)
+        for dx in (api.policy_loss(x, token, adv).dx, api.token_logprobs_grad(x, token, s.stats, -adv / 6),
+                   api.preference_loss(x, token, torch.tensor([0, 3, 6], dtype=torch.int32, device="cuda")).dx):
+            assert dx.shape == x.shape and dx.untyped_storage().nbytes() <= 4 * 6 * (n + 4)
+        assert torch.equal(api.policy_loss(x, token, adv).dx, api.policy_loss(x, token, adv, dx=torch.empty_like(x)).dx)

@@ -594,10 +594,11 @@ def _vec(t: Optional[torch.Tensor], name: str, dtype, shape, dev: int):
 
 
 def _grad_out(x: torch.Tensor, dx: Optional[torch.Tensor], ld: int) -> torch.Tensor:
-    """dx, checked; a new one has x's row pitch."""
+    """dx, checked; a new one has rows as x has them to 16 bytes (the kernels' fast case), and no more of a gap than that takes."""
     if dx is None:
         rows, n = x.shape
-        return torch.empty((rows, ld), dtype=x.dtype, device=x.device)[:, :n] if ld != n else torch.empty((rows, n), dtype=x.dtype, device=x.device)
+        gap = (ld - n) % (16 // x.element_size())
+        return torch.empty((rows, n + gap), dtype=x.dtype, device=x.device)[:, :n] if gap else torch.empty((rows, n), dtype=x.dtype, device=x.device)
     if dx.dtype != x.dtype or dx.device != x.device or dx.shape != x.shape:
         raise TypeError(f"dx: want {x.dtype} {tuple(x.shape)} on {x.device}, got {dx.dtype} {tuple(dx.shape)} on {dx.device}")
     return dx
