@@ -46,3 +46,33 @@ def test_gradient_of_rows_far_apart_takes_no_more_than_its_rows():
                    api.preference_loss(x, token, torch.tensor([0, 3, 6], dtype=torch.int32, device="cuda")).dx):
             assert dx.shape == x.shape and dx.untyped_storage().nbytes() <= 4 * 6 * (n + 4)
         assert torch.equal(api.policy_loss(x, token, adv).dx, api.policy_loss(x, token, adv, dx=torch.empty_like(x)).dx)
+
+
+def test_gradient_in_place_is_seen_by_autograd():
+    """A graph that kept the logits for its own backward pass must not use what dx = x put there."""
+    from whirl_llm_b200 import api
+    n = 2000
+    token = torch.arange(8, device="cuda", dtype=torch.int32)
+    adv = torch.ones(8, device="cuda")
+    starts = torch.tensor([0, 4, 8], dtype=torch.int32, device="cuda")
+
+    def grads(y):
+        d = y.detach()
+        s = api.token_logprobs(d, token)
+        return (lambda dx: api.policy_loss(d, token, adv, dx=dx).dx, lambda dx: api.preference_loss(d, token, starts, dx=dx).dx,
+                lambda dx: api.token_logprobs_grad(d, token, s.stats, adv, dx=dx))
+    for k in range(3):
+        w = torch.randn((8, n), device="cuda", requires_grad=True)
+        y = torch.tanh(w)                       # tanh keeps its result
+        dx = grads(y)[k](y.detach())
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            y.backward(dx)
+        w = torch.randn((8, n), device="cuda", requires_grad=True)
+        y = w * 2.0                             # a product by a number keeps nothing
+        want = grads(y)[k](None).clone()
+        y.backward(grads(y)[k](y.detach()))
+        assert torch.equal(w.grad, 2.0 * want)
+        out = torch.empty_like(y)
+        before = out._version
+        grads(torch.tanh(w))[k](out)
+        assert out._version > before

@@ -601,6 +601,7 @@ def _grad_out(x: torch.Tensor, dx: Optional[torch.Tensor], ld: int) -> torch.Ten
         return torch.empty((rows, n + gap), dtype=x.dtype, device=x.device)[:, :n] if gap else torch.empty((rows, n), dtype=x.dtype, device=x.device)
     if dx.dtype != x.dtype or dx.device != x.device or dx.shape != x.shape:
         raise TypeError(f"dx: want {x.dtype} {tuple(x.shape)} on {x.device}, got {dx.dtype} {tuple(dx.shape)} on {dx.device}")
+    torch.autograd.graph.increment_version(dx)  # (autograd does not see the kernels' writes: a graph that kept dx, or x where they are one, has to)
     return dx
 
 
