@@ -248,3 +248,18 @@ def test_errors_of_many_rows_do_not_add_up(rows, n, dtype, inv_t):
     r = api.preference_loss(x, token.int(), starts, ref_logp=z.float(), inv_t=inv_t, beta=1.0)   # what is left is small: no rounding of its own
     want = (z - z.float().double()).sum()
     assert abs(r.reward[0, 0].double() - want) < 1e-8 * rows + 6 * ref.EPS32 * math.sqrt(rows), ((r.reward[0, 0].double() - want) / rows).item()
+
+
+@pytest.mark.parametrize("n", [1003, 20001, 1000003])
+def test_policy_inputs_that_are_nan(n):
+    """An advantage, an old or a reference log-probability that is NaN: the row's loss and gradient are NaN, nobody else's."""
+    from whirl_llm_b200 import api
+    x, _, token, _, (_, _, logp, _), adv, old, rf, _ = policy_inputs(6, n, "f32", seed=8, masked=0.0)
+    want = api.policy_loss(x, token.cuda(), adv.cuda(), old.cuda(), rf.cuda(), mean=api.MEAN_SUM, kl_coef=0.1, dual_clip=2.0)
+    adv, old, rf = adv.clone(), old.clone(), rf.clone()
+    adv[1], old[2], rf[4] = math.nan, math.nan, math.nan
+    r = api.policy_loss(x, token.cuda(), adv.cuda(), old.cuda(), rf.cuda(), mean=api.MEAN_SUM, kl_coef=0.1, dual_clip=2.0)
+    bad = torch.tensor([1, 2, 4])
+    good = torch.tensor([0, 3, 5])
+    assert torch.isnan(r.row_loss[bad]).all() and torch.isnan(r.g_logp[bad]).all() and torch.isnan(r.dx[bad]).all() and torch.isnan(r.loss)
+    assert torch.equal(r.row_loss[good], want.row_loss[good]) and torch.equal(r.dx[good], want.dx[good]) and torch.equal(r.logp, want.logp)

@@ -446,7 +446,8 @@ __device__ __forceinline__ PolicyRow policy_row(const LossArgs& a, const RowOf& 
     float pg = takes_plain ? -plain : -clipped;
     p.dlogp = takes_plain && free_d ? -plain : 0.f;
     if (a.dual_clip > 0.f && adv < 0.f && pg > -a.dual_clip * adv) pg = -a.dual_clip * adv, p.dlogp = 0.f;
-    if (logp != logp) pg = p.dlogp = float(logp);  // (a ratio of 1 does not see it)
+    if (logp != logp) pg = float(logp);  // (a ratio of 1 does not see it)
+    if (pg != pg) p.dlogp = pg;          // (no clip binds where the loss is NaN: an advantage or an old log-probability that is)
     p.kl = 0.f;
     if (a.ref_logp) {
         float k = float(double(w.ref_logp) - logp);
