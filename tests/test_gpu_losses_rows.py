@@ -263,3 +263,29 @@ def test_policy_inputs_that_are_nan(n):
     good = torch.tensor([0, 3, 5])
     assert torch.isnan(r.row_loss[bad]).all() and torch.isnan(r.g_logp[bad]).all() and torch.isnan(r.dx[bad]).all() and torch.isnan(r.loss)
     assert torch.equal(r.row_loss[good], want.row_loss[good]) and torch.equal(r.dx[good], want.dx[good]) and torch.equal(r.logp, want.logp)
+
+
+@pytest.mark.parametrize("n", [1003, 20001, 60000])
+def test_largest_inv_t(n):
+    """Temperatures of next to nothing: the maxima share the row, wherever they lie."""
+    from whirl_llm_b200 import api
+    x = -1.0 - torch.rand((4, n))
+    x[:, 5], x[:, n - 2], x[:, 700] = 0.0, 0.0, 0.0
+    x[1] += 5.0
+    x[2] -= 3.0
+    x[3, ::2] = -math.inf
+    x[3, 5] = x[3, n - 2] = x[3, 700] = 0.0
+    token = torch.tensor([5, 700, 5, n - 2], dtype=torch.int32)
+    for inv_t in (3.3e38, 2e38, 1e30):
+        it = ones(inv_t, 4)
+        m, s, lp, h = ref.row_stats(x.double(), it)
+        r = api.token_logprobs(x.cuda(), token.cuda(), inv_t=inv_t, want_entropy=True)
+        assert torch.allclose(r.logp.cpu(), torch.full((4,), -math.log(3.0)), atol=1e-6) and (r.stats[:, 1] == 3).all()
+        close(r.entropy, h, ref.entropy_tol(n), "entropy")
+        g = torch.ones(4) / np.float32(inv_t)
+        p = api.policy_loss(x.cuda(), token.cuda(), -g.cuda(), inv_t=inv_t, mean=api.MEAN_SUM)
+        for dx in (api.token_logprobs_grad(x.cuda(), token.cuda(), r.stats, g.cuda(), inv_t=inv_t), p.dx):
+            want = torch.zeros((4, n))
+            want[:, [5, 700, n - 2]] = -1 / 3
+            want[torch.arange(4), token.long()] = 2 / 3
+            assert torch.allclose(dx.cpu(), want, atol=1e-6)
