@@ -455,7 +455,8 @@ int whirl_preference_loss(const void* x, int dtype, int rows, int n, int64_t ld,
  * The blocks at hand are the free ones and those that this step gives back: a sequence inside max_rows that owns more than its target
  * gives back table[s][target .. owned), pushed on the stack in the sequences' order.  New blocks come from the stack's top, in
  * the sequences' order.  An OK sequence owns its target afterwards; any other keeps its blocks and length and gets no rows.
- * Entries of table behind owned and of free_ids behind free_count are left as they were.
+ * Entries of table behind owned are left as they were; those of free_ids behind the new free_count hold what the step pushed there
+ * and took again, and are otherwise left as they were.
  * Rows: row0[s] = the first row of sequence s, row0[seqs] = their number; row r of sequence s at position p = length[s] + r -
  * row0[s] gets slot[r], position[r] = p and seq[r] = s.  The rows from row0[seqs] to max_rows (a padded batch) get slot -1,
  * position 0, seq -1.

@@ -6,10 +6,10 @@
 // exponentials times their exponents, and brings them to a new reference when a larger logit comes along; partial results merge
 // the same way.  The gradient is one elementwise pass over the row.
 //
-//   forward_kernel     statistics of long rows, a cluster of 1 to 16 CTAs each      1024 x 262144 f32: 158 us, 6.8 TB/s
-//   grad_kernel        gradient of long rows from given statistics                  1024 x 262144 bf16: 170 us, 6.3 TB/s
-//   fused_kernel       policy loss: both at once, the row held in shared memory     4096 x 151936 bf16, a third masked: 500 us, 4.1 TB/s
-//   small_rows_kernel, small_grad_kernel   the same for short rows, a warp each     60000 x 2000 bf16: 80, 181 and 88 us
+//   forward_kernel     statistics of long rows, a cluster of 1 to 16 CTAs each      1024 x 262144 f32: 165 us, 6.5 TB/s; bf16: 93 us, 5.8 TB/s
+//   grad_kernel        gradient of long rows from given statistics                  1024 x 262144 bf16: 175 us, 6.1 TB/s
+//   fused_kernel       policy loss: both at once, the row held in shared memory     4096 x 151936 bf16, a third masked: 503 us, 4.1 TB/s
+//   small_rows_kernel, small_grad_kernel   the same for short rows, a warp each     60000 x 2000 bf16: 76, 181 and 88 us
 //
 // All are bound by memory in principle (a logit costs about 7 instructions for the statistics, 5 for the gradient, and one
 // exponential of the special function unit for each).  The preference loss needs its sequences' sums before any gradient: forward_kernel,
@@ -288,7 +288,7 @@ constexpr double kLn2 = 0.6931471805599453;
 // with one correction each, and 64 bits where a last bit would add up over a sequence.  (The library's log, exp and expm1 in 64
 // bits, and the divisions around them, took 2.7 us a row.)
 // log of a sum > 0 (NaN without one): 2^k f with f in [sqrt 1/2, sqrt 2), log f = 2 atanh z, z = (f - 1) / (f + 1), |z| < 0.172; the
-// terms left out are below 1e-13.  (lg2.approx and a step of Newton's method with ex2.approx is low by 4e-8.)
+// first term left out, 2 z^15 / 15, is below 5e-13.  (lg2.approx and a step of Newton's method with ex2.approx is low by 4e-8.)
 __device__ __forceinline__ double ln_of(double d) {
     if (!(d > 1e-300 && d < 1e300)) return NAN;
     const int hi = __double2hiint(d), k = (hi - 0x3fe6a09e) >> 20;
@@ -300,7 +300,8 @@ __device__ __forceinline__ double ln_of(double d) {
     t = fma(t, y, 1.0 / 11.0), t = fma(t, y, 1.0 / 9.0), t = fma(t, y, 1.0 / 7.0), t = fma(t, y, 1.0 / 5.0), t = fma(t, y, 1.0 / 3.0);
     return fma(double(k), kLn2, 2.0 * z * fma(t, y, 1.0));
 }
-// exp of |d| <= 20, the exponent's rounding errors taken out
+// exp of |d| <= 20 (shifted: of 0.35), the exponent's rounding errors taken out; what is left is ex2.approx's own, up to 1.4e-7 of the result.  The
+// ratio of a policy row and its kl are made of it: as exact as the f32 outputs that they become.
 __device__ __forceinline__ float exp_of(float d) {
     const float hi = d * kLog2e, lo = fmaf(d, kLog2e, -hi) + d * 1.92596299e-8f;  // (log2 e = kLog2e + 1.926e-8)
     const float e = ex2_approx(hi);
@@ -818,7 +819,7 @@ __device__ __noinline__ uint32_t rare_row(const LossArgs& a, const RowOf& w, int
 // match.  The cluster's other CTAs then miss its statistics and go the same way.
 // What bounds it is the clusters' lockstep: every row waits for the slowest of its CTAs (1480 x 151936 bf16: DRAM at 55 % of the copy rate, the special
 // function units at 56 %, warps at the barrier a third of their time).  Measured beside it on 4096 x 151936 bf16, a third of the rows masked (501 us with
-// two launches and two reads, 487 to 503 here): one CTA an SM with a ring of slices and a warp of its own for the scalars, 770; tasks of
+// two launches and two reads, 500 to 505 here): one CTA an SM with a ring of slices and a warp of its own for the scalars, 770; tasks of
 // statistics and of gradients drawn from one counter, the second read from L2, 520 to 600; 384 or 512 threads, 534 and 554.
 template <typename T, bool ENT>
 __global__ void __launch_bounds__(kFusedThreads, kFusedCtas) fused_kernel(const __grid_constant__ LossArgs a, int per) {
@@ -968,7 +969,7 @@ __global__ void __launch_bounds__(kFusedThreads, kFusedCtas) fused_kernel(const 
 
 // A row of up to 8 KB fits the registers of one warp: it is read once, its statistics need no shared memory and no barrier, and (GRAD) its
 // gradient is written from the registers.  The kernels above spend 4 to 7 us of a CTA on a row however short it is: 8000 rows of
-// 2000 bf16 logits, policy loss with gradient, took 72 us with fused_kernel and take 32 here.
+// 2000 bf16 logits, policy loss with gradient, took 72 us with fused_kernel and take 33 here.
 constexpr int kSmallRowThreads = 256, kSmallVectors = 16;  // vectors a lane, at most
 
 // writes the gradient of a row's vectors from `first` on that a warp has in registers (q of zeros: zeros)
@@ -1366,7 +1367,7 @@ int vectors_of(int n, int dtype) { return int((int64_t(n) * (dtype == WHIRL_F32 
 
 // A warp per row: where it holds the whole row in its registers; or, where a row is read and done with piece by piece, for rows of up to 32 KB
 // (statistics) or 16 KB (gradient) of which there are enough to fill the GPU with warps.  20000 rows of 4200 bf16 logits: statistics by CTAs 120 us, by warps
-// 64; gradient 97 and 75.  3000 rows of 16000: statistics 31 by warps and 33 by CTAs, gradient 48 and 36.
+// 62; gradient 97 and 76.  3000 rows of 16000: statistics 31 by warps and 33 by CTAs, gradient 48 and 36.
 bool is_small(int n, int dtype) { return vectors_of(n, dtype) <= 32 * kSmallVectors; }
 bool is_short(const LossArgs& a, int dtype, int vectors) { return is_small(a.n, dtype) || (a.rows >= 148 * 16 && vectors_of(a.n, dtype) <= vectors); }
 template <typename T, int EPI, bool ENT, bool GRAD>
